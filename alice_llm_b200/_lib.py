@@ -61,6 +61,16 @@ SIGNATURES = {
     "alice_dequantize": (C.c_int32, [_vp, _vp, _vp]),
     "alice_plan_query": (C.c_int32, [_vp, _vp, C.c_int32, C.c_int32, _vp, C.c_uint32]),
     "alice_batch_plan": (C.c_int32, [_vp, _vp, C.c_int32, C.c_uint32, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
+    "alice_kv4_create": (C.c_int32, [_vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _pp]),
+    "alice_kv4_free": (C.c_int32, [_vp]),
+    "alice_kv4_batch_create": (C.c_int32, [_vp, _vp, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, _pp]),
+    "alice_kv4_batch_free": (C.c_int32, [_vp]),
+    "alice_kv4_batch_set": (C.c_int32, [_vp, C.c_uint32, _vp, _vp, _vp, C.c_uint32]),
+    "alice_kv4_batch_check": (C.c_int32, [C.c_uint32] * 6 + [_vp, _vp, _vp, C.c_uint32]),
+    "alice_kv4_append": (C.c_int32, [_vp, _vp, _vp, _vp, C.c_size_t, _vp, C.c_size_t, _vp, C.c_uint32, C.c_uint32]),
+    "alice_kv4_read": (C.c_int32, [_vp, _vp, _vp, _vp, C.c_size_t, _vp, C.c_size_t]),
+    "alice_kv4_attention": (C.c_int32, [_vp, _vp, _vp, _vp, C.c_size_t, _vp, C.c_size_t, _vp, C.c_uint32, C.c_uint32, C.c_float]),
+    "alice_log_probs": (C.c_int32, [_vp, _vp, C.c_uint32, C.c_uint32, C.c_size_t, _vp, _vp, _vp, _vp, C.c_uint32, _vp, _vp]),
     "alice_model_create": (C.c_int32, [_vp, _vp, _vp, _vp, _vp, _vp, _pp]),
     "alice_model_destroy": (C.c_int32, [_vp]),
     "alice_model_forward": (C.c_int32, [_vp, C.c_uint32]),

@@ -16,6 +16,8 @@ constexpr int KERR_WAIT_PARTIALS = 3;  // row finalizer waiting for the other wa
 constexpr int KERR_WAIT_EMPTY = 4;     // producer waiting for a stage to be released
 constexpr int KERR_WAIT_GRID = 5;      // grid-wide barrier
 constexpr int KERR_WAIT_PEER = 6;      // rows another GPU pushes into this GPU's vector (tensor parallel)
+// (7 to 9: waits of the layer-stack models' kernels)
+constexpr int KERR_KV4_BATCH = 10;     // no wait: a captured call over the 4-bit cache and the batch at its replay do not fit
 
 // A wait that has not been satisfied after this many SM clock cycles (about one second) gives
 // up, records KERR_WAIT_TIMEOUT and lets the CTA drain and return instead of spinning forever.

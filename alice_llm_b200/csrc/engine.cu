@@ -184,6 +184,8 @@ int32_t alice_sync(alice_engine* e) {
         static const char* const what[] = {"?", "unspecified wait", "weights did not land in shared memory", "partial sums of a row", "stage release",
                                            "grid barrier", "rows from a tensor-parallel peer", "operands or accumulators of a tensor-core product", "a tile of cached keys and values", "operands or weights of tensor-core attention"};
         const int code = st & 0xff;
+        if (st == KERR_KV4_BATCH)
+            return fail(ALICE_E_KERNEL, "alice_sync: a captured call over a 4-bit cache met a batch that does not fit its buffers, tables, pages or rows a job; it did nothing");
         return fail(ALICE_E_KERNEL, "alice_sync: a kernel wait ran out of its cycle budget (status %d: %s); results of the queued work are void",
                     st, code >= 1 && code <= 9 ? what[code] : what[0]);
     }

@@ -104,6 +104,63 @@ class Q8KBuffer:
             pass
 
 
+class Kv4Cache:
+    """Keys and values of one layer in pages, held in 4 bits (PagedKvCache, src/llama3.rs:5085, keeps them in f32)."""
+
+    def __init__(self, engine, handle, pages, page_tokens, kv_heads, head_dim):
+        self.engine, self._h, self.pages, self.page_tokens, self.kv_heads, self.head_dim = engine, handle, pages, page_tokens, kv_heads, head_dim
+        engine._children.add(self)
+
+    def free(self):
+        if self._h:
+            _lib.load().alice_kv4_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _kv4_step(past, tokens, tables):
+    past, tokens, tables = _np(past, np.uint32).reshape(-1), _np(tokens, np.uint32).reshape(-1), _np(tables, np.uint32)
+    if tables.ndim != 2 or past.size != tokens.size or tables.shape[0] != past.size:
+        raise AliceError(_lib.E_SHAPE, f"kv4: {past.size} pasts, {tokens.size} token counts and tables of shape {tables.shape} are not of one batch")
+    return past, tokens, tables
+
+
+def kv4_batch_check(pages, page_tokens, max_seqs, max_tokens, max_pages, past, tokens, tables):
+    """The checks of Kv4Batch.set for a cache and a batch of these sizes; needs no device."""
+    past, tokens, tables = _kv4_step(past, tokens, tables)
+    check(_lib.load().alice_kv4_batch_check(pages, page_tokens, max_seqs, max_tokens, max_pages, past.size, _ptr(past), _ptr(tokens), _ptr(tables), tables.shape[1]))
+
+
+class Kv4Batch:
+    """What one step over a Kv4Cache works on: sequences, their lengths and pages."""
+
+    def __init__(self, engine, handle, heads):
+        self.engine, self._h, self.heads = engine, handle, heads
+        engine._children.add(self)
+
+    def set(self, past, tokens, tables):
+        """past[s] positions of sequence s are in the cache, tokens[s] new ones come behind them; tables[s][p]: page of its positions
+        p * page_tokens onward."""
+        past, tokens, tables = _kv4_step(past, tokens, tables)
+        check(_lib.load().alice_kv4_batch_set(self._h, past.size, _ptr(past), _ptr(tokens), _ptr(tables), tables.shape[1]))
+
+    def free(self):
+        if self._h:
+            _lib.load().alice_kv4_batch_free(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class GpuEngine:
     """GpuEngine (src/gpu.rs:320). ``GpuEngine()`` = ``GpuEngine::new`` (:434)."""
 
@@ -274,6 +331,13 @@ class GpuEngine:
         check(self._lib.alice_buf_read_f32(self._h, buf._h, _ptr(out), n))
         return out
 
+    def upload_u32(self, data) -> GpuBuffer:
+        """32-bit whole numbers in a buffer of as many words."""
+        return self.upload_f32(_np(data, np.uint32).reshape(-1).view(np.float32))
+
+    def read_u32(self, buf: GpuBuffer, length: int | None = None) -> np.ndarray:
+        return self.read_f32(buf, length).view(np.uint32)
+
     def write_f32_async(self, buf: GpuBuffer, host_ptr: int, length: int):
         """Queues the copy of `length` floats at the (pinned) host address into `buf`; the memory must stay valid until the
         next sync(). GpuEngine::write_f32 (queue.write_buffer) does not block either."""
@@ -340,6 +404,47 @@ class GpuEngine:
         a, b = C.c_uint32(), C.c_uint32()
         check(self._lib.alice_batch_plan(self._h, w._h, int(swiglu), batch, C.byref(a), C.byref(b)))
         return a.value, b.value
+
+    # -- paged key / value cache in 4 bits --
+    def kv4_cache(self, pages: int, page_tokens: int, kv_heads: int, head_dim: int) -> Kv4Cache:
+        h = C.c_void_p()
+        check(self._lib.alice_kv4_create(self._h, pages, page_tokens, kv_heads, head_dim, C.byref(h)))
+        return Kv4Cache(self, h, pages, page_tokens, kv_heads, head_dim)
+
+    def kv4_batch(self, cache: Kv4Cache, heads: int, max_seqs: int, max_tokens: int, max_pages: int) -> Kv4Batch:
+        """Room for steps of up to max_seqs sequences with max_tokens new tokens in all and max_pages pages each, over `cache` or any other
+        cache of its shape."""
+        h = C.c_void_p()
+        check(self._lib.alice_kv4_batch_create(self._h, cache._h, heads, max_seqs, max_tokens, max_pages, C.byref(h)))
+        return Kv4Batch(self, h, heads)
+
+    def kv4_append(self, cache: Kv4Cache, batch: Kv4Batch, k: GpuBuffer, v: GpuBuffer, rope: GpuBuffer | None = None, rot_dims: int = 0, neox: bool = False,
+                   k_stride: int = 0, v_stride: int = 0):
+        """Keys (rotated on the way) and values of the batch's new tokens into the cache. rope: see ``rope_table``."""
+        check(self._lib.alice_kv4_append(self._h, cache._h, batch._h, k._h, k_stride, v._h, v_stride, rope and rope._h, rot_dims, int(neox)))
+
+    def kv4_read(self, cache: Kv4Cache, batch: Kv4Batch, k: GpuBuffer, v: GpuBuffer, k_stride: int = 0, v_stride: int = 0):
+        """The values the cache holds for the batch's new tokens."""
+        check(self._lib.alice_kv4_read(self._h, cache._h, batch._h, k._h, k_stride, v._h, v_stride))
+
+    def kv4_attention(self, cache: Kv4Cache, batch: Kv4Batch, q: GpuBuffer, out: GpuBuffer, scale: float, rope: GpuBuffer | None = None, rot_dims: int = 0,
+                      neox: bool = False, q_stride: int = 0, out_stride: int = 0):
+        """Attention of the batch's new tokens, which have been appended, over what their sequences hold."""
+        check(self._lib.alice_kv4_attention(self._h, cache._h, batch._h, q._h, q_stride, out._h, out_stride, rope and rope._h, rot_dims, int(neox), scale))
+
+    def rope_table(self, positions: int, rot_dims: int, theta: float) -> GpuBuffer:
+        """[positions][rot_dims / 2] of (sin, cos), frequencies theta^(-2 j / rot_dims), from 64-bit angles."""
+        freq = float(theta) ** (-np.arange(0, rot_dims, 2, dtype=np.float64) / rot_dims)
+        angle = np.arange(positions, dtype=np.float64)[:, None] * freq
+        return self.upload_f32(np.stack((np.sin(angle), np.cos(angle)), -1))
+
+    # -- log probabilities --
+    def log_probs(self, logits: GpuBuffer, rows: int, vocab: int, targets: GpuBuffer | None, log_probs: GpuBuffer | None, entropy: GpuBuffer | None = None,
+                  rank: GpuBuffer | None = None, top: int = 0, top_ids: GpuBuffer | None = None, top_log_probs: GpuBuffer | None = None, stride: int = 0):
+        """Log probability and rank of each row's target, entropy, and the `top` most probable tokens; what is None is left out. targets,
+        rank and top_ids hold 32-bit whole numbers (upload_u32, read_u32)."""
+        h = [b and b._h for b in (targets, log_probs, entropy, rank)]
+        check(self._lib.alice_log_probs(self._h, logits._h, rows, vocab, stride, *h, top, top_ids and top_ids._h, top_log_probs and top_log_probs._h))
 
     # -- one-shot helpers (src/gpu.rs:838, 962) --
     def matvec(self, weights: GpuWeightBuffer, input_) -> np.ndarray:

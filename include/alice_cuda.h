@@ -186,6 +186,57 @@ int32_t alice_batch_plan(alice_engine* e, const alice_weights* w, int32_t swiglu
  * (more than 8) vectors of q, with `up` the SwiGLU of both, plus resid where that is not null. y[k * rows + r]. No reference counterpart. */
 int32_t alice_debug_prompt_product(alice_engine* e, const alice_weights* w, const alice_weights* up, const alice_q8k* q, const alice_buf* resid, alice_buf* y);
 
+/* ---- a paged key / value cache in 4 bits ---------------------------------------------------- */
+/* Keys and values of one layer in pages (PagedKvCache, src/llama3.rs:5085, keeps f32 pages of 16 positions), in blocks of 32 along a
+ * head: minimum m and step d in half precision and a code of 4 bits a value, 5 bits in all; value = m + d * code with m = half(min),
+ * d = half(max(max - m, 0) / 15), code = (x - m) / d to the nearest whole number, ties to even, in 0..15 (0 where d is 0). m and d stop
+ * at 65504; a block that holds an infinity or a NaN reads back as NaN. What the formulas say is met to the bit.
+ * head_dim 64, 128 or 256; page_tokens a multiple of 16. The pool has pages * kv_heads * page_tokens * head_dim * 1.25 bytes. */
+typedef struct alice_kv4 alice_kv4;
+int32_t alice_kv4_create(alice_engine* e, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, alice_kv4** out);
+int32_t alice_kv4_free(alice_kv4* c);
+/* What one step works on: sequences with `past` positions in the cache already, `tokens` new ones behind them and a table of pages each.
+ * It serves any cache (layer) of the shape of `cache`, which it is made from, with `heads` query heads; room for max_tokens new tokens in
+ * all and max_pages pages a sequence. It owns the scratch of alice_kv4_attention: calls with one batch must not overlap on the device
+ * (on one engine's stream they never do).
+ * alice_kv4_batch_set takes tables[s * table_ld + p], the page of positions p * page_tokens onward of sequence s; entries past the pages
+ * a sequence needs are not looked at, and of a sequence without new tokens none. Sequences may share pages, but none that this step
+ * writes into may occur twice among the written ones. Set is not possible in a stream capture; a captured append, read or attention
+ * works at its replay on what the batch was set to last, provided that asks for as many rows a job (up to 4, up to 8, or more
+ * (token, head) rows of the sequence with most; else alice_sync reports ALICE_E_KERNEL) and fits the buffers and tables of the capture.
+ * alice_kv4_batch_check: the checks of set alone, on the host. */
+typedef struct alice_kv4_batch alice_kv4_batch;
+int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t heads, uint32_t max_seqs, uint32_t max_tokens, uint32_t max_pages,
+                               alice_kv4_batch** out);
+int32_t alice_kv4_batch_free(alice_kv4_batch* b);
+int32_t alice_kv4_batch_set(alice_kv4_batch* b, uint32_t seqs, const uint32_t* past, const uint32_t* tokens, const uint32_t* tables, uint32_t table_ld);
+int32_t alice_kv4_batch_check(uint32_t pages, uint32_t page_tokens, uint32_t max_seqs, uint32_t max_tokens, uint32_t max_pages, uint32_t seqs, const uint32_t* past,
+                              const uint32_t* tokens, const uint32_t* tables, uint32_t table_ld);
+/* Keys and values of the batch's new tokens (rows in the order of the sequences, kv_heads * head_dim floats each, stride floats apart, 0 =
+ * next to one another) into the cache, the keys rotated on the way. rope[position * rot_dims + 2 j] = (sin, cos) of pair j, or null; the
+ * first rot_dims (a multiple of 16) of a head are rotated, neox 0: pairs (2 j, 2 j + 1) (apply_rope, src/llama3.rs:5323), 1: pairs
+ * (j, j + rot_dims / 2) (apply_rope_neox, :5367). KvCache::append, src/llama3.rs:4773. */
+int32_t alice_kv4_append(alice_engine* e, alice_kv4* c, const alice_kv4_batch* b, const alice_buf* k, size_t k_stride, const alice_buf* v, size_t v_stride,
+                         const alice_buf* rope, uint32_t rot_dims, uint32_t neox);
+/* The values the cache holds for the batch's new tokens. */
+int32_t alice_kv4_read(alice_engine* e, const alice_kv4* c, const alice_kv4_batch* b, alice_buf* k, size_t k_stride, alice_buf* v, size_t v_stride);
+/* out = softmax(scale * q K^T) V for the batch's new tokens over the cache: token i of a sequence sees its past + i + 1 first positions,
+ * which have been appended. heads * head_dim floats a row; consecutive query heads share a key / value head; q is rotated on the way
+ * like the keys. Rows of out behind the last token stay as they were. A NaN that a row sees makes it NaN, what it does not see has no
+ * part in it. gqa_attention, src/llama3.rs:5431. */
+int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4_batch* b, const alice_buf* q, size_t q_stride, alice_buf* out, size_t out_stride,
+                            const alice_buf* rope, uint32_t rot_dims, uint32_t neox, float scale);
+
+/* ---- log probabilities ------------------------------------------------------------------------ */
+/* Of each row of logits (vocab floats, stride floats apart, 0 = next to one another): the log probability of its target, the target's
+ * rank (1 + the tokens with a larger logit), the entropy in nats, and the `top` (0..32) most probable tokens with their log
+ * probabilities, the most probable first, the lower index first among equals. targets, rank and top_ids hold 32-bit whole numbers.
+ * Outputs that are null are left out. A target that is no token has NaN and rank 0; a row that holds a NaN or a positive infinity, or
+ * nothing but negative infinities, has NaN, rank 0 and ids 0xffffffff. No reference counterpart (sampling.rs works on the host). */
+#define ALICE_LOGP_MAX_TOP 32
+int32_t alice_log_probs(alice_engine* e, const alice_buf* logits, uint32_t rows, uint32_t vocab, size_t stride, const alice_buf* targets, alice_buf* log_probs,
+                        alice_buf* entropy, alice_buf* rank, uint32_t top, alice_buf* top_ids, alice_buf* top_log_probs);
+
 /* ---- tensor parallel ------------------------------------------------------------------------ */
 /* One engine (one process) per GPU; output rows of every projection are sharded over the group and the
  * full vector is rebuilt on every rank by an NCCL all-gather queued on the engine's stream (the row
