@@ -120,7 +120,7 @@ int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t
     if (!b) return alice_fail(ALICE_E_NOMEM, "%s: host allocation failed", who);
     b->e = e; b->shape = s; b->group = heads / s.kv_heads;
     b->max_seqs = max_seqs; b->max_tokens = max_tokens; b->max_pages = max_pages;
-    b->max_jobs = kv4_max_jobs(max_seqs, max_tokens, b->group);
+    b->max_jobs = kv4_max_jobs(max_seqs, max_tokens, b->group, s.dim);
     alice_engine_retain(e);
     size_t at = 0;
     auto take = [&](size_t words) { const size_t o = at; at += (words * 4 + 15) & ~size_t(15); return o; };
@@ -177,7 +177,7 @@ int32_t alice_kv4_batch_set(alice_kv4_batch* b, uint32_t seqs, const uint32_t* p
         CU(cudaStreamIsCapturing(st, &capturing));
         if (capturing != cudaStreamCaptureStatusNone) return alice_cuda_fail(cudaErrorStreamCaptureUnsupported, "alice_kv4_batch_set: lengths and pages of a captured stream");
         Kv4HostPlan h;
-        if (!kv4_make_plan(h, b->shape.page_tokens, b->group, seqs, past, tokens, tables, table_ld, b->max_pages))
+        if (!kv4_make_plan(h, b->shape.dim, b->shape.page_tokens, b->group, seqs, past, tokens, tables, table_ld, b->max_pages))
             return alice_fail(ALICE_E_SHAPE, "%s: too many tokens over too many positions for one step", who);
         // copies from pageable memory: the vectors have been read when a call returns
         auto up = [&](const uint32_t* dst, const std::vector<uint32_t>& src) -> cudaError_t {

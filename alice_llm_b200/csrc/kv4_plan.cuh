@@ -17,8 +17,11 @@ inline int kv4_check_shape(const char* who, uint32_t pages, uint32_t page_tokens
     return ALICE_OK;
 }
 
-// Jobs of 16 rows, or one for each sequence where it has fewer.
-inline uint32_t kv4_max_jobs(uint32_t seqs, uint32_t tokens, uint32_t group) { return seqs + (uint32_t)(((uint64_t)tokens * group + 15) / 16); }
+// Jobs of 8 or 16 rows, or one for each sequence where it has fewer.
+inline uint32_t kv4_max_jobs(uint32_t seqs, uint32_t tokens, uint32_t group, uint32_t dim) {
+    const uint32_t rows = dim == 256 ? 8 : 16;
+    return seqs + (uint32_t)(((uint64_t)tokens * group + rows - 1) / rows);
+}
 
 inline int kv4_check_limits(const char* who, uint32_t kv_heads, uint32_t dim, uint32_t heads, uint32_t max_seqs, uint32_t max_tokens, uint32_t max_pages) {
     if (!heads || heads % kv_heads) return alice_fail(ALICE_E_SHAPE, "%s: %u query heads over %u key / value heads", who, heads, kv_heads);
@@ -62,12 +65,12 @@ struct Kv4HostPlan {
 };
 
 // Of checked arguments. Rows of one job see up to `last` keys, those of its last token. false: more than 2^31 tiles.
-inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t page_tokens, uint32_t group, uint32_t seqs, const uint32_t* past, const uint32_t* tokens, const uint32_t* tables,
+inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t page_tokens, uint32_t group, uint32_t seqs, const uint32_t* past, const uint32_t* tokens, const uint32_t* tables,
                           uint32_t table_ld, uint32_t max_pages) {
     uint32_t most = 0, total = 0;
     uint64_t tiles = 0;
     for (uint32_t s = 0; s < seqs; s++) most = std::max(most, tokens[s] * group);
-    const uint32_t rows = kv4_job_rows(most);
+    const uint32_t rows = kv4_job_rows(most, dim);
     h.past.assign(past, past + seqs); h.count.assign(tokens, tokens + seqs);
     h.table.assign((size_t)seqs * max_pages, 0);
     h.job_tile.push_back(0);
