@@ -7,7 +7,7 @@
 // A page holds page_tokens (a multiple of 16) positions of every key / value head: [page][kv head][tile of 16 positions], so one tile of
 // one head is one contiguous piece of memory:
 //   16 rows of key codes | 16 rows of value codes | 16 rows of key scales | 16 rows of value scales
-// A row of codes has dim / 2 bytes, a row of scales a (d, m) pair for each block. The order within is the one in which the lanes of a
+// A row of codes has dim / 2 bytes, a row of scales the d of all blocks, then their m. The order within is the one in which the lanes of a
 // warp hold the operands of m16n8k16 products, lane = 4 * g + t, so that a lane's share of a row is one load:
 //   keys    row kv4_row(T) for position T of the tile; the 8 codes of dims 32 b + 8 t .. + 7 are word t * NB + b (NB = dim / 32; of 256
 //           dims each half of the row by itself). Nibble i of a word is dim 8 t + i.

@@ -177,7 +177,8 @@ int32_t alice_kv4_batch_set(alice_kv4_batch* b, uint32_t seqs, const uint32_t* p
         CU(cudaStreamIsCapturing(st, &capturing));
         if (capturing != cudaStreamCaptureStatusNone) return alice_cuda_fail(cudaErrorStreamCaptureUnsupported, "alice_kv4_batch_set: lengths and pages of a captured stream");
         Kv4HostPlan h;
-        if (!kv4_make_plan(h, b->shape.dim, b->shape.page_tokens, b->group, seqs, past, tokens, tables, table_ld, b->max_pages))
+        const bool fits = kv4_make_plan(h, b->shape.dim, b->shape.page_tokens, b->group, seqs, past, tokens, tables, table_ld, b->max_pages);
+        if (!fits || (uint64_t)h.head.tiles * b->shape.kv_heads > 0x7fffffffull)     // tiles of all heads are numbered in 32 bits
             return alice_fail(ALICE_E_SHAPE, "%s: too many tokens over too many positions for one step", who);
         // copies from pageable memory: the vectors have been read when a call returns
         auto up = [&](const uint32_t* dst, const std::vector<uint32_t>& src) -> cudaError_t {

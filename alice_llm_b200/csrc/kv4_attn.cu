@@ -1,10 +1,10 @@
 // Attention of one or several new tokens over the 4-bit cache (csrc/kv4.cuh).
 //
 // A warp takes a job's 4, 8 or 16 (token, query head) rows against tiles of 16 keys with m16n8k16 products in half precision:
-//   scores^T [key][row]  = sum over blocks of d * (codes . q) + m * (sum of q)
+//   scores^T [key][row]  = sum over blocks of d * (codes . q), and m * (sum of q) of all blocks as a product of its own
 //   out^T [dim][row]    += codes * (p * d), and m * p apart in f32
-// with d, m a block's step and minimum. Codes enter less 8 (and m is m + 8 d), so that the two parts of a sum over many keys do not
-// cancel; unpacking two of them is a mask and an exact addition in half precision. (Masked bits alone are exact operands too, as numbers
+// with d, m a block's step and minimum. Codes of values enter less 8 (and m is m + 8 d), so that the two parts of a sum over many keys do
+// not cancel; unpacking two of them is a mask and an exact addition in half precision. (Masked bits alone are exact operands too, as numbers
 // below 2^-14, but the products of those lose bits in the sum: results were 4e-5 to 4e-4 off.) The other operand, q or p * d, is a pair of half-precision
 // numbers (value and remainder, 22 bits), scaled by powers of two into the middle of their range.
 // With up to 4 rows the pair fills two columns of the product, with more they are two products.
@@ -17,6 +17,8 @@
 // on tensor cores add up with less than f32 rounding, which over a long chain would add up itself.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv4.cuh"
 
@@ -24,10 +26,16 @@ namespace alice {
 
 namespace {
 
-constexpr int STAGES = 3;
+constexpr int STAGES = 4;
 constexpr uint32_t FLUSH = 16;       // tiles
 constexpr uint32_t MAX_CTAS = 192;
 constexpr float ROOM = 8.0f;         // what a score may exceed the reference by, in powers of two
+
+// A warp's part of a job that is not all of it.
+struct Segment {
+    uint32_t ends;                       // 1: has the job's first tile, 2: its last; 4: there is one
+    uint32_t head, job, row, rows, first;
+};
 
 template <int NB, int R>
 struct Cfg {
@@ -41,8 +49,7 @@ struct Cfg {
     struct Smem {
         float4 sum[WARPS][2][NF][32];
         float2 ml[WARPS][2][R];                                   // reference and sum of weights
-        long long seg_job[WARPS][2];                              // key head * jobs + job, -1: nothing to join
-        uint32_t seg_ends[WARPS][2];                              // 1: has the job's first tile, 2: its last
+        Segment seg[2 * WARPS];
         float weight[2 * WARPS][R], total[R];
         uint32_t last[2];
         alignas(16) uint8_t ring[WARPS][STAGES][TILE];
@@ -57,23 +64,31 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // the same with a sum that starts at zero
-__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&z)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z[0]), "f"(z[1]), "f"(z[2]), "f"(z[3]));
 }
-// The eight codes of a word less 8, two to a register: .. [0] nibbles 0 and 4, [1] 1 and 5, [2] 2 and 6, [3] 3 and 7. Four bits put under
+// The eight codes of a word less LESS, two to a register: .. [0] nibbles 0 and 4, [1] 1 and 5, [2] 2 and 6, [3] 3 and 7. Four bits put under
 // the exponent of 1024 are 1024 + code, or with the next four 1024 + 16 code; both steps are exact.
 struct Codes { uint32_t v[4]; };
+__device__ __forceinline__ uint32_t under_exponent(uint32_t x, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(0x64006400u));      // x & mask | 1024s, one instruction
+    return r;
+}
+template <int LESS>
 __device__ __forceinline__ Codes unpack(uint32_t x) {
-    constexpr uint32_t MAGIC = 0x64006400u, EVEN = 0x000f000fu, ODD = 0x00f000f0u;
-    const __half2 less = __half2half2(__ushort_as_half(0xe408)), sixteenth = __half2half2(__ushort_as_half(0x2c00)), less16 = __half2half2(__ushort_as_half(0xd480));  // -1032, 1 / 16, -72
+    static_assert(LESS == 0 || LESS == 8, "");
+    constexpr uint32_t EVEN = 0x000f000fu, ODD = 0x00f000f0u;
+    const __half2 less = __half2half2(__ushort_as_half(LESS ? 0xe408 : 0xe400)), sixteenth = __half2half2(__ushort_as_half(0x2c00)),
+                  less16 = __half2half2(__ushort_as_half(LESS ? 0xd480 : 0xd400));      // -1024 - LESS, 1 / 16, -64 - LESS
     const uint32_t y = x >> 8;
     Codes c;
-    c.v[0] = half2_bits(__hadd2(bits_half2(x & EVEN | MAGIC), less));
-    c.v[1] = half2_bits(__hfma2(bits_half2(x & ODD | MAGIC), sixteenth, less16));
-    c.v[2] = half2_bits(__hadd2(bits_half2(y & EVEN | MAGIC), less));
-    c.v[3] = half2_bits(__hfma2(bits_half2(y & ODD | MAGIC), sixteenth, less16));
+    c.v[0] = half2_bits(__hadd2(bits_half2(under_exponent(x, EVEN)), less));
+    c.v[1] = half2_bits(__hfma2(bits_half2(under_exponent(x, ODD)), sixteenth, less16));
+    c.v[2] = half2_bits(__hadd2(bits_half2(under_exponent(y, EVEN)), less));
+    c.v[3] = half2_bits(__hfma2(bits_half2(under_exponent(y, ODD)), sixteenth, less16));
     return c;
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
@@ -103,6 +118,10 @@ __device__ __forceinline__ Words<N> lds_words(uint32_t a) {
     }
     return r;
 }
+
+// half-precision number i of a lane's words
+template <int N>
+__device__ __forceinline__ float half_of(const Words<N>& x, int i) { return i & 1 ? __high2float(bits_half2(x.w[i / 2])) : __low2float(bits_half2(x.w[i / 2])); }
 
 // 8 consecutive floats of a query, from dim0 on, rotated.
 __device__ __forceinline__ void rotated8(float (&x)[8], const float* q, uint32_t dim0, const float* turn, const Kv4Rope& rope) {
@@ -177,25 +196,41 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     const Kv4Plan& pl = a.plan;
     const Kv4Head hd = *pl.head;
     if (!kv4_fits(hd, a.most_tokens, a.rope, a.shape, R, a.status)) return;
-    const unsigned long long total = (unsigned long long)hd.tiles * a.shape.kv_heads;
-    // a part of a CTA is at least a tile for each of its warps
-    const uint32_t grid = (uint32_t)min((unsigned long long)gridDim.x, (total + W - 1) / W);
-    if (blockIdx.x >= grid) return;
-    const unsigned long long c0 = total * blockIdx.x / grid, c1 = total * (blockIdx.x + 1) / grid;
-    const unsigned long long w0 = c0 + (c1 - c0) * warp / W, w1 = c0 + (c1 - c0) * (warp + 1) / W;
-    if (lane < 2) sh.seg_job[warp][lane] = -1;
+    // Equal parts for the CTAs, those of one job only (a sequence of few new tokens) at the borders of key heads: no CTA has parts of two
+    // of them then, and where a CTA can have all of a head there is nothing to join between CTAs.
+    const uint32_t tiles = hd.tiles, total = tiles * a.shape.kv_heads, cta = blockIdx.x;
+    uint32_t grid, splits = 0, c0, c1;
+    if (hd.jobs == 1 && a.shape.kv_heads <= gridDim.x) {
+        splits = tiles <= 2 * W ? 1 : min(gridDim.x / a.shape.kv_heads, (tiles + W - 1) / W);
+        grid = splits * a.shape.kv_heads;
+        const uint32_t h = cta / splits, i = cta - h * splits, per = tiles / splits, more = tiles - per * splits;
+        c0 = h * tiles + i * per + min(i, more);
+        c1 = c0 + per + (i < more ? 1 : 0);
+    } else {
+        grid = min(gridDim.x, (total + W - 1) / W);
+        if (grid == 0) return;
+        const uint32_t per = total / grid, more = total - per * grid;
+        c0 = cta * per + min(cta, more);
+        c1 = c0 + per + (cta < more ? 1 : 0);
+    }
+    if (cta >= grid) return;
+    const uint32_t w0 = c0 + (c1 - c0) * warp / W, w1 = c0 + (c1 - c0) * (warp + 1) / W;
+    if (lane < 2) sh.seg[2 * warp + lane].ends = 0;
+    float zero[4];       // registers of their own: the start of a product's sums
+#pragma unroll
+    for (int i = 0; i < 4; i++) asm volatile("mov.f32 %0, 0f00000000;" : "=f"(zero[i]));
 
     if (w0 < w1) {
         // ---- the ring: tiles are asked for STAGES - 1 ahead ----
         const uint32_t ring = smem_u32(sh.ring[warp][0]);
         const uint32_t per_page = a.shape.tiles();
-        uint32_t p_head = (uint32_t)(w0 / hd.tiles), p_tile = (uint32_t)(w0 - (unsigned long long)p_head * hd.tiles);
+        uint32_t p_head = w0 / tiles, p_tile = w0 - p_head * tiles;
         uint32_t p_job = find_job(pl.job_tile, hd.jobs, p_tile, lane);
         uint32_t job = p_job, head = p_head;
         uint32_t p_seq = 0, p_tile0 = 0, p_end = 0, p_pages = 0, p_base = 0xffffffffu;    // of the job; pages of 32 pages, a lane each
         uint32_t p_left = 0;                                                             // tiles to come of the page and the job
         const uint8_t* p_src = nullptr;
-        uint32_t p_count = (uint32_t)(w1 - w0);
+        uint32_t p_count = w1 - w0;
         bool p_new = true;
         auto ask = [&](uint32_t stage) {
             if (p_count) {
@@ -221,7 +256,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 p_src += TILE; p_tile++;
                 if (--p_left == 0 && p_tile == p_end) {
                     p_new = true; p_job++;
-                    if (p_tile == hd.tiles) { p_tile = 0; p_job = 0; p_head++; }
+                    if (p_tile == tiles) { p_tile = 0; p_job = 0; p_head++; }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -230,16 +265,16 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         for (int s = 0; s < STAGES - 1; s++) ask(s);
 
         uint32_t stage = 0, slot = 0;
-        for (unsigned long long at = w0; at < w1;) {
+        for (uint32_t at = w0; at < w1;) {
             // ---- a job, or this warp's part of it ----
             const Job jb = get_job(pl, job, a.group, R);
-            const unsigned long long j0 = (unsigned long long)head * hd.tiles + jb.tile0, j1 = (unsigned long long)head * hd.tiles + jb.tile1;
-            const unsigned long long end = min(j1, w1);
+            const uint32_t j0 = head * tiles + jb.tile0, j1 = head * tiles + jb.tile1, end = min(j1, w1);
             const bool has_first = at == j0, has_last = end == j1;
 
             // queries: columns of the product in the order of a lane's codes, and what each row needs beside them
             uint32_t qf[NT][NB][SPLIT ? 4 : 8];      // [..][0..3]: (value, or by column value and remainder), [4..7]: remainders
-            float qsum[RT][NB], factor[RT];
+            uint32_t qm[NT][2];                      // sums of a block's queries, values and remainders: columns of the product with the minima
+            float factor[RT];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const uint32_t row = SPLIT ? g >> 1 : n * 8 + g;
@@ -264,13 +299,14 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 const float down = pow2(-e2);
                 const float up = pow2(e2);
                 const bool low = SPLIT && (g & 1);
+                float sums[NB];
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     float sum = 0;
 #pragma unroll
                     for (int e = 0; e < 8; e++) sum += x[b][e] * down;
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    sums[b] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const float v0 = x[b][e] * down, v1 = x[b][e + 4] * down;
@@ -280,12 +316,25 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         if (SPLIT) qf[n][b][e] = half2_bits(low ? lo : hi);
                         else { qf[n][b][e] = half2_bits(hi); qf[n][b][SPLIT ? 0 : 4 + e] = half2_bits(lo); }
                     }
-                    if (SPLIT) qsum[0][b] = __shfl_sync(0xffffffffu, sum, t * 8);
+                }
+                // The minima of a key are the first columns (of 8 blocks all) of an operand's 16, again as the next; the sums' values and
+                // remainders stand against them.
+                auto pair = [&](int p, bool remainder) -> uint32_t {
+                    const __half2 hi = __floats2half2_rn(sums[2 * p % NB], sums[(2 * p + 1) % NB]);
+                    if (!remainder) return half2_bits(hi);
+                    const float2 back = __half22float2(hi);
+                    return half2_bits(__floats2half2_rn(sums[2 * p % NB] - back.x, sums[(2 * p + 1) % NB] - back.y));
+                };
+                uint32_t m0 = 0, m1 = 0;
+#pragma unroll
+                for (int p = 0; p < NB / 2; p++) {
+                    if (NB == 8) { if ((int)t == p) { m0 = pair(p, false); m1 = pair(p, true); } }
                     else {
-                        qsum[2 * n % RT][b] = __shfl_sync(0xffffffffu, sum, t * 8);
-                        qsum[(2 * n + 1) % RT][b] = __shfl_sync(0xffffffffu, sum, t * 8 + 4);
+                        if ((int)t == p) m0 = pair(p, false);
+                        if ((int)t == p + NB / 2) m0 = pair(p, true);
                     }
                 }
+                qm[n][0] = low ? 0 : m0; qm[n][1] = low ? 0 : m1;
                 const float f = up;
                 if (SPLIT) factor[0] = __shfl_sync(0xffffffffu, f, t * 8) * 1.44269504088896341f;
                 else {
@@ -355,57 +404,74 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 held = 0; begun = true;
             };
 
-            uint32_t key0 = (uint32_t)(at - j0) * KV4_TILE;
-            for (; at < end; at++, key0 += KV4_TILE) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-                __syncwarp();
-                ask((stage + STAGES - 1) % STAGES);       // where the tile before this one was: every lane is done with it
-                const uint32_t base = ring + stage * TILE;
-                // ---- scores ----
-                float s[RT][2];                 // of keys tau(g), 8 + tau(g)
-#pragma unroll
-                for (int i = 0; i < RT; i++) s[i][0] = s[i][1] = 0;
+            uint32_t key0 = (at - j0) * KV4_TILE;
+            float s[RT][2], p[RT][2];           // of keys tau(g), 8 + tau(g)
+            Words<NB> va, vb;                   // scales of their values
+            auto scores = [&](uint32_t base) {
                 const uint32_t krow = base + g * (DIM / 2), srow = base + kv4_k_scales(DIM) + g * (4 * NB);
+                // a row of scales: the steps of its blocks, then their minima
+                Words<NB / 2> sa = lds_words<NB / 2>(srow), sb = lds_words<NB / 2>(srow + 32 * NB);
+                const uint32_t mat = srow + 2 * NB + 4 * (t % (NB / 2)), ma = lds32(mat), mb = lds32(mat + 32 * NB);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float c[4];
+                    mma_f16_first(c, ma, mb, ma, mb, qm[n][0], qm[n][1], zero);
+                    if (SPLIT) { s[0][0] = c[0]; s[0][1] = c[2]; }
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 2; j++) { s[(2 * n + j) % RT][0] = c[j]; s[(2 * n + j) % RT][1] = c[2 + j]; }
+                    }
+                }
 #pragma unroll
                 for (int h = 0; h < (NB + 3) / 4; h++) {
                     constexpr int NW = NB < 4 ? NB : 4;
                     const uint32_t kat = krow + (NB == 8 ? h * 64 + t * 16 : t * NB * 4);
                     const Words<NW> ka = lds_words<NW>(kat), kb = lds_words<NW>(kat + 4 * DIM);
-                    const Words<NW> sa = lds_words<NW>(srow + h * 16), sb = lds_words<NW>(srow + h * 16 + 32 * NB);
 #pragma unroll
                     for (int w = 0; w < NW; w++) {
                         const int b = h * 4 + w;
-                        const Codes xa = unpack(ka.w[w]), xb = unpack(kb.w[w]);
-                        float2 da = __half22float2(bits_half2(sa.w[w])), db = __half22float2(bits_half2(sb.w[w]));
-                        da.y = fmaf(8.0f, da.x, da.y); db.y = fmaf(8.0f, db.x, db.y);       // what a code of 8 stands for
+                        const Codes xa = unpack<0>(ka.w[w]), xb = unpack<0>(kb.w[w]);
+                        const __half2 ha = bits_half2(sa.w[b / 2]), hb = bits_half2(sb.w[b / 2]);
+                        const float da = b & 1 ? __high2float(ha) : __low2float(ha), db = b & 1 ? __high2float(hb) : __low2float(hb);
 #pragma unroll
                         for (int n = 0; n < NT; n++) {
                             float c[4];
-                            mma_f16_first(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][0], qf[n][b][1]);
+                            mma_f16_first(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][0], qf[n][b][1], zero);
                             mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][2], qf[n][b][3]);
                             if (!SPLIT) {
                                 mma_f16(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][SPLIT ? 0 : 4], qf[n][b][SPLIT ? 0 : 5]);
                                 mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][SPLIT ? 0 : 6], qf[n][b][SPLIT ? 0 : 7]);
                             }
                             if (SPLIT) {
-                                s[0][0] = fmaf(da.x, c[0] + c[1], fmaf(da.y, qsum[0][b], s[0][0]));
-                                s[0][1] = fmaf(db.x, c[2] + c[3], fmaf(db.y, qsum[0][b], s[0][1]));
+                                s[0][0] = fmaf(da, c[0] + c[1], s[0][0]);
+                                s[0][1] = fmaf(db, c[2] + c[3], s[0][1]);
                             } else {
 #pragma unroll
                                 for (int j = 0; j < 2; j++) {
                                     const int i = (2 * n + j) % RT;
-                                    s[i][0] = fmaf(da.x, c[j], fmaf(da.y, qsum[i][b], s[i][0]));
-                                    s[i][1] = fmaf(db.x, c[2 + j], fmaf(db.y, qsum[i][b], s[i][1]));
+                                    s[i][0] = fmaf(da, c[j], s[i][0]);
+                                    s[i][1] = fmaf(db, c[2 + j], s[i][1]);
                                 }
                             }
                         }
                     }
                 }
+            };
+            // the scores of a tile are worked out beside the sums of the one before it
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncwarp();
+            scores(ring + stage * TILE);
+            for (; at < end; at++, key0 += KV4_TILE) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 3) : "memory");
+                __syncwarp();
+                ask((stage + STAGES - 1) % STAGES);       // where the tile before this one was: every lane is done with it
+                const uint32_t base = ring + stage * TILE;
+                auto weights = [&](auto edge_t) {
+                constexpr bool edge = decltype(edge_t)::value;       // some row does not see all of the tile
                 // ---- weights ----
                 const uint32_t tau = (g >> 1) + 4 * (g & 1), keyA = key0 + tau, keyB = keyA + 8;
                 const uint32_t vsrow = base + kv4_v_scales(DIM) + g * (4 * NB);
-                Words<NB> va = lds_words<NB>(vsrow), vb = lds_words<NB>(vsrow + 32 * NB);
-                const bool edge = key0 + KV4_TILE > least;       // some row does not see all of the tile
+                va = lds_words<NB>(vsrow); vb = lds_words<NB>(vsrow + 32 * NB);
                 bool move = false;
 #pragma unroll
                 for (int i = 0; i < RT; i++) {
@@ -429,8 +495,8 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 }
                 __half2 both = __hmax2(bits_half2(va.w[0]), bits_half2(vb.w[0]));
 #pragma unroll
-                for (int b = 1; b < NB; b++) both = __hmax2(both, __hmax2(bits_half2(va.w[b]), bits_half2(vb.w[b])));
-                const uint32_t dmax = half2_bits(both) & 0x7c00u;
+                for (int b = 1; b < NB / 2; b++) both = __hmax2(both, __hmax2(bits_half2(va.w[b]), bits_half2(vb.w[b])));
+                const uint32_t dmax = max(half2_bits(both) & 0x7c00u, half2_bits(both) >> 16 & 0x7c00u);
                 move |= dmax > dtop;
                 if (__any_sync(0xffffffffu, move)) {
                     if (held) flush();
@@ -446,7 +512,6 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         ref[i] = fmaxf(ref[i], m);
                     }
                 }
-                float p[RT][2];
 #pragma unroll
                 for (int i = 0; i < RT; i++) {
                     p[i][0] = ex2(s[i][0] - ref[i]); p[i][1] = ex2(s[i][1] - ref[i]);
@@ -456,7 +521,21 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                     }
                     l[i] += p[i][0] + p[i][1];
                 }
-                // ---- values ----
+                // minima: of a key that a row does not see not even a NaN
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const float ma = fmaf(8.0f, half_of(va, b), half_of(va, NB + b)), mb = fmaf(8.0f, half_of(vb, b), half_of(vb, NB + b));   // what a code of 8 stands for
+#pragma unroll
+                    for (int i = 0; i < RT; i++) {
+                        if (!edge) accm[i][b] = fmaf(p[i][0], ma, fmaf(p[i][1], mb, accm[i][b]));
+                        else {
+                            if (keyA < limit[i]) accm[i][b] = fmaf(p[i][0], ma, accm[i][b]);
+                            if (keyB < limit[i]) accm[i][b] = fmaf(p[i][1], mb, accm[i][b]);
+                        }
+                    }
+                }
+                };
+                auto values = [&]() {
                 Words<(NB + 1) / 2> v[4];
                 const uint32_t vrow = base + kv4_v_codes(DIM) + t * (DIM / 2) + g * (2 * NB);
 #pragma unroll
@@ -465,8 +544,8 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 for (int b = 0; b < NB; b++) {
                     const uint32_t pick = b & 1 ? 0x7632u : 0x5410u;
                     const uint32_t xa = __byte_perm(v[0].w[b / 2], v[1].w[b / 2], pick), xb = __byte_perm(v[2].w[b / 2], v[3].w[b / 2], pick);
-                    const Codes ca = unpack(xa), cb = unpack(xb);
-                    const float dax = __low2float(bits_half2(va.w[b])) * dscale, dbx = __low2float(bits_half2(vb.w[b])) * dscale;
+                    const Codes ca = unpack<8>(xa), cb = unpack<8>(xb);
+                    const float da = half_of(va, b), db = half_of(vb, b), dax = da * dscale, dbx = db * dscale;
 #pragma unroll
                     for (int n = 0; n < NT; n++) {
                         if (SPLIT) {
@@ -490,22 +569,11 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         }
                     }
                 }
-                // minima: of a key that a row does not see not even a NaN
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    float2 da = __half22float2(bits_half2(va.w[b])), db = __half22float2(bits_half2(vb.w[b]));
-                    const float ma = fmaf(8.0f, da.x, da.y), mb = fmaf(8.0f, db.x, db.y);
-#pragma unroll
-                    for (int i = 0; i < RT; i++) {
-                        if (!edge) accm[i][b] = fmaf(p[i][0], ma, fmaf(p[i][1], mb, accm[i][b]));
-                        else {
-                            if (keyA < limit[i]) accm[i][b] = fmaf(p[i][0], ma, accm[i][b]);
-                            if (keyB < limit[i]) accm[i][b] = fmaf(p[i][1], mb, accm[i][b]);
-                        }
-                    }
-                }
-                held++;
+                };
+                if (key0 + KV4_TILE > least) weights(std::true_type{}); else weights(std::false_type{});
                 stage = stage + 1 == STAGES ? 0 : stage + 1;
+                if (at + 1 < end) { scores(ring + stage * TILE); values(); } else values();
+                held++;
                 if (held == FLUSH) flush();
             }
             if (held) flush();
@@ -530,10 +598,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
 #pragma unroll
                     for (int i = 0; i < RT; i++) sh.ml[warp][slot][SPLIT ? t : (i >> 1) * 8 + 2 * t + (i & 1)] = make_float2(mref[i], lsum[i]);
                 }
-                if (lane == 0) {
-                    sh.seg_job[warp][slot] = (long long)head * hd.jobs + job;
-                    sh.seg_ends[warp][slot] = (has_first ? 1u : 0u) | (has_last ? 2u : 0u);
-                }
+                if (lane == 0) sh.seg[2 * warp + slot] = Segment{4u | (has_first ? 1u : 0u) | (has_last ? 2u : 0u), head, job, jb.row, jb.rows, jb.first};
             }
             slot = 1;
             if (has_last) {
@@ -547,87 +612,108 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     // ---- parts of jobs: joined in the CTA, then by the last CTA of each job ----
     if (tid < 2) sh.last[tid] = 0;
     __syncthreads();
-    const long long my_job = lane < 2 * W ? sh.seg_job[lane >> 1][lane & 1] : -1;
-    const uint32_t my_ends = my_job >= 0 ? sh.seg_ends[lane >> 1][lane & 1] : 0u;
-    const uint32_t valid = __ballot_sync(0xffffffffu, my_job >= 0);
-    // a row's place in the fragments: element f = (i * NB + b) * 32 + lane
-    auto row_of = [](uint32_t f) { const uint32_t i = f / (NB * 32), ln = f & 31; return SPLIT ? ln & 3 : (i >> 1) * 8 + 2 * (ln & 3) + (i & 1); };
-    auto store_out = [&](long long jid, uint32_t f, float4 o, float l) {
-        const uint32_t head = (uint32_t)(jid / hd.jobs);
-        const Job jb = get_job(pl, (uint32_t)(jid - (long long)head * hd.jobs), a.group, R);
-        const uint32_t row = row_of(f);
-        if (row >= jb.rows) return;
-        const uint32_t r = jb.row + row, b = f / 32 % NB, ln = f & 31;
-        const float inv = 1.0f / l;
-        float* out = a.out + (size_t)(jb.first + r / a.group) * a.out_ld + (size_t)(head * a.group + r % a.group) * DIM + b * 32 + 4 * (ln >> 2);
-        *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    };
-    auto part_at = [&](uint32_t cta, uint32_t which) { return a.part + ((size_t)cta * 2 + which) * C::PART; };
-    // weights of the parts: a warp a row, a part a lane
+    // Parts in the order of the work, a lane each; those of one job are a run.
+    Segment sg{};
+    if (lane < 2 * W) sg = sh.seg[lane];
+    const uint32_t valid = __ballot_sync(0xffffffffu, sg.ends != 0), below = valid & ((1u << lane) - 1);
+    if (!valid) return;
+    const int before = below ? 31 - __clz(below) : 0;
+    const uint32_t pj = __shfl_sync(0xffffffffu, sg.job, before), ph = __shfl_sync(0xffffffffu, sg.head, before);
+    const uint32_t starts = __ballot_sync(0xffffffffu, sg.ends && (!below || pj != sg.job || ph != sg.head));
+    const int runs = __popc(starts), run = __popc(starts & (0xffffffffu >> (31 - lane))) - 1;
+    // weights of the parts: a warp a row
     for (uint32_t row = warp; row < R; row += W) {
-        float2 ml = my_job >= 0 ? sh.ml[lane >> 1][lane & 1][row] : make_float2(0, 0);
-        for (uint32_t left = valid; left;) {
-            const long long jid = __shfl_sync(0xffffffffu, my_job, __ffs(left) - 1);
-            const bool member = my_job == jid;
-            left &= ~__ballot_sync(0xffffffffu, member);
-            float m = member ? ml.x : -INFINITY;
+        const float2 ml = sg.ends ? sh.ml[lane >> 1][lane & 1][row] : make_float2(-INFINITY, 0);
+        const uint32_t later = starts & ~(0xffffffffu >> (31 - lane));
+        const int last = later ? __ffs(later) - 2 : 31;
+        float m = ml.x;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float c = member ? ml.x == m ? 1.0f : ex2(ml.x - m) : 0.0f;
-            float l = member ? ml.y * c : 0.0f;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (member) { sh.ml[lane >> 1][lane & 1][row] = make_float2(m, l); sh.weight[lane][row] = c; }
+        for (int o = 1; o < 32; o <<= 1) {
+            const float v = __shfl_up_sync(0xffffffffu, m, o);
+            if (__shfl_up_sync(0xffffffffu, run, o) == run && (int)lane >= o) m = fmaxf(m, v);
         }
+        m = __shfl_sync(0xffffffffu, m, last);
+        const float c = ml.x == m ? 1.0f : ex2(ml.x - m);
+        float l = sg.ends ? ml.y * c : 0.0f;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const float v = __shfl_up_sync(0xffffffffu, l, o);
+            if (__shfl_up_sync(0xffffffffu, run, o) == run && (int)lane >= o) l += v;
+        }
+        l = __shfl_sync(0xffffffffu, l, last);
+        if (sg.ends) { sh.weight[lane][row] = c; sh.ml[lane >> 1][lane & 1][row] = make_float2(m, l); }
     }
     __syncthreads();
-    long long open_job[2] = {-1, -1};        // of this CTA: one that began before it, one that began in it
-    for (uint32_t left = valid; left;) {
-        const int first = __ffs(left) - 1;
-        const long long jid = __shfl_sync(0xffffffffu, my_job, first);
-        const uint32_t members = __ballot_sync(0xffffffffu, my_job == jid);
-        const uint32_t ends = __reduce_or_sync(0xffffffffu, my_job == jid ? my_ends : 0u);
-        left &= ~members;
-        if (ends == 1) open_job[1] = jid;
-        if (!(ends & 1)) open_job[0] = jid;
-        for (uint32_t f = tid; f < NF * 32; f += W * 32) {
-            const uint32_t row = row_of(f);
-            float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-            for (uint32_t e = first; e < 2 * W; e++) {
-                if (!(members >> e & 1)) continue;
-                const float c = sh.weight[e][row];
-                const float4 x = (&sh.sum[e >> 1][e & 1][0][0])[f];
-                o.x = fmaf(x.x, c, o.x); o.y = fmaf(x.y, c, o.y); o.z = fmaf(x.z, c, o.z); o.w = fmaf(x.w, c, o.w);
+    // a row's place in the fragments: element f = (i * NB + b) * 32 + lane
+    auto row_of = [](uint32_t f) { const uint32_t i = f / (NB * 32), ln = f & 31; return SPLIT ? ln & 3 : (i >> 1) * 8 + 2 * (ln & 3) + (i & 1); };
+    auto store_out = [&](const Segment& of, uint32_t f, float4 o, float l) {
+        const uint32_t row = row_of(f);
+        if (row >= of.rows) return;
+        const uint32_t r = of.row + row, b = f / 32 % NB, tok = r / a.group;
+        const float inv = 1.0f / l;
+        float* out = a.out + (size_t)(of.first + tok) * a.out_ld + (size_t)(of.head * a.group + r - tok * a.group) * DIM + b * 32 + 4 * ((f & 31) >> 2);
+        *reinterpret_cast<float4*>(out) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    };
+    auto part_at = [&](uint32_t of, uint32_t which) { return a.part + ((size_t)of * 2 + which) * C::PART; };
+    constexpr uint32_t NE = NF * 32;
+    for (uint32_t i = tid; i < runs * NE; i += W * 32) {
+        const uint32_t k = i / NE, f = i % NE, row = row_of(f);
+        uint32_t members = __ballot_sync(0xffffffffu, sg.ends && run == (int)k);
+        const uint32_t ends = __reduce_or_sync(0xffffffffu, run == (int)k ? sg.ends : 0u), e0 = __ffs(members) - 1;
+        float4 o = make_float4(0, 0, 0, 0);
+        while (members) {        // four at a time
+            float c[4];
+            float4 x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t e = members ? __ffs(members) - 1 : e0;
+                c[j] = members ? sh.weight[e][row] : 0.0f;
+                x[j] = (&sh.sum[e >> 1][e & 1][0][0])[f];
+                if (!members) x[j] = make_float4(0, 0, 0, 0);
+                members &= members - 1;
             }
-            const float2 ml = sh.ml[first >> 1][first & 1][row];
-            if (ends == 3) store_out(jid, f, o, ml.y);
-            else {
-                float* to = part_at(blockIdx.x, ends & 1);
-                __stcg(reinterpret_cast<float4*>(to) + f, o);
-                if ((f / 32) % NB == 0 && (f & 31) < 4) __stcg(reinterpret_cast<float2*>(to + R * DIM) + row, ml);
-            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) { o.x = fmaf(x[j].x, c[j], o.x); o.y = fmaf(x[j].y, c[j], o.y); o.z = fmaf(x[j].z, c[j], o.z); o.w = fmaf(x[j].w, c[j], o.w); }
+        }
+        const float2 ml = sh.ml[e0 >> 1][e0 & 1][row];
+        if ((ends & 3) == 3) store_out(sh.seg[e0], f, o, ml.y);
+        else {
+            float* to = part_at(cta, ends & 1);
+            __stcg(reinterpret_cast<float4*>(to) + f, o);
+            if ((f / 32) % NB == 0 && (f & 31) < 4) __stcg(reinterpret_cast<float2*>(to + R * DIM) + row, ml);
         }
     }
-    if (open_job[0] < 0 && open_job[1] < 0) return;
+    // Jobs that other CTAs have parts of: [0] one that began before this CTA, [1] one that begins in it. A lane of each warp finds the
+    // same two.
+    uint32_t open[2] = {0xffffffffu, 0xffffffffu};
+    for (int k = 0; k < runs; k++) {
+        const uint32_t ends = __reduce_or_sync(0xffffffffu, run == k ? sg.ends & 3 : 0u), e = __ffs(__ballot_sync(0xffffffffu, sg.ends && run == k)) - 1;
+        if (ends == 1) open[1] = e;
+        if (!(ends & 1)) open[0] = e;
+    }
+    if ((open[0] & open[1]) == 0xffffffffu) return;
     __threadfence();
     __syncthreads();
     uint32_t first_cta[2], count[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         first_cta[k] = count[k] = 0;
-        if (open_job[k] < 0) continue;
-        const unsigned long long head = open_job[k] / hd.jobs, j = open_job[k] - head * hd.jobs;
-        const unsigned long long j0 = head * hd.tiles + __ldg(pl.job_tile + j), j1 = head * hd.tiles + __ldg(pl.job_tile + j + 1);
-        first_cta[k] = (uint32_t)(((j0 + 1) * grid - 1) / total);
-        count[k] = (uint32_t)((j1 * grid - 1) / total) - first_cta[k] + 1;
+        if (open[k] == 0xffffffffu) continue;
+        const Segment& of = sh.seg[open[k]];
+        if (splits) { first_cta[k] = of.head * splits; count[k] = splits; }
+        else {
+            const uint32_t per = total / grid, more = total - per * grid, wide = more * (per + 1);
+            auto cta_of = [&](uint32_t x) { return x < wide ? x / (per + 1) : more + (x - wide) / per; };
+            first_cta[k] = cta_of(of.head * tiles + __ldg(pl.job_tile + of.job));
+            count[k] = cta_of(of.head * tiles + __ldg(pl.job_tile + of.job + 1) - 1) - first_cta[k] + 1;
+        }
         if (tid == 0 && atomicAdd(a.tickets + first_cta[k], 1u) == count[k] - 1) {
             a.tickets[first_cta[k]] = 0;
             sh.last[k] = 1;
         }
     }
     __syncthreads();
-#pragma unroll 1
+#pragma unroll
     for (int k = 0; k < 2; k++) {
         if (!sh.last[k]) continue;
         __threadfence();
@@ -668,7 +754,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 }
             }
             const float l = sh.total[row];
-            store_out(open_job[k], f, o, l);
+            store_out(sh.seg[open[k]], f, o, l);
         }
         __syncthreads();
     }

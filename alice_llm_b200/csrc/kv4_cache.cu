@@ -34,7 +34,7 @@ __device__ __forceinline__ CodePlace code_place(const RowPlace& p, uint32_t slot
     CodePlace c;
     c.codes = tile + (p.value ? kv4_v_codes(s.dim) + pos * (s.dim / 2) + (p.sub * nb + p.block) * 2
                               : row * (s.dim / 2) + kv4_k_word(nb, p.block, p.sub >> 1) * 4 + (p.sub & 1) * 2);
-    c.scales = tile + (p.value ? kv4_v_scales(s.dim) : kv4_k_scales(s.dim)) + (row * nb + p.block) * 4;
+    c.scales = tile + (p.value ? kv4_v_scales(s.dim) : kv4_k_scales(s.dim)) + row * (4 * nb) + p.block * 2;     // d; m is 2 nb further
     return c;
 }
 
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const __grid_constant__
         if (p.in) {
             const CodePlace c = code_place(p, a.plan.tok_slot[p.tok], a.shape);
             *reinterpret_cast<uint16_t*>(a.pool + c.codes) = (uint16_t)codes;
-            if (p.sub == 0) *reinterpret_cast<__half2*>(a.pool + c.scales) = __halves2half2(d, m);
+            if (p.sub < 2) *reinterpret_cast<__half*>(a.pool + c.scales + p.sub * 2 * nb) = p.sub ? m : d;
         }
     }
 }
@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
         const RowPlace p = row_place(i, n, a.shape);
         const CodePlace c = code_place(p, a.plan.tok_slot[p.tok], a.shape);
         const uint32_t codes = __ldcg(reinterpret_cast<const unsigned short*>(a.pool + c.codes));
-        const uint32_t dm = __ldcg(reinterpret_cast<const unsigned int*>(a.pool + c.scales));
-        const float d = f16_bits_to_f32(dm & 0xffff), m = f16_bits_to_f32(dm >> 16);
+        const float d = f16_bits_to_f32(__ldcg(reinterpret_cast<const unsigned short*>(a.pool + c.scales)));
+        const float m = f16_bits_to_f32(__ldcg(reinterpret_cast<const unsigned short*>(a.pool + c.scales + 2 * nb)));
         float4 o;      // d * code is exact in f32: one rounding
         o.x = __fmaf_rn(d, (float)(codes & 15), m);
         o.y = __fmaf_rn(d, (float)(codes >> 4 & 15), m);
