@@ -46,17 +46,19 @@ struct Kv4Head {
     uint32_t end, top_page;              // positions of the longest sequence, highest page of a table
 };
 
-// A job: up to `rows` consecutive (token, query head of the group) rows of a sequence, against the keys the last of them sees.
+// A job: up to `rows` of Kv4Head consecutive (token, query head of the group) rows of a sequence, against the keys the last of them sees.
+struct alignas(32) Kv4Job {
+    uint32_t seq, row, rows;     // its first row, and how many it has
+    uint32_t first, past;        // of the sequence: row of its first token in q, k, v; positions before it
+    uint32_t tile0, tile1;       // of the tiles of all jobs of a key / value head
+    uint32_t unused;
+};
 struct Kv4Plan {
     const Kv4Head* head;
     const uint32_t* tok_slot;    // [tokens] page * page_tokens + place in it
     const uint32_t* tok_pos;     // [tokens] row of the rotation table: the position
-    const uint32_t* seq_past;    // [seqs]
-    const uint32_t* seq_count;   // [seqs] new tokens
-    const uint32_t* seq_first;   // [seqs] their first row in q, k, v
-    const uint32_t* job_seq;     // [jobs]
-    const uint32_t* job_row;     // [jobs] first row
-    const uint32_t* job_tile;    // [jobs + 1] tiles of the jobs before
+    const Kv4Job* job;           // [jobs]
+    const uint32_t* job_tile;    // [jobs] their tile0 by themselves
     const uint32_t* table;       // [seqs][table_ld] pages
     uint32_t table_ld;
 };

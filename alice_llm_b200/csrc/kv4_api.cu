@@ -124,9 +124,8 @@ int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t
     alice_engine_retain(e);
     size_t at = 0;
     auto take = [&](size_t words) { const size_t o = at; at += (words * 4 + 15) & ~size_t(15); return o; };
-    const size_t o_head = take(sizeof(Kv4Head) / 4), o_past = take(max_seqs), o_count = take(max_seqs), o_first = take(max_seqs), o_jseq = take(b->max_jobs),
-                 o_jrow = take(b->max_jobs), o_jtile = take((size_t)b->max_jobs + 1), o_slot = take(max_tokens), o_pos = take(max_tokens),
-                 o_table = take((size_t)max_seqs * max_pages);
+    const size_t o_job = take((size_t)b->max_jobs * (sizeof(Kv4Job) / 4)), o_head = take(sizeof(Kv4Head) / 4), o_jtile = take(b->max_jobs), o_slot = take(max_tokens),
+                 o_pos = take(max_tokens), o_table = take((size_t)max_seqs * max_pages);
     cudaError_t err = cudaSetDevice(e->device);
     if (err == cudaSuccess) err = cudaMalloc(reinterpret_cast<void**>(&b->blob), at);
     if (err == cudaSuccess) err = cudaMalloc(reinterpret_cast<void**>(&b->part), kv4_part_floats(s.dim, e->num_sms) * sizeof(float));
@@ -137,8 +136,7 @@ int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t
     auto u32 = [&](size_t o) { return reinterpret_cast<const uint32_t*>(b->blob + o); };
     b->plan.head = reinterpret_cast<const Kv4Head*>(b->blob + o_head);
     b->plan.tok_slot = u32(o_slot); b->plan.tok_pos = u32(o_pos);
-    b->plan.seq_past = u32(o_past); b->plan.seq_count = u32(o_count); b->plan.seq_first = u32(o_first);
-    b->plan.job_seq = u32(o_jseq); b->plan.job_row = u32(o_jrow); b->plan.job_tile = u32(o_jtile);
+    b->plan.job = reinterpret_cast<const Kv4Job*>(b->blob + o_job); b->plan.job_tile = u32(o_jtile);
     b->plan.table = u32(o_table); b->plan.table_ld = max_pages;
     *out = b;
     return ALICE_OK;
@@ -181,11 +179,10 @@ int32_t alice_kv4_batch_set(alice_kv4_batch* b, uint32_t seqs, const uint32_t* p
         if (!fits || (uint64_t)h.head.tiles * b->shape.kv_heads > 0x7fffffffull)     // tiles of all heads are numbered in 32 bits
             return alice_fail(ALICE_E_SHAPE, "%s: too many tokens over too many positions for one step", who);
         // copies from pageable memory: the vectors have been read when a call returns
-        auto up = [&](const uint32_t* dst, const std::vector<uint32_t>& src) -> cudaError_t {
-            return src.empty() ? cudaSuccess : cudaMemcpyAsync(const_cast<uint32_t*>(dst), src.data(), src.size() * 4, cudaMemcpyHostToDevice, st);
+        auto up = [&](const auto* dst, const auto& src) -> cudaError_t {
+            return src.empty() ? cudaSuccess : cudaMemcpyAsync(const_cast<void*>(static_cast<const void*>(dst)), src.data(), src.size() * sizeof(src[0]), cudaMemcpyHostToDevice, st);
         };
-        CU(up(b->plan.seq_past, h.past)); CU(up(b->plan.seq_count, h.count)); CU(up(b->plan.seq_first, h.first));
-        CU(up(b->plan.job_seq, h.job_seq)); CU(up(b->plan.job_row, h.job_row)); CU(up(b->plan.job_tile, h.job_tile));
+        CU(up(b->plan.job, h.job)); CU(up(b->plan.job_tile, h.job_tile));
         CU(up(b->plan.tok_slot, h.slot)); CU(up(b->plan.tok_pos, h.pos)); CU(up(b->plan.table, h.table));
         CU(cudaMemcpyAsync(const_cast<Kv4Head*>(b->plan.head), &h.head, sizeof(Kv4Head), cudaMemcpyHostToDevice, st));
         b->now = h.head;

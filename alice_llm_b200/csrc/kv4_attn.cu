@@ -30,11 +30,13 @@ constexpr int STAGES = 4;
 constexpr uint32_t FLUSH = 16;       // tiles
 constexpr uint32_t MAX_CTAS = 192;
 constexpr float ROOM = 8.0f;         // what a score may exceed the reference by, in powers of two
+constexpr float LIFT = 7.0f;         // weights are 2^7 times as large as they are (sums of them too): up to 2^15
 
 // A warp's part of a job that is not all of it.
 struct Segment {
-    uint32_t ends;                       // 1: has the job's first tile, 2: its last; 4: there is one
-    uint32_t head, job, row, rows, first;
+    uint32_t head;
+    uint32_t job, row, first;
+    uint16_t rows, ends;                 // 1: has the job's first tile, 2: its last; 4: there is one
 };
 
 template <int NB, int R>
@@ -42,6 +44,7 @@ struct Cfg {
     static constexpr bool SPLIT = R == 4;
     static constexpr int NT = R == 16 ? 2 : 1;                    // eight-column products
     static constexpr int RT = SPLIT ? 1 : 2 * NT;                 // rows a lane has scores and outputs of
+    static constexpr int TP = R == 16 ? 1 : 2;                    // tiles taken together: as many as the registers hold
     static constexpr int WARPS = NB == 8 ? (R == 4 ? 8 : 6) : R == 4 ? 16 : R == 8 ? 12 : 8;
     static constexpr uint32_t DIM = 32 * NB, TILE = kv4_tile_bytes(DIM);
     static constexpr int NF = NB * RT;                            // float4 of output a lane has
@@ -50,7 +53,7 @@ struct Cfg {
         float4 sum[WARPS][2][NF][32];
         float2 ml[WARPS][2][R];                                   // reference and sum of weights
         Segment seg[2 * WARPS];
-        float weight[2 * WARPS][R], total[R];
+        float aside[WARPS * R * (NB + 1)];                        // of a job's queries: what is beside their operands; then the weights of parts
         uint32_t last[2];
         alignas(16) uint8_t ring[WARPS][STAGES][TILE];
     };
@@ -123,37 +126,21 @@ __device__ __forceinline__ Words<N> lds_words(uint32_t a) {
 template <int N>
 __device__ __forceinline__ float half_of(const Words<N>& x, int i) { return i & 1 ? __high2float(bits_half2(x.w[i / 2])) : __low2float(bits_half2(x.w[i / 2])); }
 
-// 8 consecutive floats of a query, from dim0 on, rotated.
-__device__ __forceinline__ void rotated8(float (&x)[8], const float* q, uint32_t dim0, const float* turn, const Kv4Rope& rope) {
-    auto load8 = [](float (&v)[8], const float* p) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    };
-    load8(x, q + dim0);
-    if (dim0 >= rope.dims) return;
+// 4 consecutive floats of a query, from dim0 on, rotated.
+__device__ __forceinline__ float4 rotated4(const float* q, uint32_t dim0, const float* turn, const Kv4Rope& rope) {
+    auto at = [](const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); };
+    const float4 x = at(q + dim0);
+    if (dim0 >= rope.dims) return x;
     if (rope.neox) {
         const uint32_t half = rope.dims / 2;
         const bool upper = dim0 >= half;
         const uint32_t j = upper ? dim0 - half : dim0;
-        float other[8], w0[8], w1[8];
-        load8(other, q + (upper ? j : dim0 + half));
-        load8(w0, turn + 2 * j);
-        load8(w1, turn + 2 * j + 8);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float sn = e < 4 ? w0[2 * e] : w1[2 * e - 8], cs = e < 4 ? w0[2 * e + 1] : w1[2 * e - 7];
-            x[e] = x[e] * cs + (upper ? other[e] * sn : -(other[e] * sn));
-        }
-    } else {
-        float w[8];
-        load8(w, turn + dim0);
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const float a = x[e], b = x[e + 1];
-            x[e] = a * w[e + 1] - b * w[e];
-            x[e + 1] = a * w[e] + b * w[e + 1];
-        }
+        const float4 o = at(q + (upper ? j : dim0 + half)), w0 = at(turn + 2 * j), w1 = at(turn + 2 * j + 4);
+        const float sg = upper ? 1.0f : -1.0f;
+        return make_float4(x.x * w0.y + sg * (o.x * w0.x), x.y * w0.w + sg * (o.y * w0.z), x.z * w1.y + sg * (o.z * w1.x), x.w * w1.w + sg * (o.w * w1.z));
     }
+    const float4 w = at(turn + dim0);
+    return make_float4(x.x * w.y - x.y * w.x, x.x * w.x + x.y * w.y, x.z * w.w - x.w * w.z, x.z * w.z + x.w * w.w);
 }
 
 // The job that tile x of a key head belongs to: the last with job_tile <= x. All lanes look, 32 places at a time.
@@ -169,25 +156,15 @@ __device__ __forceinline__ uint32_t find_job(const uint32_t* job_tile, uint32_t 
     return lo;
 }
 
-struct Job {
-    uint32_t seq, row, rows, first, past, tile0, tile1;   // row: of the sequence's (token, head) rows; rows: how many it has from there
-};
-__device__ __forceinline__ Job get_job(const Kv4Plan& p, uint32_t j, uint32_t group, uint32_t most) {
-    Job b;
-    b.seq = __ldg(p.job_seq + j); b.row = __ldg(p.job_row + j); b.tile0 = __ldg(p.job_tile + j); b.tile1 = __ldg(p.job_tile + j + 1);
-    b.first = __ldg(p.seq_first + b.seq); b.past = __ldg(p.seq_past + b.seq);
-    b.rows = min(most, __ldg(p.seq_count + b.seq) * group - b.row);
-    return b;
-}
-
 }  // namespace
 
 template <int NB, int R>
 __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using C = Cfg<NB, R>;
-    constexpr int NT = C::NT, RT = C::RT, NF = C::NF, W = C::WARPS;
+    constexpr int NT = C::NT, RT = C::RT, NF = C::NF, W = C::WARPS, TP = C::TP;
     constexpr bool SPLIT = C::SPLIT;
     constexpr uint32_t DIM = C::DIM, TILE = C::TILE;
+    static_assert(sizeof(typename C::Smem) <= 227 * 1024 && NB >= 2, "");
     extern __shared__ __align__(16) uint8_t raw[];
     auto& sh = *reinterpret_cast<typename C::Smem*>(raw);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -237,7 +214,8 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 p_count--;
                 if (p_left == 0) {
                     if (p_new) {
-                        p_seq = __ldg(pl.job_seq + p_job); p_tile0 = __ldg(pl.job_tile + p_job); p_end = __ldg(pl.job_tile + p_job + 1);
+                        const Kv4Job nj = pl.job[p_job];
+                        p_seq = nj.seq; p_tile0 = nj.tile0; p_end = nj.tile1;
                         p_base = 0xffffffffu; p_new = false;
                     }
                     const uint32_t i = p_tile - p_tile0, n = i / per_page, in = i - n * per_page;
@@ -261,95 +239,111 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-#pragma unroll
-        for (int s = 0; s < STAGES - 1; s++) ask(s);
 
         uint32_t stage = 0, slot = 0;
         for (uint32_t at = w0; at < w1;) {
             // ---- a job, or this warp's part of it ----
-            const Job jb = get_job(pl, job, a.group, R);
+            const Kv4Job jb = pl.job[job];
             const uint32_t j0 = head * tiles + jb.tile0, j1 = head * tiles + jb.tile1, end = min(j1, w1);
             const bool has_first = at == j0, has_last = end == j1;
 
-            // queries: columns of the product in the order of a lane's codes, and what each row needs beside them
-            uint32_t qf[NT][NB][SPLIT ? 4 : 8];      // [..][0..3]: (value, or by column value and remainder), [4..7]: remainders
-            uint32_t qm[NT][2];                      // sums of a block's queries, values and remainders: columns of the product with the minima
+            // Queries: rotated, scaled, cut into pairs row by row, then read back as columns of the product in the order of a lane's codes. The
+            // place is that of the job's sums, which have not begun.
+            uint32_t qf[NT][NB][SPLIT ? 4 : 8];      // [..][0..3]: values (or by column values and remainders), [4..7]: remainders
+            uint32_t qm[NT][2];                      // sums of a block's queries, likewise: against the minima
             float factor[RT];
+            {
+                constexpr uint32_t CH = R * DIM / 128, PER = DIM / 4 < 32 ? DIM / 4 : 32;      // pieces of 128 floats; lanes of a row
+                const uint32_t place = smem_u32(&sh.sum[warp][slot][0][0]);      // [row][value, remainder][block][t][4 words]
+                float* const aside = sh.aside + warp * R * (NB + 1);             // [row][sums of blocks, factor]
+                float4 x[CH];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const uint32_t row = SPLIT ? g >> 1 : n * 8 + g;
-                const bool there = row < jb.rows;
-                const uint32_t r = jb.row + (there ? row : 0), tok = r / a.group, qh = head * a.group + r % a.group, at_tok = jb.first + tok;
-                const float* q = a.q + at_tok * a.q_ld + (size_t)qh * DIM;
-                const float* turn = a.rope.table + (size_t)(a.rope.by_token ? at_tok : jb.past + tok) * a.rope.dims;
-                float x[NB][8], top = 0;
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    rotated8(x[b], q, b * 32 + 8 * t, turn, a.rope);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[b][e] = there ? x[b][e] * a.scale : 0.0f;      // log2(e) comes with the factor below: a lone rounding of the score
-                        top = fmaxf(top, fabsf(x[b][e]));
-                    }
+                for (uint32_t c = 0; c < CH; c++) {
+                    const uint32_t at_c = c * 128 + lane * 4, row = at_c / DIM, dim0 = at_c % DIM;
+                    const uint32_t r = jb.row + min(row, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
+                    const float* q = a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM;
+                    x[c] = rotated4(q, dim0, a.rope.table + (size_t)(a.rope.by_token ? at_tok : jb.past + tok) * a.rope.dims, a.rope);
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                int e2 = (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 9;     // the largest into 2^9 .. 2^10
-                e2 = min(max(e2, -100), 120);
-                const float down = pow2(-e2);
-                const float up = pow2(e2);
-                const bool low = SPLIT && (g & 1);
-                float sums[NB];
+                __syncwarp();
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
+                for (uint32_t c = 0; c < CH; c++) {
+                    const uint32_t at_c = c * 128 + lane * 4, row = at_c / DIM, b = at_c % DIM / 32;
+                    const float f = row < jb.rows ? a.scale : 0.0f;
+                    float v[4] = {x[c].x * f, x[c].y * f, x[c].z * f, x[c].w * f};
+                    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                    if (DIM == 256) {      // the other half of the row
+                        const float4 y = x[c ^ 1];
+                        top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x * f), fabsf(y.y * f)), fmaxf(fabsf(y.z * f), fabsf(y.w * f))));
+                    }
+#pragma unroll
+                    for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    int e2 = (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 9;     // the largest into 2^9 .. 2^10
+                    e2 = min(max(e2, -100), 120);
+                    const float down = pow2(-e2);
                     float sum = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) sum += x[b][e] * down;
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    sums[b] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+                    for (int e = 0; e < 4; e++) { v[e] *= down; sum += v[e]; }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float v0 = x[b][e] * down, v1 = x[b][e + 4] * down;
-                        const __half2 hi = __floats2half2_rn(v0, v1);
-                        const float2 back = __half22float2(hi);
-                        const __half2 lo = __floats2half2_rn(v0 - back.x, v1 - back.y);
-                        if (SPLIT) qf[n][b][e] = half2_bits(low ? lo : hi);
-                        else { qf[n][b][e] = half2_bits(hi); qf[n][b][SPLIT ? 0 : 4 + e] = half2_bits(lo); }
+                    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane % 8 == 0) aside[row * (NB + 1) + b] = sum;
+                    if (at_c % DIM == 0) aside[row * (NB + 1) + NB] = pow2(e2) * 1.44269504088896341f;
+                    // dims 8 t + e and 8 t + e + 4 share a word: with the neighbouring lane's
+                    const __half2 h01 = __floats2half2_rn(v[0], v[1]), h23 = __floats2half2_rn(v[2], v[3]);
+                    const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
+                    const uint32_t mine[2][2] = {{half2_bits(h01), half2_bits(h23)},
+                                                 {half2_bits(__floats2half2_rn(v[0] - f01.x, v[1] - f01.y)), half2_bits(__floats2half2_rn(v[2] - f23.x, v[3] - f23.y))}};
+                    const bool odd = lane & 1;
+#pragma unroll
+                    for (int part = 0; part < 2; part++) {
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, mine[part][odd ? 0 : 1], 1), keep = mine[part][odd ? 1 : 0];
+                        // even lane: words 0, 1 of (its, the other's); odd: words 2, 3 of (the other's, its)
+                        const uint32_t lo = odd ? got : keep, hi = odd ? keep : got;
+                        const uint32_t to = place + ((row * 2 + part) * NB + b) * 64 + (lane % 8 / 2) * 16 + (odd ? 8 : 0);
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to), "r"(__byte_perm(lo, hi, 0x5410)), "r"(__byte_perm(lo, hi, 0x7632)) : "memory");
                     }
                 }
-                // The minima of a key are the first columns (of 8 blocks all) of an operand's 16, again as the next; the sums' values and
-                // remainders stand against them.
-                auto pair = [&](int p, bool remainder) -> uint32_t {
-                    const __half2 hi = __floats2half2_rn(sums[2 * p % NB], sums[(2 * p + 1) % NB]);
-                    if (!remainder) return half2_bits(hi);
+                __syncwarp();
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const uint32_t row = SPLIT ? g >> 1 : n * 8 + g;
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int part = 0; part < (SPLIT ? 1 : 2); part++) {
+                            const uint4 w = lds128(place + ((row * 2 + (SPLIT ? g & 1 : part)) * NB + b) * 64 + t * 16);
+                            qf[n][b][part * 4] = w.x; qf[n][b][part * 4 + 1] = w.y; qf[n][b][part * 4 + 2] = w.z; qf[n][b][part * 4 + 3] = w.w;
+                        }
+                    // The minima of a key are the first columns (of 8 blocks all) of an operand's 16, again as the next; the sums' values and
+                    // remainders stand against them.
+                    const uint32_t p = NB == 8 ? t : t % (NB / 2);
+                    const float s0 = aside[row * (NB + 1) + 2 * p], s1 = aside[row * (NB + 1) + 2 * p + 1];
+                    const __half2 hi = __floats2half2_rn(s0, s1);
                     const float2 back = __half22float2(hi);
-                    return half2_bits(__floats2half2_rn(sums[2 * p % NB] - back.x, sums[(2 * p + 1) % NB] - back.y));
-                };
-                uint32_t m0 = 0, m1 = 0;
+                    const uint32_t value = half2_bits(hi), left = half2_bits(__floats2half2_rn(s0 - back.x, s1 - back.y));
+                    qm[n][0] = NB == 8 || t < NB / 2 ? value : t < NB ? left : 0;
+                    qm[n][1] = NB == 8 ? left : 0;
+                    if (SPLIT && (g & 1)) qm[n][0] = qm[n][1] = 0;
+                }
 #pragma unroll
-                for (int p = 0; p < NB / 2; p++) {
-                    if (NB == 8) { if ((int)t == p) { m0 = pair(p, false); m1 = pair(p, true); } }
-                    else {
-                        if ((int)t == p) m0 = pair(p, false);
-                        if ((int)t == p + NB / 2) m0 = pair(p, true);
-                    }
-                }
-                qm[n][0] = low ? 0 : m0; qm[n][1] = low ? 0 : m1;
-                const float f = up;
-                if (SPLIT) factor[0] = __shfl_sync(0xffffffffu, f, t * 8) * 1.44269504088896341f;
-                else {
-                    factor[2 * n % RT] = __shfl_sync(0xffffffffu, f, t * 8) * 1.44269504088896341f;
-                    factor[(2 * n + 1) % RT] = __shfl_sync(0xffffffffu, f, t * 8 + 4) * 1.44269504088896341f;
-                }
+                for (int i = 0; i < RT; i++) factor[i] = aside[(SPLIT ? t : (i >> 1) * 8 + 2 * t + (i & 1)) * (NB + 1) + NB];
+                __syncwarp();
             }
-            uint32_t limit[RT], least = 0xffffffffu;        // positions a row sees
+            // the first tiles are asked for behind the first queries, which would wait for all of them otherwise
+            if (at == w0) {
+#pragma unroll
+                for (int i = 0; i < STAGES; i++) ask(i);
+            }
+            const uint32_t to_key = (end - j0) * KV4_TILE;      // of this warp's part
+            uint32_t limit[RT], least = to_key, far = 0;        // positions a row sees, of this part
 #pragma unroll
             for (int i = 0; i < RT; i++) {
                 const uint32_t row = SPLIT ? t : (i >> 1) * 8 + 2 * t + (i & 1);
-                limit[i] = row < jb.rows ? jb.past + (jb.row + row) / a.group + 1 : 0u;
+                limit[i] = row < jb.rows ? min(to_key, jb.past + (jb.row + row) / a.group + 1) : 0u;
                 if (row < jb.rows) least = min(least, limit[i]);
+                far = max(far, limit[i]);
             }
             least = __reduce_min_sync(0xffffffffu, least);
+            far = __reduce_max_sync(0xffffffffu, far);
 
             float acc[NT][NB][2][4], accm[RT][NB], l[RT], ref[RT], lsum[RT], mref[RT];
 #pragma unroll
@@ -367,7 +361,8 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
 #pragma unroll
                         for (int c = 0; c < 4; c++) acc[n][b][u][c] = 0;
             uint32_t dtop = 0;                  // exponent field of the largest step so far, in the top bits of a half
-            float dscale = 0, dback = 0;        // 2^z on p * d, and 2^-z
+            __half2 dscale = __float2half2_rn(0.0f);      // 2^z on steps
+            float dback = 0;                    // 2^-z
             uint32_t held = 0;                  // tiles in acc
             bool begun = false;                 // sums are in shared memory
             float4* const mine = &sh.sum[warp][slot][0][lane];
@@ -405,176 +400,219 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             };
 
             uint32_t key0 = (at - j0) * KV4_TILE;
-            float s[RT][2], p[RT][2];           // of keys tau(g), 8 + tau(g)
-            Words<NB> va, vb;                   // scales of their values
-            auto scores = [&](uint32_t base) {
-                const uint32_t krow = base + g * (DIM / 2), srow = base + kv4_k_scales(DIM) + g * (4 * NB);
-                // a row of scales: the steps of its blocks, then their minima
-                Words<NB / 2> sa = lds_words<NB / 2>(srow), sb = lds_words<NB / 2>(srow + 32 * NB);
-                const uint32_t mat = srow + 2 * NB + 4 * (t % (NB / 2)), ma = lds32(mat), mb = lds32(mat + 32 * NB);
+            while (at < end) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - TP) : "memory");
+                __syncwarp();
+                uint32_t base[TP];
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float c[4];
-                    mma_f16_first(c, ma, mb, ma, mb, qm[n][0], qm[n][1], zero);
-                    if (SPLIT) { s[0][0] = c[0]; s[0][1] = c[2]; }
-                    else {
+                for (int x = 0; x < TP; x++) base[x] = ring + (stage + x) % STAGES * TILE;
+                float s[TP][RT][2];             // of keys tau(g), 8 + tau(g)
+                // ---- scores: the minima's part, then block by block ----
 #pragma unroll
-                        for (int j = 0; j < 2; j++) { s[(2 * n + j) % RT][0] = c[j]; s[(2 * n + j) % RT][1] = c[2 + j]; }
+                for (int x = 0; x < TP; x++) {
+                    const uint32_t mat = base[x] + kv4_k_scales(DIM) + g * (4 * NB) + 2 * NB + 4 * (t % (NB / 2)), ma = lds32(mat), mb = lds32(mat + 32 * NB);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float c[4];
+                        mma_f16_first(c, ma, mb, ma, mb, qm[n][0], qm[n][1], zero);
+                        if (SPLIT) { s[x][0][0] = c[0]; s[x][0][1] = c[2]; }
+                        else {
+#pragma unroll
+                            for (int j = 0; j < 2; j++) { s[x][(2 * n + j) % RT][0] = c[j]; s[x][(2 * n + j) % RT][1] = c[2 + j]; }
+                        }
                     }
                 }
 #pragma unroll
                 for (int h = 0; h < (NB + 3) / 4; h++) {
                     constexpr int NW = NB < 4 ? NB : 4;
-                    const uint32_t kat = krow + (NB == 8 ? h * 64 + t * 16 : t * NB * 4);
-                    const Words<NW> ka = lds_words<NW>(kat), kb = lds_words<NW>(kat + 4 * DIM);
+                    Words<NW> ka[TP], kb[TP];
+                    Words<NW / 2> sa[TP], sb[TP];
 #pragma unroll
-                    for (int w = 0; w < NW; w++) {
-                        const int b = h * 4 + w;
-                        const Codes xa = unpack<0>(ka.w[w]), xb = unpack<0>(kb.w[w]);
-                        const __half2 ha = bits_half2(sa.w[b / 2]), hb = bits_half2(sb.w[b / 2]);
-                        const float da = b & 1 ? __high2float(ha) : __low2float(ha), db = b & 1 ? __high2float(hb) : __low2float(hb);
+                    for (int x = 0; x < TP; x++) {
+                        const uint32_t kat = base[x] + g * (DIM / 2) + (NB == 8 ? h * 64 + t * 16 : t * NB * 4), srow = base[x] + kv4_k_scales(DIM) + g * (4 * NB) + h * 8;
+                        ka[x] = lds_words<NW>(kat); kb[x] = lds_words<NW>(kat + 4 * DIM);
+                        sa[x] = lds_words<NW / 2>(srow); sb[x] = lds_words<NW / 2>(srow + 32 * NB);
+                    }
 #pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            float c[4];
-                            mma_f16_first(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][0], qf[n][b][1], zero);
-                            mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][2], qf[n][b][3]);
-                            if (!SPLIT) {
-                                mma_f16(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][SPLIT ? 0 : 4], qf[n][b][SPLIT ? 0 : 5]);
-                                mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][SPLIT ? 0 : 6], qf[n][b][SPLIT ? 0 : 7]);
-                            }
-                            if (SPLIT) {
-                                s[0][0] = fmaf(da, c[0] + c[1], s[0][0]);
-                                s[0][1] = fmaf(db, c[2] + c[3], s[0][1]);
-                            } else {
+                    for (int w = 0; w < NW; w++)
 #pragma unroll
-                                for (int j = 0; j < 2; j++) {
-                                    const int i = (2 * n + j) % RT;
-                                    s[i][0] = fmaf(da, c[j], s[i][0]);
-                                    s[i][1] = fmaf(db, c[2 + j], s[i][1]);
+                        for (int x = 0; x < TP; x++) {
+                            const int b = h * 4 + w;
+                            const Codes xa = unpack<0>(ka[x].w[w]), xb = unpack<0>(kb[x].w[w]);
+                            const float da = half_of(sa[x], w), db = half_of(sb[x], w);
+#pragma unroll
+                            for (int n = 0; n < NT; n++) {
+                                float c[4];
+                                mma_f16_first(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][0], qf[n][b][1], zero);
+                                mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][2], qf[n][b][3]);
+                                if (!SPLIT) {
+                                    mma_f16(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][SPLIT ? 0 : 4], qf[n][b][SPLIT ? 0 : 5]);
+                                    mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][SPLIT ? 0 : 6], qf[n][b][SPLIT ? 0 : 7]);
+                                }
+                                if (SPLIT) {
+                                    s[x][0][0] = fmaf(da, c[0] + c[1], s[x][0][0]);
+                                    s[x][0][1] = fmaf(db, c[2] + c[3], s[x][0][1]);
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 2; j++) {
+                                        const int i = (2 * n + j) % RT;
+                                        s[x][i][0] = fmaf(da, c[j], s[x][i][0]);
+                                        s[x][i][1] = fmaf(db, c[2 + j], s[x][i][1]);
+                                    }
                                 }
                             }
                         }
-                    }
                 }
-            };
-            // the scores of a tile are worked out beside the sums of the one before it
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            __syncwarp();
-            scores(ring + stage * TILE);
-            for (; at < end; at++, key0 += KV4_TILE) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 3) : "memory");
-                __syncwarp();
-                ask((stage + STAGES - 1) % STAGES);       // where the tile before this one was: every lane is done with it
-                const uint32_t base = ring + stage * TILE;
-                auto weights = [&](auto edge_t) {
-                constexpr bool edge = decltype(edge_t)::value;       // some row does not see all of the tile
                 // ---- weights ----
-                const uint32_t tau = (g >> 1) + 4 * (g & 1), keyA = key0 + tau, keyB = keyA + 8;
-                const uint32_t vsrow = base + kv4_v_scales(DIM) + g * (4 * NB);
-                va = lds_words<NB>(vsrow); vb = lds_words<NB>(vsrow + 32 * NB);
-                bool move = false;
+                const uint32_t tau = (g >> 1) + 4 * (g & 1), key = key0 + tau;
+                Words<NB> va[TP], vb[TP];       // scales of the values
 #pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    s[i][0] *= factor[i]; s[i][1] *= factor[i];
-                    if (edge) {
-                        if (keyA >= limit[i]) s[i][0] = -INFINITY;
-                        if (keyB >= limit[i]) s[i][1] = -INFINITY;
-                    }
-                    move |= fmaxf(s[i][0], s[i][1]) > ref[i] + ROOM;
+                for (int x = 0; x < TP; x++) {
+                    const uint32_t vsrow = base[x] + kv4_v_scales(DIM) + g * (4 * NB);
+                    va[x] = lds_words<NB>(vsrow); vb[x] = lds_words<NB>(vsrow + 32 * NB);
                 }
-                if (edge) {      // keys that no row sees: whatever lies there has no part
-                    uint32_t far = limit[0];
-#pragma unroll
-                    for (int i = 1; i < RT; i++) far = max(far, limit[i]);
-                    far = __reduce_max_sync(0xffffffffu, far);
-#pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        if (keyA >= far) va.w[b] = 0;
-                        if (keyB >= far) vb.w[b] = 0;
-                    }
-                }
-                __half2 both = __hmax2(bits_half2(va.w[0]), bits_half2(vb.w[0]));
-#pragma unroll
-                for (int b = 1; b < NB / 2; b++) both = __hmax2(both, __hmax2(bits_half2(va.w[b]), bits_half2(vb.w[b])));
-                const uint32_t dmax = max(half2_bits(both) & 0x7c00u, half2_bits(both) >> 16 & 0x7c00u);
-                move |= dmax > dtop;
-                if (__any_sync(0xffffffffu, move)) {
-                    if (held) flush();
-                    dtop = __reduce_max_sync(0xffffffffu, max(dmax, dtop));
-                    // steps below 2^(e + 1), weights up to 2^8: their products into less than 2^15
-                    const int z = 6 - ((int)(dtop >> 10) - 15);
-                    dscale = pow2(z); dback = pow2(-z);
+                auto weights = [&](auto edge_t) {
+                    constexpr bool edge = decltype(edge_t)::value;       // some row does not see all of the tiles
+                    bool move = false;
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
-                        float m = fmaxf(s[i][0], s[i][1]);
+                        float m = -INFINITY;
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        ref[i] = fmaxf(ref[i], m);
+                        for (int x = 0; x < TP; x++)
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                if (edge && key + 16 * x + 8 * k >= limit[i]) s[x][i][k] = -INFINITY;
+                                m = fmaxf(m, s[x][i][k]);
+                            }
+                        move |= m * factor[i] > ref[i] + ROOM;
                     }
-                }
+                    __half2 both = __float2half2_rn(0.0f);
 #pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    p[i][0] = ex2(s[i][0] - ref[i]); p[i][1] = ex2(s[i][1] - ref[i]);
-                    if (edge) {
-                        if (keyA >= limit[i]) p[i][0] = 0;
-                        if (keyB >= limit[i]) p[i][1] = 0;
-                    }
-                    l[i] += p[i][0] + p[i][1];
-                }
-                // minima: of a key that a row does not see not even a NaN
+                    for (int x = 0; x < TP; x++)
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const float ma = fmaf(8.0f, half_of(va, b), half_of(va, NB + b)), mb = fmaf(8.0f, half_of(vb, b), half_of(vb, NB + b));   // what a code of 8 stands for
+                        for (int b = 0; b < NB / 2; b++) {
+                            if (edge) {      // keys that no row sees: whatever lies there has no part
+                                if (key + 16 * x >= far) va[x].w[b] = 0;
+                                if (key + 16 * x + 8 >= far) vb[x].w[b] = 0;
+                            }
+                            both = __hmax2(both, __hmax2(bits_half2(va[x].w[b]), bits_half2(vb[x].w[b])));
+                        }
+                    const uint32_t dmax = max(half2_bits(both) & 0x7c00u, half2_bits(both) >> 16 & 0x7c00u);
+                    move |= dmax > dtop;
+                    if (__any_sync(0xffffffffu, move)) {
+                        if (held) flush();
+                        dtop = __reduce_max_sync(0xffffffffu, max(dmax, dtop));
+                        // steps to below 1, so that with weights up to 2^15 their products stay in range
+                        const int z = 14 - (int)(dtop >> 10);
+                        dscale = __half2half2(__ushort_as_half(z >= -14 ? (z + 15) << 10 : 0x400 >> (-14 - z)));
+                        dback = pow2(-z);
 #pragma unroll
-                    for (int i = 0; i < RT; i++) {
-                        if (!edge) accm[i][b] = fmaf(p[i][0], ma, fmaf(p[i][1], mb, accm[i][b]));
-                        else {
-                            if (keyA < limit[i]) accm[i][b] = fmaf(p[i][0], ma, accm[i][b]);
-                            if (keyB < limit[i]) accm[i][b] = fmaf(p[i][1], mb, accm[i][b]);
+                        for (int i = 0; i < RT; i++) {
+                            float m = fmaxf(s[0][i][0], s[0][i][1]);
+#pragma unroll
+                            for (int x = 1; x < TP; x++) m = fmaxf(m, fmaxf(s[x][i][0], s[x][i][1]));
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+                            ref[i] = fmaxf(ref[i], m * factor[i]);
                         }
                     }
-                }
+#pragma unroll
+                    for (int i = 0; i < RT; i++)
+#pragma unroll
+                        for (int x = 0; x < TP; x++) {
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                s[x][i][k] = ex2(fmaf(s[x][i][k], factor[i], LIFT - ref[i]));
+                                if (edge && key + 16 * x + 8 * k >= limit[i]) s[x][i][k] = 0;
+                            }
+                            l[i] += s[x][i][0] + s[x][i][1];
+                        }
+                    // minima: of a key that a row does not see not even a NaN
+#pragma unroll
+                    for (int x = 0; x < TP; x++)
+#pragma unroll
+                        for (int b = 0; b < NB; b++) {
+                            const float ma = fmaf(8.0f, half_of(va[x], b), half_of(va[x], NB + b)), mb = fmaf(8.0f, half_of(vb[x], b), half_of(vb[x], NB + b));   // what a code of 8 stands for
+#pragma unroll
+                            for (int i = 0; i < RT; i++) {
+                                if (!edge) accm[i][b] = fmaf(s[x][i][0], ma, fmaf(s[x][i][1], mb, accm[i][b]));
+                                else {
+                                    if (key + 16 * x < limit[i]) accm[i][b] = fmaf(s[x][i][0], ma, accm[i][b]);
+                                    if (key + 16 * x + 8 < limit[i]) accm[i][b] = fmaf(s[x][i][1], mb, accm[i][b]);
+                                }
+                            }
+                        }
                 };
-                auto values = [&]() {
-                Words<(NB + 1) / 2> v[4];
-                const uint32_t vrow = base + kv4_v_codes(DIM) + t * (DIM / 2) + g * (2 * NB);
+                if (key0 + KV4_TILE * TP > least) weights(std::true_type{}); else weights(std::false_type{});
+                // ---- values: weight times step as a pair of half-precision numbers, from the weight's pair ----
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = lds_words<(NB + 1) / 2>(vrow + i * 2 * DIM);
+                for (int x = 0; x < TP; x++) {
+                    Words<(NB + 1) / 2> v[4];
+                    const uint32_t vrow = base[x] + kv4_v_codes(DIM) + t * (DIM / 2) + g * (2 * NB);
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const uint32_t pick = b & 1 ? 0x7632u : 0x5410u;
-                    const uint32_t xa = __byte_perm(v[0].w[b / 2], v[1].w[b / 2], pick), xb = __byte_perm(v[2].w[b / 2], v[3].w[b / 2], pick);
-                    const Codes ca = unpack<8>(xa), cb = unpack<8>(xb);
-                    const float da = half_of(va, b), db = half_of(vb, b), dax = da * dscale, dbx = db * dscale;
+                    for (int i = 0; i < 4; i++) v[i] = lds_words<(NB + 1) / 2>(vrow + i * 2 * DIM);
+                    __half2 ph[NT][2], pl[NT][2];       // of two rows, or of one twice
 #pragma unroll
-                    for (int n = 0; n < NT; n++) {
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const float p0 = s[x][SPLIT ? 0 : 2 * n % RT][k], p1 = s[x][SPLIT ? 0 : (2 * n + 1) % RT][k];
+                            ph[n][k] = __floats2half2_rn(p0, p1);
+                            const float2 back = __half22float2(ph[n][k]);
+                            pl[n][k] = __floats2half2_rn(p0 - back.x, p1 - back.y);
+                        }
+#pragma unroll
+                    for (int b2 = 0; b2 < NB / 2; b2++) {
+                        const __half2 d2[2] = {__hmul2(bits_half2(va[x].w[b2]), dscale), __hmul2(bits_half2(vb[x].w[b2]), dscale)};
+                        Codes ca[2], cb[2];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t pick = u ? 0x7632u : 0x5410u;
+                            ca[u] = unpack<8>(__byte_perm(v[0].w[b2], v[1].w[b2], pick));
+                            cb[u] = unpack<8>(__byte_perm(v[2].w[b2], v[3].w[b2], pick));
+                        }
+                        // w1 = p d to half precision, w2 = what is missing: p's value times d less w1 is exact
+                        auto product = [](__half2 hi, __half2 lo, __half2 d, __half2& w1, __half2& w2) {
+                            w1 = __hmul2(hi, d);
+                            w2 = __hfma2(lo, d, __hfma2(hi, d, __hneg2(w1)));
+                        };
                         if (SPLIT) {
-                            const float wa = p[0][0] * dax, wb = p[0][1] * dbx;
-                            const __half ha = __float2half_rn(wa), hb = __float2half_rn(wb);
-                            const uint32_t b0 = transposed(half2_bits(__halves2half2(ha, __float2half_rn(wa - __half2float(ha)))));
-                            const uint32_t b1 = transposed(half2_bits(__halves2half2(hb, __float2half_rn(wb - __half2float(hb)))));
-                            mma_f16(acc[0][b][0], ca.v[0], ca.v[1], cb.v[0], cb.v[1], b0, b1);
-                            mma_f16(acc[0][b][1], ca.v[2], ca.v[3], cb.v[2], cb.v[3], b0, b1);
+                            __half2 w1[2], w2[2];
+#pragma unroll
+                            for (int k = 0; k < 2; k++) product(ph[0][k], pl[0][k], d2[k], w1[k], w2[k]);
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const uint32_t pick = u ? 0x7632u : 0x5410u;
+                                const uint32_t b0 = transposed(__byte_perm(half2_bits(w1[0]), half2_bits(w2[0]), pick)), b1 = transposed(__byte_perm(half2_bits(w1[1]), half2_bits(w2[1]), pick));
+                                mma_f16(acc[0][2 * b2 + u][0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], b0, b1);
+                                mma_f16(acc[0][2 * b2 + u][1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], b0, b1);
+                            }
                         } else {
-                            const int i = 2 * n % RT, j = (2 * n + 1) % RT;
-                            const float a0 = p[i][0] * dax, a1 = p[j][0] * dax, e0 = p[i][1] * dbx, e1 = p[j][1] * dbx;
-                            const __half2 ha = __floats2half2_rn(a0, a1), hb = __floats2half2_rn(e0, e1);
-                            const float2 fa = __half22float2(ha), fb = __half22float2(hb);
-                            const uint32_t b0 = transposed(half2_bits(ha)), b1 = transposed(half2_bits(hb));
-                            const uint32_t d0 = transposed(half2_bits(__floats2half2_rn(a0 - fa.x, a1 - fa.y))), d1 = transposed(half2_bits(__floats2half2_rn(e0 - fb.x, e1 - fb.y)));
-                            mma_f16(acc[n][b][0], ca.v[0], ca.v[1], cb.v[0], cb.v[1], b0, b1);
-                            mma_f16(acc[n][b][1], ca.v[2], ca.v[3], cb.v[2], cb.v[3], b0, b1);
-                            mma_f16(acc[n][b][0], ca.v[0], ca.v[1], cb.v[0], cb.v[1], d0, d1);
-                            mma_f16(acc[n][b][1], ca.v[2], ca.v[3], cb.v[2], cb.v[3], d0, d1);
+#pragma unroll
+                            for (int u = 0; u < 2; u++)
+#pragma unroll
+                                for (int n = 0; n < NT; n++) {
+                                    __half2 w1[2], w2[2];
+#pragma unroll
+                                    for (int k = 0; k < 2; k++) product(ph[n][k], pl[n][k], u ? __high2half2(d2[k]) : __low2half2(d2[k]), w1[k], w2[k]);
+                                    float (&o)[2][4] = acc[n][2 * b2 + u];
+                                    const uint32_t b0 = transposed(half2_bits(w1[0])), b1 = transposed(half2_bits(w1[1])), e0 = transposed(half2_bits(w2[0])), e1 = transposed(half2_bits(w2[1]));
+                                    mma_f16(o[0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], b0, b1);
+                                    mma_f16(o[1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], b0, b1);
+                                    mma_f16(o[0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], e0, e1);
+                                    mma_f16(o[1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], e0, e1);
+                                }
                         }
                     }
                 }
-                };
-                if (key0 + KV4_TILE > least) weights(std::true_type{}); else weights(std::false_type{});
-                stage = stage + 1 == STAGES ? 0 : stage + 1;
-                if (at + 1 < end) { scores(ring + stage * TILE); values(); } else values();
-                held++;
-                if (held == FLUSH) flush();
+                __syncwarp();
+                ask(stage);
+                stage = (stage + 1) % STAGES; at++; held++; key0 += KV4_TILE;
+                if (TP == 2 && at < end) {
+                    ask(stage);
+                    stage = (stage + 1) % STAGES; at++; held++; key0 += KV4_TILE;
+                }
+                if (held >= FLUSH) flush();
             }
             if (held) flush();
 
@@ -598,7 +636,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
 #pragma unroll
                     for (int i = 0; i < RT; i++) sh.ml[warp][slot][SPLIT ? t : (i >> 1) * 8 + 2 * t + (i & 1)] = make_float2(mref[i], lsum[i]);
                 }
-                if (lane == 0) sh.seg[2 * warp + slot] = Segment{4u | (has_first ? 1u : 0u) | (has_last ? 2u : 0u), head, job, jb.row, jb.rows, jb.first};
+                if (lane == 0) sh.seg[2 * warp + slot] = Segment{head, job, jb.row, jb.first, (uint16_t)jb.rows, (uint16_t)(4u | (has_first ? 1u : 0u) | (has_last ? 2u : 0u))};
             }
             slot = 1;
             if (has_last) {
@@ -641,7 +679,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             if (__shfl_up_sync(0xffffffffu, run, o) == run && (int)lane >= o) l += v;
         }
         l = __shfl_sync(0xffffffffu, l, last);
-        if (sg.ends) { sh.weight[lane][row] = c; sh.ml[lane >> 1][lane & 1][row] = make_float2(m, l); }
+        if (sg.ends) { sh.aside[lane * R + row] = c; sh.ml[lane >> 1][lane & 1][row] = make_float2(m, l); }
     }
     __syncthreads();
     // a row's place in the fragments: element f = (i * NB + b) * 32 + lane
@@ -659,7 +697,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     for (uint32_t i = tid; i < runs * NE; i += W * 32) {
         const uint32_t k = i / NE, f = i % NE, row = row_of(f);
         uint32_t members = __ballot_sync(0xffffffffu, sg.ends && run == (int)k);
-        const uint32_t ends = __reduce_or_sync(0xffffffffu, run == (int)k ? sg.ends : 0u), e0 = __ffs(members) - 1;
+        const uint32_t ends = __reduce_or_sync(0xffffffffu, run == (int)k ? (uint32_t)sg.ends : 0u), e0 = __ffs(members) - 1;
         float4 o = make_float4(0, 0, 0, 0);
         while (members) {        // four at a time
             float c[4];
@@ -667,7 +705,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const uint32_t e = members ? __ffs(members) - 1 : e0;
-                c[j] = members ? sh.weight[e][row] : 0.0f;
+                c[j] = members ? sh.aside[e * R + row] : 0.0f;
                 x[j] = (&sh.sum[e >> 1][e & 1][0][0])[f];
                 if (!members) x[j] = make_float4(0, 0, 0, 0);
                 members &= members - 1;
@@ -687,7 +725,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     // same two.
     uint32_t open[2] = {0xffffffffu, 0xffffffffu};
     for (int k = 0; k < runs; k++) {
-        const uint32_t ends = __reduce_or_sync(0xffffffffu, run == k ? sg.ends & 3 : 0u), e = __ffs(__ballot_sync(0xffffffffu, sg.ends && run == k)) - 1;
+        const uint32_t ends = __reduce_or_sync(0xffffffffu, run == k ? sg.ends & 3u : 0u), e = __ffs(__ballot_sync(0xffffffffu, sg.ends && run == k)) - 1;
         if (ends == 1) open[1] = e;
         if (!(ends & 1)) open[0] = e;
     }
@@ -704,8 +742,8 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         else {
             const uint32_t per = total / grid, more = total - per * grid, wide = more * (per + 1);
             auto cta_of = [&](uint32_t x) { return x < wide ? x / (per + 1) : more + (x - wide) / per; };
-            first_cta[k] = cta_of(of.head * tiles + __ldg(pl.job_tile + of.job));
-            count[k] = cta_of(of.head * tiles + __ldg(pl.job_tile + of.job + 1) - 1) - first_cta[k] + 1;
+            first_cta[k] = cta_of(of.head * tiles + pl.job[of.job].tile0);
+            count[k] = cta_of(of.head * tiles + pl.job[of.job].tile1 - 1) - first_cta[k] + 1;
         }
         if (tid == 0 && atomicAdd(a.tickets + first_cta[k], 1u) == count[k] - 1) {
             a.tickets[first_cta[k]] = 0;
@@ -736,7 +774,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             }
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane == 0) sh.total[row] = l;
+            if (lane == 0) sh.aside[2 * W * R + row] = l;
         }
         __syncthreads();
         for (uint32_t f = tid; f < NF * 32; f += W * 32) {
@@ -753,7 +791,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                     o.x = fmaf(x[c].x, w, o.x); o.y = fmaf(x[c].y, w, o.y); o.z = fmaf(x[c].z, w, o.z); o.w = fmaf(x[c].w, w, o.w);
                 }
             }
-            const float l = sh.total[row];
+            const float l = sh.aside[2 * W * R + row];
             store_out(sh.seg[open[k]], f, o, l);
         }
         __syncthreads();

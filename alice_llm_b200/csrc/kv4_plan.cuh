@@ -61,7 +61,8 @@ inline int kv4_check_batch(const char* who, uint32_t pages, uint32_t page_tokens
 
 struct Kv4HostPlan {
     Kv4Head head{};
-    std::vector<uint32_t> past, count, first, job_seq, job_row, job_tile, slot, pos, table;
+    std::vector<uint32_t> job_tile, slot, pos, table;
+    std::vector<Kv4Job> job;
 };
 
 // Of checked arguments. Rows of one job see up to `last` keys, those of its last token. false: more than 2^31 tiles.
@@ -71,11 +72,9 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t page_tokens, ui
     uint64_t tiles = 0;
     for (uint32_t s = 0; s < seqs; s++) most = std::max(most, tokens[s] * group);
     const uint32_t rows = kv4_job_rows(most, dim);
-    h.past.assign(past, past + seqs); h.count.assign(tokens, tokens + seqs);
     h.table.assign((size_t)seqs * max_pages, 0);
-    h.job_tile.push_back(0);
     for (uint32_t s = 0; s < seqs; s++) {
-        h.first.push_back(total);
+        const uint32_t first = total;
         total += tokens[s];
         if (!tokens[s]) continue;
         const uint32_t end = past[s] + tokens[s], need = (end + page_tokens - 1) / page_tokens;
@@ -89,13 +88,13 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t page_tokens, ui
             h.slot.push_back(t[at / page_tokens] * page_tokens + at % page_tokens);
         }
         for (uint32_t r = 0; r < tokens[s] * group; r += rows) {
-            const uint32_t last = past[s] + std::min(r + rows - 1, tokens[s] * group - 1) / group + 1;
-            h.job_seq.push_back(s); h.job_row.push_back(r);
+            const uint32_t n = std::min(rows, tokens[s] * group - r), last = past[s] + (r + n - 1) / group + 1, tile0 = (uint32_t)tiles;
             tiles += (last + KV4_TILE - 1) / KV4_TILE;
-            h.job_tile.push_back((uint32_t)tiles);
+            h.job.push_back({s, r, n, first, past[s], tile0, (uint32_t)tiles, 0});
+            h.job_tile.push_back(tile0);
         }
     }
-    h.head.seqs = seqs; h.head.tokens = total; h.head.jobs = (uint32_t)h.job_seq.size(); h.head.rows = rows; h.head.tiles = h.job_tile.back();
+    h.head.seqs = seqs; h.head.tokens = total; h.head.jobs = (uint32_t)h.job.size(); h.head.rows = rows; h.head.tiles = (uint32_t)tiles;
     return tiles <= 0x7fffffffull;
 }
 
