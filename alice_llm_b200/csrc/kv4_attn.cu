@@ -26,11 +26,38 @@ namespace alice {
 
 namespace {
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 constexpr int STAGES = 4;
 constexpr uint32_t FLUSH = 16;       // tiles
-constexpr uint32_t MAX_CTAS = 192;
 constexpr float ROOM = 8.0f;         // what a score may exceed the reference by, in powers of two
 constexpr float LIFT = 7.0f;         // weights are 2^7 times as large as they are (sums of them too): up to 2^15
+
+// Parts of a row's sums brought to one reference, N at a time.
+template <int N>
+struct Joined {
+    float m = -INFINITY, l = 0;
+    float4 sum = make_float4(0, 0, 0, 0);
+    __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&x)[N], int n) {      // the first n count
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < N; j++) top = fmaxf(top, j < n ? ml[j].x : -INFINITY);
+        float c = m == top ? 1.0f : ex2(m - top);
+        l *= c; sum.x *= c; sum.y *= c; sum.z *= c; sum.w *= c;
+        m = top;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            if (j >= n) continue;
+            c = ml[j].x == top ? 1.0f : ex2(ml[j].x - top);
+            l = fmaf(ml[j].y, c, l);
+            sum.x = fmaf(x[j].x, c, sum.x); sum.y = fmaf(x[j].y, c, sum.y); sum.z = fmaf(x[j].z, c, sum.z); sum.w = fmaf(x[j].w, c, sum.w);
+        }
+    }
+};
 
 // A warp's part of a job that is not all of it.
 struct Segment {
@@ -44,8 +71,8 @@ struct Cfg {
     static constexpr bool SPLIT = R == 4;
     static constexpr int NT = R == 16 ? 2 : 1;                    // eight-column products
     static constexpr int RT = SPLIT ? 1 : 2 * NT;                 // rows a lane has scores and outputs of
-    static constexpr int TP = R == 16 ? 1 : 2;                    // tiles taken together: as many as the registers hold
-    static constexpr int WARPS = NB == 8 ? (R == 4 ? 8 : 6) : R == 4 ? 16 : R == 8 ? 12 : 8;
+    static constexpr int TP = R == 16 || NB == 8 ? 1 : 2;                    // tiles taken together: as many as the registers hold
+    static constexpr int WARPS = NB == 8 ? (R == 4 ? 8 : 6) : R == 4 ? 12 : 8;
     static constexpr uint32_t DIM = 32 * NB, TILE = kv4_tile_bytes(DIM);
     static constexpr int NF = NB * RT;                            // float4 of output a lane has
     static constexpr uint32_t PART = R * DIM + 2 * R;             // floats of a part of a job
@@ -53,7 +80,7 @@ struct Cfg {
         float4 sum[WARPS][2][NF][32];
         float2 ml[WARPS][2][R];                                   // reference and sum of weights
         Segment seg[2 * WARPS];
-        float aside[WARPS * R * (NB + 1)];                        // of a job's queries: what is beside their operands; then the weights of parts
+        float aside[WARPS * R * (NB + 1)];                        // of a job's queries: what is beside their operands
         uint32_t last[2];
         alignas(16) uint8_t ring[WARPS][STAGES][TILE];
     };
@@ -100,11 +127,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     return r;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }    // -126 <= e <= 127
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 
 // Words of a row that a lane reads in one go.
@@ -126,21 +148,38 @@ __device__ __forceinline__ Words<N> lds_words(uint32_t a) {
 template <int N>
 __device__ __forceinline__ float half_of(const Words<N>& x, int i) { return i & 1 ? __high2float(bits_half2(x.w[i / 2])) : __low2float(bits_half2(x.w[i / 2])); }
 
-// 4 consecutive floats of a query, from dim0 on, rotated.
-__device__ __forceinline__ float4 rotated4(const float* q, uint32_t dim0, const float* turn, const Kv4Rope& rope) {
+// (sin, cos) of the pairs that dims dim0 .. dim0 + 3 are in: of two pairs, or (pairs half a head apart) of four.
+struct Turn { float4 a, b; };
+__device__ __forceinline__ Turn turn_at(const float* turn, uint32_t dim0, const Kv4Rope& rope) {
     auto at = [](const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); };
-    const float4 x = at(q + dim0);
-    if (dim0 >= rope.dims) return x;
-    if (rope.neox) {
-        const uint32_t half = rope.dims / 2;
-        const bool upper = dim0 >= half;
-        const uint32_t j = upper ? dim0 - half : dim0;
-        const float4 o = at(q + (upper ? j : dim0 + half)), w0 = at(turn + 2 * j), w1 = at(turn + 2 * j + 4);
-        const float sg = upper ? 1.0f : -1.0f;
-        return make_float4(x.x * w0.y + sg * (o.x * w0.x), x.y * w0.w + sg * (o.y * w0.z), x.z * w1.y + sg * (o.z * w1.x), x.w * w1.w + sg * (o.w * w1.z));
+    Turn w{};
+    if (dim0 < rope.dims) {
+        const uint32_t half = rope.dims / 2, j = rope.neox ? 2 * (dim0 < half ? dim0 : dim0 - half) : dim0;
+        w.a = at(turn + j);
+        if (rope.neox) w.b = at(turn + j + 4);
     }
-    const float4 w = at(turn + dim0);
-    return make_float4(x.x * w.y - x.y * w.x, x.x * w.x + x.y * w.y, x.z * w.w - x.w * w.z, x.z * w.z + x.w * w.w);
+    return w;
+}
+// 4 consecutive floats of a query, those of piece k (of 128 dims) from dim0 on, rotated. The lanes of a row hold it 4 dims a lane and piece.
+template <int PIECES>
+__device__ __forceinline__ float4 rotated4(const float4 (&row)[PIECES], int k, uint32_t dim0, const Turn& w, const Kv4Rope& rope) {
+    const float4 x = row[k];
+    if (rope.neox) {
+        const uint32_t half = rope.dims / 2, lane = threadIdx.x & 31;
+        const bool in = dim0 < rope.dims, upper = dim0 >= half;
+        const uint32_t other = upper ? dim0 - half : dim0 + half, from = in ? lane + other / 4 - dim0 / 4 & 31 : lane;      // a piece is 32 lanes, or all of the row
+        float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) {
+            const float4 y = make_float4(__shfl_sync(0xffffffffu, row[i].x, from), __shfl_sync(0xffffffffu, row[i].y, from), __shfl_sync(0xffffffffu, row[i].z, from), __shfl_sync(0xffffffffu, row[i].w, from));
+            if (PIECES == 1 || other / 128 == (uint32_t)i) o = y;
+        }
+        if (!in) return x;
+        const float sg = upper ? 1.0f : -1.0f;
+        return make_float4(x.x * w.a.y + sg * (o.x * w.a.x), x.y * w.a.w + sg * (o.y * w.a.z), x.z * w.b.y + sg * (o.z * w.b.x), x.w * w.b.w + sg * (o.w * w.b.z));
+    }
+    if (dim0 >= rope.dims) return x;
+    return make_float4(x.x * w.a.y - x.y * w.a.x, x.x * w.a.x + x.y * w.a.y, x.z * w.a.w - x.w * w.a.z, x.z * w.a.z + x.w * w.a.w);
 }
 
 // The job that tile x of a key head belongs to: the last with job_tile <= x. All lanes look, 32 places at a time.
@@ -209,24 +248,29 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         const uint8_t* p_src = nullptr;
         uint32_t p_count = w1 - w0;
         bool p_new = true;
+        uint32_t p_n = 0, p_in = 0;
+        auto look = [&]() {          // asks for the page of the next tile,
+            if (p_new) {
+                const Kv4Job nj = pl.job[p_job];
+                p_seq = nj.seq; p_tile0 = nj.tile0; p_end = nj.tile1;
+                p_base = 0xffffffffu; p_new = false;
+            }
+            const uint32_t i = p_tile - p_tile0;
+            p_n = i / per_page; p_in = i - p_n * per_page;
+            if (p_base == 0xffffffffu || p_n >= p_base + 32) {
+                p_base = p_n;
+                p_pages = __ldg(pl.table + (size_t)p_seq * pl.table_ld + min(p_n + lane, (p_end - 1 - p_tile0) / per_page));
+            }
+        };
+        auto found = [&]() {         // and has it
+            const uint32_t page = __shfl_sync(0xffffffffu, p_pages, p_n - p_base);
+            p_src = a.pool + (((size_t)page * a.shape.kv_heads + p_head) * per_page + p_in) * TILE + lane * 16;
+            p_left = min(per_page - p_in, p_end - p_tile);
+        };
         auto ask = [&](uint32_t stage) {
             if (p_count) {
                 p_count--;
-                if (p_left == 0) {
-                    if (p_new) {
-                        const Kv4Job nj = pl.job[p_job];
-                        p_seq = nj.seq; p_tile0 = nj.tile0; p_end = nj.tile1;
-                        p_base = 0xffffffffu; p_new = false;
-                    }
-                    const uint32_t i = p_tile - p_tile0, n = i / per_page, in = i - n * per_page;
-                    if (p_base == 0xffffffffu || n >= p_base + 32) {
-                        p_base = n;
-                        p_pages = __ldg(pl.table + (size_t)p_seq * pl.table_ld + min(n + lane, (p_end - 1 - p_tile0) / per_page));
-                    }
-                    const uint32_t page = __shfl_sync(0xffffffffu, p_pages, n - p_base);
-                    p_src = a.pool + (((size_t)page * a.shape.kv_heads + p_head) * per_page + in) * TILE + lane * 16;
-                    p_left = min(per_page - in, p_end - p_tile);
-                }
+                if (p_left == 0) { look(); found(); }
                 const uint32_t dst = ring + stage * TILE + lane * 16;
 #pragma unroll
                 for (uint32_t c = 0; c < (TILE / 16 + 31) / 32; c++)
@@ -240,6 +284,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
+        look();
         uint32_t stage = 0, slot = 0;
         for (uint32_t at = w0; at < w1;) {
             // ---- a job, or this warp's part of it ----
@@ -257,12 +302,28 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 const uint32_t place = smem_u32(&sh.sum[warp][slot][0][0]);      // [row][value, remainder][block][t][4 words]
                 float* const aside = sh.aside + warp * R * (NB + 1);             // [row][sums of blocks, factor]
                 float4 x[CH];
+                uint32_t of[CH];          // row of the rotation table
 #pragma unroll
                 for (uint32_t c = 0; c < CH; c++) {
                     const uint32_t at_c = c * 128 + lane * 4, row = at_c / DIM, dim0 = at_c % DIM;
                     const uint32_t r = jb.row + min(row, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
-                    const float* q = a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM;
-                    x[c] = rotated4(q, dim0, a.rope.table + (size_t)(a.rope.by_token ? at_tok : jb.past + tok) * a.rope.dims, a.rope);
+                    x[c] = __ldg(reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0));
+                    of[c] = a.rope.by_token ? at_tok : jb.past + tok;
+                }
+                if (a.rope.dims) {
+                    constexpr uint32_t PER_ROW = DIM > 128 ? DIM / 128 : 1;
+                    Turn w[PER_ROW];
+#pragma unroll
+                    for (uint32_t c = 0; c < CH; c += PER_ROW) {
+#pragma unroll
+                        for (uint32_t k = 0; k < PER_ROW; k++)      // rows of one token share it
+                            if (c == 0 || of[c] != of[c >= PER_ROW ? c - PER_ROW : 0]) w[k] = turn_at(a.rope.table + (size_t)of[c] * a.rope.dims, lane * 4 % DIM + 128 * k, a.rope);
+                        float4 y[PER_ROW];
+#pragma unroll
+                        for (uint32_t k = 0; k < PER_ROW; k++) y[k] = x[c + k];
+#pragma unroll
+                        for (uint32_t k = 0; k < PER_ROW; k++) x[c + k] = rotated4(y, k, lane * 4 % DIM + 128 * k, w[k], a.rope);
+                    }
                 }
                 __syncwarp();
 #pragma unroll
@@ -330,6 +391,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             }
             // the first tiles are asked for behind the first queries, which would wait for all of them otherwise
             if (at == w0) {
+                found();
 #pragma unroll
                 for (int i = 0; i < STAGES; i++) ask(i);
             }
@@ -433,35 +495,50 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         ka[x] = lds_words<NW>(kat); kb[x] = lds_words<NW>(kat + 4 * DIM);
                         sa[x] = lds_words<NW / 2>(srow); sb[x] = lds_words<NW / 2>(srow + 32 * NB);
                     }
+                    // two blocks of every tile side by side: a product's sum is waited for by the next one of its chain
 #pragma unroll
-                    for (int w = 0; w < NW; w++)
+                    for (int w = 0; w < NW; w += 2) {
+                        Codes xa[2][TP], xb[2][TP];
+                        float c[2][TP][NT][4];
 #pragma unroll
-                        for (int x = 0; x < TP; x++) {
-                            const int b = h * 4 + w;
-                            const Codes xa = unpack<0>(ka[x].w[w]), xb = unpack<0>(kb[x].w[w]);
-                            const float da = half_of(sa[x], w), db = half_of(sb[x], w);
+                        for (int u = 0; u < 2; u++)
 #pragma unroll
-                            for (int n = 0; n < NT; n++) {
-                                float c[4];
-                                mma_f16_first(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][0], qf[n][b][1], zero);
-                                mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][2], qf[n][b][3]);
-                                if (!SPLIT) {
-                                    mma_f16(c, xa.v[0], xb.v[0], xa.v[1], xb.v[1], qf[n][b][SPLIT ? 0 : 4], qf[n][b][SPLIT ? 0 : 5]);
-                                    mma_f16(c, xa.v[2], xb.v[2], xa.v[3], xb.v[3], qf[n][b][SPLIT ? 0 : 6], qf[n][b][SPLIT ? 0 : 7]);
-                                }
-                                if (SPLIT) {
-                                    s[x][0][0] = fmaf(da, c[0] + c[1], s[x][0][0]);
-                                    s[x][0][1] = fmaf(db, c[2] + c[3], s[x][0][1]);
-                                } else {
+                            for (int x = 0; x < TP; x++) { xa[u][x] = unpack<0>(ka[x].w[w + u]); xb[u][x] = unpack<0>(kb[x].w[w + u]); }
 #pragma unroll
-                                    for (int j = 0; j < 2; j++) {
-                                        const int i = (2 * n + j) % RT;
-                                        s[x][i][0] = fmaf(da, c[j], s[x][i][0]);
-                                        s[x][i][1] = fmaf(db, c[2 + j], s[x][i][1]);
+                        for (int step = 0; step < (SPLIT ? 2 : 4); step++)
+#pragma unroll
+                            for (int u = 0; u < 2; u++)
+#pragma unroll
+                                for (int x = 0; x < TP; x++)
+#pragma unroll
+                                    for (int n = 0; n < NT; n++) {
+                                        const int b = h * 4 + w + u, o = step & 1 ? 2 : 0;
+                                        const uint32_t q0 = qf[n][b][SPLIT ? o : 2 * step], q1 = qf[n][b][SPLIT ? o + 1 : 2 * step + 1];
+                                        if (step == 0) mma_f16_first(c[u][x][n], xa[u][x].v[o], xb[u][x].v[o], xa[u][x].v[o + 1], xb[u][x].v[o + 1], q0, q1, zero);
+                                        else mma_f16(c[u][x][n], xa[u][x].v[o], xb[u][x].v[o], xa[u][x].v[o + 1], xb[u][x].v[o + 1], q0, q1);
+                                    }
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int x = 0; x < TP; x++) {
+                                const float da = half_of(sa[x], w + u), db = half_of(sb[x], w + u);
+#pragma unroll
+                                for (int n = 0; n < NT; n++) {
+                                    const float (&y)[4] = c[u][x][n];
+                                    if (SPLIT) {
+                                        s[x][0][0] = fmaf(da, y[0] + y[1], s[x][0][0]);
+                                        s[x][0][1] = fmaf(db, y[2] + y[3], s[x][0][1]);
+                                    } else {
+#pragma unroll
+                                        for (int j = 0; j < 2; j++) {
+                                            const int i = (2 * n + j) % RT;
+                                            s[x][i][0] = fmaf(da, y[j], s[x][i][0]);
+                                            s[x][i][1] = fmaf(db, y[2 + j], s[x][i][1]);
+                                        }
                                     }
                                 }
                             }
-                        }
+                    }
                 }
                 // ---- weights ----
                 const uint32_t tau = (g >> 1) + 4 * (g & 1), key = key0 + tau;
@@ -659,29 +736,6 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     const uint32_t pj = __shfl_sync(0xffffffffu, sg.job, before), ph = __shfl_sync(0xffffffffu, sg.head, before);
     const uint32_t starts = __ballot_sync(0xffffffffu, sg.ends && (!below || pj != sg.job || ph != sg.head));
     const int runs = __popc(starts), run = __popc(starts & (0xffffffffu >> (31 - lane))) - 1;
-    // weights of the parts: a warp a row
-    for (uint32_t row = warp; row < R; row += W) {
-        const float2 ml = sg.ends ? sh.ml[lane >> 1][lane & 1][row] : make_float2(-INFINITY, 0);
-        const uint32_t later = starts & ~(0xffffffffu >> (31 - lane));
-        const int last = later ? __ffs(later) - 2 : 31;
-        float m = ml.x;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float v = __shfl_up_sync(0xffffffffu, m, o);
-            if (__shfl_up_sync(0xffffffffu, run, o) == run && (int)lane >= o) m = fmaxf(m, v);
-        }
-        m = __shfl_sync(0xffffffffu, m, last);
-        const float c = ml.x == m ? 1.0f : ex2(ml.x - m);
-        float l = sg.ends ? ml.y * c : 0.0f;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const float v = __shfl_up_sync(0xffffffffu, l, o);
-            if (__shfl_up_sync(0xffffffffu, run, o) == run && (int)lane >= o) l += v;
-        }
-        l = __shfl_sync(0xffffffffu, l, last);
-        if (sg.ends) { sh.aside[lane * R + row] = c; sh.ml[lane >> 1][lane & 1][row] = make_float2(m, l); }
-    }
-    __syncthreads();
     // a row's place in the fragments: element f = (i * NB + b) * 32 + lane
     auto row_of = [](uint32_t f) { const uint32_t i = f / (NB * 32), ln = f & 31; return SPLIT ? ln & 3 : (i >> 1) * 8 + 2 * (ln & 3) + (i & 1); };
     auto store_out = [&](const Segment& of, uint32_t f, float4 o, float l) {
@@ -698,27 +752,26 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         const uint32_t k = i / NE, f = i % NE, row = row_of(f);
         uint32_t members = __ballot_sync(0xffffffffu, sg.ends && run == (int)k);
         const uint32_t ends = __reduce_or_sync(0xffffffffu, run == (int)k ? (uint32_t)sg.ends : 0u), e0 = __ffs(members) - 1;
-        float4 o = make_float4(0, 0, 0, 0);
-        while (members) {        // four at a time
-            float c[4];
+        Joined<4> o;
+        while (members) {
+            float2 ml[4];
             float4 x[4];
+            int n = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const uint32_t e = members ? __ffs(members) - 1 : e0;
-                c[j] = members ? sh.aside[e * R + row] : 0.0f;
+                n += members != 0;
+                ml[j] = sh.ml[e >> 1][e & 1][row];
                 x[j] = (&sh.sum[e >> 1][e & 1][0][0])[f];
-                if (!members) x[j] = make_float4(0, 0, 0, 0);
                 members &= members - 1;
             }
-#pragma unroll
-            for (int j = 0; j < 4; j++) { o.x = fmaf(x[j].x, c[j], o.x); o.y = fmaf(x[j].y, c[j], o.y); o.z = fmaf(x[j].z, c[j], o.z); o.w = fmaf(x[j].w, c[j], o.w); }
+            o.add(ml, x, n);
         }
-        const float2 ml = sh.ml[e0 >> 1][e0 & 1][row];
-        if ((ends & 3) == 3) store_out(sh.seg[e0], f, o, ml.y);
+        if ((ends & 3) == 3) store_out(sh.seg[e0], f, o.sum, o.l);
         else {
             float* to = part_at(cta, ends & 1);
-            __stcg(reinterpret_cast<float4*>(to) + f, o);
-            if ((f / 32) % NB == 0 && (f & 31) < 4) __stcg(reinterpret_cast<float2*>(to + R * DIM) + row, ml);
+            __stcg(reinterpret_cast<float4*>(to) + f, o.sum);
+            if ((f / 32) % NB == 0 && (f & 31) < 4) __stcg(reinterpret_cast<float2*>(to + R * DIM) + row, make_float2(o.m, o.l));
         }
     }
     // Jobs that other CTAs have parts of: [0] one that began before this CTA, [1] one that begins in it. A lane of each warp finds the
@@ -755,46 +808,24 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     for (int k = 0; k < 2; k++) {
         if (!sh.last[k]) continue;
         __threadfence();
-        // weights of the CTAs' parts, where the ring was
-        float2* const ml = reinterpret_cast<float2*>(sh.ring[0][0]);
-        static_assert(sizeof(sh.ring) >= sizeof(float2) * R * MAX_CTAS, "a weight a row of every CTA");
-        for (uint32_t i = tid; i < count[k] * R; i += W * 32)
-            ml[i] = __ldcg(reinterpret_cast<const float2*>(part_at(first_cta[k] + i / R, i < R) + R * DIM) + i % R);
-        __syncthreads();
-        for (uint32_t row = warp; row < R; row += W) {
-            float m = -INFINITY, l = 0;
-            for (uint32_t c = lane; c < count[k]; c += 32) m = fmaxf(m, ml[c * R + row].x);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (uint32_t c = lane; c < count[k]; c += 32) {
-                const float2 x = ml[c * R + row];
-                const float w = x.x == m ? 1.0f : ex2(x.x - m);
-                ml[c * R + row].x = w;
-                l = fmaf(x.y, w, l);
-            }
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            if (lane == 0) sh.aside[2 * W * R + row] = l;
-        }
-        __syncthreads();
-        for (uint32_t f = tid; f < NF * 32; f += W * 32) {
+        for (uint32_t f = tid; f < NE; f += W * 32) {
+            constexpr int AT_ONCE = 10;
             const uint32_t row = row_of(f);
-            float4 o = make_float4(0, 0, 0, 0);
-            for (uint32_t c0 = 0; c0 < count[k]; c0 += 8) {
-                float4 x[8];
+            Joined<AT_ONCE> o;
+            for (uint32_t i = 0; i < count[k]; i += AT_ONCE) {
+                float2 ml[AT_ONCE];
+                float4 x[AT_ONCE];
 #pragma unroll
-                for (int c = 0; c < 8; c++) x[c] = __ldcg(reinterpret_cast<const float4*>(part_at(first_cta[k] + min(c0 + c, count[k] - 1), c0 + c == 0)) + f);
-#pragma unroll
-                for (int c = 0; c < 8; c++) {
-                    if (c0 + c >= count[k]) break;
-                    const float w = ml[(c0 + c) * R + row].x;
-                    o.x = fmaf(x[c].x, w, o.x); o.y = fmaf(x[c].y, w, o.y); o.z = fmaf(x[c].z, w, o.z); o.w = fmaf(x[c].w, w, o.w);
+                for (int j = 0; j < AT_ONCE; j++) {
+                    const uint32_t c = min(i + j, count[k] - 1);
+                    const float* from = part_at(first_cta[k] + c, c == 0);
+                    ml[j] = __ldcg(reinterpret_cast<const float2*>(from + R * DIM) + row);
+                    x[j] = __ldcg(reinterpret_cast<const float4*>(from) + f);
                 }
+                o.add(ml, x, (int)min(count[k] - i, (uint32_t)AT_ONCE));
             }
-            const float l = sh.aside[2 * W * R + row];
-            store_out(sh.seg[open[k]], f, o, l);
+            store_out(sh.seg[open[k]], f, o.sum, o.l);
         }
-        __syncthreads();
     }
 }
 
@@ -814,7 +845,7 @@ cudaError_t launch(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl)
         if (dev < 64) done[dev] = true;
     }
     cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[1];
-    lc.gridDim = dim3(num_sms < (int)MAX_CTAS ? num_sms : (int)MAX_CTAS); lc.blockDim = dim3(C::WARPS * 32); lc.dynamicSmemBytes = sizeof(typename C::Smem); lc.stream = st;
+    lc.gridDim = dim3(num_sms); lc.blockDim = dim3(C::WARPS * 32); lc.dynamicSmemBytes = sizeof(typename C::Smem); lc.stream = st;
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at; lc.numAttrs = pdl ? 1 : 0;

@@ -181,6 +181,15 @@ def test_several_tokens(engine, tokens, heads, kv_heads, dim):
     s.check()
 
 
+@pytest.mark.parametrize("dim,rot", [(64, 16), (64, 48), (128, 96), (128, 112), (256, 16), (256, 144), (256, 192), (256, 240), (256, 256)])
+@pytest.mark.parametrize("neox", [False, True])
+def test_parts_of_a_head_rotated(engine, dim, rot, neox):
+    """Pairs whose halves lie with other lanes, and dims that are not rotated."""
+    s = Step(engine, 6, 2, dim, 32, [37, 0, 5], [1, 1, 3], rot, neox, seed=rot)
+    s.fill()
+    s.check()
+
+
 @pytest.mark.parametrize("page", [16, 48, 64, 4096])
 @pytest.mark.parametrize("past", [2047, 5000])
 def test_long_contexts(engine, past, page):
