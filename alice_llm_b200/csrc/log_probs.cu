@@ -1,8 +1,15 @@
 // Log probabilities, entropy, rank and the most probable tokens of rows of logits.
 //
 // With m the largest logit and s the sum of exp(x - m) over all others but that one:
-//   log p(x) = (x - m) - log1p(s),   H = log1p(s) - sum (x - m) exp(x - m) / (1 + s)
-// so that what is small beside the largest term is not lost where one token has nearly all the weight.
+//   log p(x) = (x - m) - log1p(s),   H = log1p(s) - w / (1 + s),   w = sum (x - m) exp(x - m)
+// so that what is small beside the largest term is not lost where one token has nearly all the weight. Every partial sum, of a thread,
+// a warp or a CTA, is a triple (m, s, w) in which the 1 of its own largest term is left out.
+//
+// One pass: a thread takes 16 logits at a time, splits them into their largest and the 15 others by minima and maxima and adds them to its
+// triple. The alternatives come from the same registers: the k-th largest of the threads' maxima is a bound that at least k logits reach and
+// few more, those go to a list in shared memory and are put in order by counting; later logits only enter the list when they exceed its
+// last. A row is cut among the CTAs of a cluster, as many as keep the chip busy, and joined through distributed shared memory: no scratch,
+// nothing that calls or graphs could share, and the same order of sums at every call.
 #include <cmath>
 
 #include "abi_internal.cuh"
@@ -13,96 +20,289 @@ namespace alice {
 
 namespace {
 
-// Logits in order as whole numbers, the lower index first among equals.
+// Logits in order as whole numbers, the lower index first among equals. 0: no logit.
 __device__ __forceinline__ unsigned long long logit_key(float x, uint32_t i) {
     const uint32_t u = __float_as_uint(x + 0.0f);      // -0 as 0
     return (unsigned long long)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - i);
 }
+__device__ __forceinline__ float key_logit(unsigned long long k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
 
-constexpr int LP_THREADS = 256;
+constexpr int THREADS = 256, WARPS = THREADS / 32, FOURS = 4, EACH = 4 * FOURS;      // a thread's logits at a time
+constexpr uint32_t MAX_CLUSTER = 16;
+// what can enter the list at a time: all logits of the threads whose largest is among the top, and the list itself
+constexpr int CAP = LOGP_MAX_TOP * EACH + LOGP_MAX_TOP > (int)(MAX_CLUSTER * LOGP_MAX_TOP) ? LOGP_MAX_TOP * EACH + LOGP_MAX_TOP : (int)(MAX_CLUSTER * LOGP_MAX_TOP);
+constexpr float LEAST = -3.402823466e38f;
 
-template <class T, class F>
-__device__ __forceinline__ T over_cta(T v, T* red, F f) {
-    __syncthreads();
-    red[threadIdx.x] = v;
-    __syncthreads();
-    for (int o = LP_THREADS / 2; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) red[threadIdx.x] = f(red[threadIdx.x], red[threadIdx.x + o]);
-        __syncthreads();
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float exp_of(float t) {     // t <= 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t * 1.44269504088896341f));
+    return y;
+}
+// Differences end at -200, whose exponential is 0: the term of a ruled-out token is 0 and not 0 times infinity.
+__device__ __forceinline__ float diff(float x, float m) { return max_nan(x - m, -200.0f); }
+
+struct Triple {
+    float m, s, w;
+    __device__ __forceinline__ void join(const Triple& o) {
+        const float top = max_nan(m, o.m), ref = max_nan(top, LEAST);
+        const bool first = m >= o.m;
+        const float t = diff(first ? o.m : m, ref), f = exp_of(t), ls = (first ? o.s : s) + 1.0f, lw = first ? o.w : w;
+        s = fmaf(f, ls, first ? s : o.s);
+        w = fmaf(f, fmaf(t, ls, lw), first ? w : o.w);
+        m = top;
     }
-    return red[0];
+};
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t there(const void* p, uint32_t rank) {      // the same place in another CTA
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float far_f32(uint32_t a) { float v; asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory"); return v; }
+__device__ __forceinline__ uint32_t far_u32(uint32_t a) { uint32_t v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory"); return v; }
+__device__ __forceinline__ unsigned long long far_u64(uint32_t a) { unsigned long long v; asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory"); return v; }
+
+struct Smem {
+    Triple part[WARPS];
+    uint32_t above[WARPS];
+    Triple all;
+    uint32_t all_above, listed;                      // logits above the target; entries of `top`
+    uint32_t entering;                               // of `cand`
+    unsigned long long bound;
+    unsigned long long most[THREADS];                // the threads' largest
+    unsigned long long top[LOGP_MAX_TOP];            // the list, the largest first
+    unsigned long long cand[CAP];
+};
+
+// cand[0 .. n) in order: the first `want` of them to top. All threads; n and want are the CTA's.
+__device__ __forceinline__ uint32_t put_in_order(Smem& sh, uint32_t n, uint32_t want) {
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        const unsigned long long k = sh.cand[i];
+        uint32_t before = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; j++) before += sh.cand[j] > k;
+        if (before < want) sh.top[before] = k;
+    }
+    return min(n, want);
 }
 
 }  // namespace
 
-// A CTA a row.
-__global__ void __launch_bounds__(LP_THREADS) log_probs_kernel(const __grid_constant__ LogProbArgs a) {
-    __shared__ unsigned long long keys[LP_THREADS];
-    __shared__ float sums[LP_THREADS];
-    __shared__ uint32_t counts[LP_THREADS];
+template <bool TOP>
+__global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_constant__ LogProbArgs a) {
+    __shared__ Smem sh;
     pdl_launch_dependents();
     pdl_wait();
-    const size_t r = blockIdx.x;
-    const float* x = a.x + r * a.ld;
-    auto most = [](unsigned long long p, unsigned long long q) { return p > q ? p : q; };
-    auto add = [](float p, float q) { return p + q; };
-    auto addu = [](uint32_t p, uint32_t q) { return p + q; };
-    unsigned long long best = 0;
-    uint32_t odd = 0;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += LP_THREADS) {
-        const float v = x[i];
-        odd |= !(v < INFINITY);
-        best = most(best, logit_key(v, i));
-    }
-    best = over_cta(best, keys, most);
-    odd = over_cta(odd, counts, addu);
-    const uint32_t at = 0xffffffffu - (uint32_t)best;
-    const float m = x[at];
-    const bool none = odd || m == -INFINITY;
-    const uint32_t t = a.target ? a.target[r] : 0u;
-    const bool valid = a.target && t < a.vocab && !none;
-    const float xt = valid ? x[t] : 0.f;
-    float s = 0, w = 0;
-    uint32_t above = 0;
-    for (uint32_t i = threadIdx.x; i < a.vocab; i += LP_THREADS) {
-        const float v = x[i], z = fmaxf(v - m, -200.f), e = i == at ? 0.f : expf(z);
-        s += e;
-        w += e * z;
-        above += v > xt;
-    }
-    s = over_cta(s, sums, add);
-    w = over_cta(w, sums, add);
-    above = over_cta(above, counts, addu);
-    const float l = log1pf(s), nan = __uint_as_float(0x7fc00000u);
-    if (threadIdx.x == 0) {
-        if (a.lp) a.lp[r] = valid ? (xt - m) - l : nan;
-        if (a.rank) a.rank[r] = valid ? above + 1 : 0u;
-        if (a.entropy) a.entropy[r] = none ? nan : l - w / (1.f + s);
-    }
-    unsigned long long below = ~0ull;
-    for (uint32_t k = 0; k < a.top; k++) {
-        unsigned long long b = 0;
-        for (uint32_t i = threadIdx.x; i < a.vocab; i += LP_THREADS) {
-            const unsigned long long key = logit_key(x[i], i);
-            if (key < below) b = most(b, key);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, parts = cluster_size(), part = cluster_rank();
+    const size_t r = blockIdx.x / parts;
+    // The row in pieces of four that lie on 16-byte boundaries; its first and last may hold less of it.
+    const float* const row = a.x + r * a.ld;
+    const uint32_t skip = (uint32_t)((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
+    const float4* const four = reinterpret_cast<const float4*>(row - skip);
+    const uint32_t fours = (uint32_t)(((uint64_t)a.vocab + skip + 3) / 4), per = (fours + parts - 1) / parts, begin = min(part * per, fours), end = min(begin + per, fours);
+    auto load = [&](float (&x)[EACH], uint32_t at) {
+#pragma unroll
+        for (int i = 0; i < FOURS; i++) {
+            const uint32_t p = at + i * THREADS + tid;
+            float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (p < end) {
+                const long long e = (long long)p * 4 - skip;
+                if (e >= 0 && e + 4 <= (long long)a.vocab) v = __ldcs(four + p);
+                else {
+                    float* const f = &v.x;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) if (e + j >= 0 && e + j < (long long)a.vocab) f[j] = __ldcs(row + (e + j));
+                }
+            }
+            x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
         }
-        below = over_cta(b, keys, most);
-        if (threadIdx.x == 0) {
-            const uint32_t id = 0xffffffffu - (uint32_t)below;
-            a.top_ids[r * a.top + k] = none ? 0xffffffffu : id;
-            a.top_lp[r * a.top + k] = none ? nan : (x[id] - m) - l;
+    };
+    float x[EACH], next[EACH];
+    load(x, begin);
+    const uint32_t t = a.target ? __ldg(a.target + r) : 0u;
+    const bool aimed = a.target && t < a.vocab;
+    const float xt = aimed ? __ldg(row + t) : INFINITY;
+    if (tid == 0) { sh.listed = 0; sh.entering = 0; }
+    if (TOP) __syncthreads();
+
+    Triple me{-INFINITY, 0, 0};
+    uint32_t above = 0, listed = 0;
+    for (uint32_t at = begin; at < end; at += FOURS * THREADS) {
+        if (at + FOURS * THREADS < end) load(next, at + FOURS * THREADS);
+        // ---- the largest, and the others ----
+        float big = x[0], other[EACH];
+#pragma unroll
+        for (int i = 1; i < EACH; i++) {
+            other[i] = fminf(big, x[i]);
+            big = max_nan(big, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++) above += x[i] > xt;
+        {
+            const float top = max_nan(me.m, big), ref = max_nan(top, LEAST);
+            const bool moved = me.m < top;
+            const float d = diff(moved ? me.m : big, ref), f = exp_of(d);      // of the two largest, the lesser
+            if (at == begin) me.s = me.w = 0;                                    // there is only one
+            else if (moved) { me.w = f * fmaf(d, me.s + 1.0f, me.w); me.s = f * (me.s + 1.0f); }
+            else { me.s += f; me.w = fmaf(f, d, me.w); }
+            float s = 0, w = 0;
+#pragma unroll
+            for (int i = 1; i < EACH; i++) {
+                const float z = diff(other[i], ref), e = exp_of(z);
+                s += e;
+                w = fmaf(e, z, w);
+            }
+            me.s += s; me.w += w; me.m = top;
+        }
+        // ---- the list ----
+        if (TOP) {
+            const unsigned long long bound = listed == a.top ? sh.top[a.top - 1] : 0ull;
+            // the thread's largest with its place; what is past the row is no logit
+            unsigned long long mine = 0;
+            auto place = [&](int i) { return (long long)(at + (i >> 2) * THREADS + tid) * 4 - skip + (i & 3); };
+            auto key = [&](int i) {
+                const long long e = place(i);
+                return at + (i >> 2) * THREADS + tid < end && e >= 0 && e < (long long)a.vocab ? logit_key(x[i], (uint32_t)e) : 0ull;
+            };
+            const bool reach = listed < a.top || big >= key_logit(bound);
+            if (reach) {
+#pragma unroll
+                for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); mine = k > mine ? k : mine; }
+            }
+            const uint32_t over = __syncthreads_count(mine > bound);
+            if (over) {
+                unsigned long long from = bound;                 // what is larger enters
+                if (over > a.top) {
+                    // the top-th largest of the threads' largest: by its bits, from the highest
+                    sh.most[tid] = mine;
+                    __syncthreads();
+                    if (warp == 0) {
+                        unsigned long long k[THREADS / 32], found = 0;
+#pragma unroll
+                        for (int i = 0; i < THREADS / 32; i++) k[i] = sh.most[lane + 32 * i];
+                        for (int bit = 63; bit >= 0; bit--) {
+                            const unsigned long long trial = found | 1ull << bit;
+                            uint32_t n = 0;
+#pragma unroll
+                            for (int i = 0; i < THREADS / 32; i++) n += k[i] >= trial;
+                            n = __reduce_add_sync(0xffffffffu, n);
+                            if (n >= a.top) found = trial;
+                            if (n == a.top) break;
+                        }
+                        if (lane == 0) sh.bound = found - 1;
+                    }
+                    __syncthreads();
+                    from = sh.bound > bound ? sh.bound : bound;
+                }
+                if (mine > from) {
+#pragma unroll
+                    for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); if (k > from) sh.cand[atomicAdd(&sh.entering, 1u)] = k; }
+                }
+                if (tid < listed) sh.cand[atomicAdd(&sh.entering, 1u)] = sh.top[tid];
+                __syncthreads();
+                const uint32_t n = sh.entering;
+                listed = put_in_order(sh, n, a.top);
+                __syncthreads();
+                if (tid == 0) sh.entering = 0;
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; i++) x[i] = next[i];
+    }
+
+    // ---- threads, warps, CTAs ----
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Triple you;
+        you.m = __shfl_down_sync(0xffffffffu, me.m, o); you.s = __shfl_down_sync(0xffffffffu, me.s, o); you.w = __shfl_down_sync(0xffffffffu, me.w, o);
+        me.join(you);
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    if (lane == 0) { sh.part[warp] = me; sh.above[warp] = above; }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+        for (int i = 1; i < WARPS; i++) { me.join(sh.part[i]); above += sh.above[i]; }
+        sh.all = me; sh.all_above = above; sh.listed = listed;
+    }
+    cluster_sync();
+    if (part == 0) {
+        // each thread of the first CTA joins the triples of all, in order; its threads bring the lists together
+        me = sh.all; above = sh.all_above;
+        for (uint32_t c = 1; c < parts; c++) {
+            const uint32_t p = there(&sh.all, c);
+            me.join(Triple{far_f32(p), far_f32(p + 4), far_f32(p + 8)});
+            above += far_u32(there(&sh.all_above, c));
+        }
+        const bool none = !(me.m > -INFINITY && me.m < INFINITY);
+        const float l = log1pf(me.s), nan = __uint_as_float(0x7fc00000u);
+        if (tid == 0) {
+            if (a.lp) a.lp[r] = aimed && !none ? (xt - me.m) - l : nan;
+            if (a.rank) a.rank[r] = aimed && !none ? above + 1 : 0u;
+            if (a.entropy) a.entropy[r] = none ? nan : l - me.w / (1.0f + me.s);
+        }
+        if (TOP) {
+            if (parts > 1) {
+                for (uint32_t i = tid; i < parts * a.top; i += THREADS) {
+                    const uint32_t c = i / a.top, j = i % a.top;
+                    if (j < far_u32(there(&sh.listed, c))) sh.cand[atomicAdd(&sh.entering, 1u)] = far_u64(there(&sh.top[j], c));
+                }
+                __syncthreads();
+                put_in_order(sh, sh.entering, a.top);
+                __syncthreads();
+            }
+            if (tid < a.top) {
+                const unsigned long long k = sh.top[tid];
+                a.top_ids[r * a.top + tid] = none ? 0xffffffffu : 0xffffffffu - (uint32_t)k;
+                a.top_lp[r * a.top + tid] = none ? nan : (key_logit(k) - me.m) - l;
+            }
         }
     }
+    if (parts > 1) cluster_sync();      // what the first CTA reads stays until it has
 }
 
-cudaError_t launch_log_probs(const LogProbArgs& a, int, cudaStream_t st, bool pdl) {
+namespace {
+template <bool TOP>
+cudaError_t launch(const LogProbArgs& a, uint32_t parts, cudaStream_t st, bool pdl) {
+    static bool done[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !done[dev]) {
+        err = cudaFuncSetAttribute(log_probs_kernel<TOP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);      // 16 CTAs
+        if (err != cudaSuccess) return err;
+        if (dev < 64) done[dev] = true;
+    }
+    cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[2];
+    lc.gridDim = dim3(a.rows * parts); lc.blockDim = dim3(THREADS); lc.stream = st;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = parts; at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at; lc.numAttrs = pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&lc, log_probs_kernel<TOP>, a);
+}
+}  // namespace
+
+cudaError_t launch_log_probs(const LogProbArgs& a, int num_sms, cudaStream_t st, bool pdl) {
     if (!a.rows) return cudaSuccess;
-    cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[1];
-    lc.gridDim = dim3(a.rows); lc.blockDim = dim3(LP_THREADS); lc.stream = st;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.attrs = at; lc.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&lc, log_probs_kernel, a);
+    // Twice as many CTAs as an SM holds at a time, as long as each has logits for all its threads.
+    uint32_t parts = 1;
+    while (parts < MAX_CLUSTER && (uint64_t)a.rows * parts < 8ull * num_sms && (uint64_t)parts * THREADS * EACH < a.vocab) parts *= 2;
+    return a.top ? launch<true>(a, parts, st, pdl) : launch<false>(a, parts, st, pdl);
 }
 
 }  // namespace alice
@@ -113,6 +313,7 @@ extern "C" int32_t alice_log_probs(alice_engine* e, const alice_buf* logits, uin
                                    alice_buf* entropy, alice_buf* rank, uint32_t top, alice_buf* top_ids, alice_buf* top_log_probs) {
     const char* who = "alice_log_probs";
     if (!e || !logits) return alice_fail(ALICE_E_INVALID, "%s: null argument", who);
+    if (rows > 0x7fffffffu) return alice_fail(ALICE_E_SHAPE, "%s: %u rows", who, rows);
     if (vocab == 0) return alice_fail(ALICE_E_SHAPE, "%s: a vocabulary of none", who);
     if (stride == 0) stride = vocab;
     if (stride < vocab || stride > ((size_t)1 << 40)) return alice_fail(ALICE_E_SHAPE, "%s: rows of %u logits %zu floats apart", who, vocab, stride);
