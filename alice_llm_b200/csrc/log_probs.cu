@@ -6,9 +6,9 @@
 // a warp or a CTA, is a triple (m, s, w) in which the 1 of its own largest term is left out.
 //
 // One pass: a thread takes 16 logits at a time, splits them into their largest and the 15 others by minima and maxima and adds them to its
-// triple. The alternatives come from the same registers: the k-th largest of the threads' maxima is a bound that at least k logits reach and
-// few more, those go to a list in shared memory and are put in order by counting; later logits only enter the list when they exceed its
-// last. A row is cut among the CTAs of a cluster, as many as keep the chip busy, and joined through distributed shared memory: no scratch,
+// triple. The alternatives come from the same registers: a bound that at least k of the threads' maxima reach and few more is found by
+// halving; logits above it go to a list in shared memory, later ones too, and the list is put in order by counting, at the end or when it
+// is full (the bound then rises to its k-th). A row is cut among the CTAs of a cluster, as many as keep the chip busy, and joined through distributed shared memory: no scratch,
 // nothing that calls or graphs could share, and the same order of sums at every call.
 #include <cmath>
 
@@ -32,8 +32,9 @@ __device__ __forceinline__ float key_logit(unsigned long long k) {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, FOURS = 4, EACH = 4 * FOURS;      // a thread's logits at a time
 constexpr uint32_t MAX_CLUSTER = 16;
-// what can enter the list at a time: all logits of the threads whose largest is among the top, and the list itself
-constexpr int CAP = LOGP_MAX_TOP * EACH + LOGP_MAX_TOP > (int)(MAX_CLUSTER * LOGP_MAX_TOP) ? LOGP_MAX_TOP * EACH + LOGP_MAX_TOP : (int)(MAX_CLUSTER * LOGP_MAX_TOP);
+// Entries of the list. A bound may be reached by as many threads as leave room for all their logits beside the alternatives so far.
+constexpr uint32_t CAP = 1024, REACH = (CAP - LOGP_MAX_TOP) / EACH;
+static_assert(MAX_CLUSTER * LOGP_MAX_TOP <= CAP && REACH >= LOGP_MAX_TOP, "");
 constexpr float LEAST = -3.402823466e38f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -60,6 +61,17 @@ struct Triple {
         m = top;
     }
 };
+// Of the first N lanes: each of them has the whole.
+template <int N>
+__device__ __forceinline__ void join_lanes(Triple& me, uint32_t& count) {
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+        Triple you;
+        you.m = __shfl_xor_sync(0xffffffffu, me.m, o); you.s = __shfl_xor_sync(0xffffffffu, me.s, o); you.w = __shfl_xor_sync(0xffffffffu, me.w, o);
+        count += __shfl_xor_sync(0xffffffffu, count, o);
+        me.join(you);
+    }
+}
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync() {
@@ -86,14 +98,18 @@ struct Smem {
     unsigned long long cand[CAP];
 };
 
-// cand[0 .. n) in order: the first `want` of them to top. All threads; n and want are the CTA's.
+// cand[0 .. n) in order: the first `want` of them to top. All threads, four to an entry; n and want are the CTA's.
 __device__ __forceinline__ uint32_t put_in_order(Smem& sh, uint32_t n, uint32_t want) {
-    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
-        const unsigned long long k = sh.cand[i];
+    const uint32_t q = threadIdx.x & 3;
+    for (uint32_t i0 = 0; i0 < n; i0 += THREADS / 4) {
+        const uint32_t i = i0 + threadIdx.x / 4;
+        const unsigned long long k = i < n ? sh.cand[i] : 0ull;
         uint32_t before = 0;
 #pragma unroll 4
-        for (uint32_t j = 0; j < n; j++) before += sh.cand[j] > k;
-        if (before < want) sh.top[before] = k;
+        for (uint32_t j = q; j < n; j += 4) before += sh.cand[j] > k;
+        before += __shfl_xor_sync(0xffffffffu, before, 1);
+        before += __shfl_xor_sync(0xffffffffu, before, 2);
+        if (i < n && q == 0 && before < want) sh.top[before] = k;
     }
     return min(n, want);
 }
@@ -138,7 +154,8 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     if (TOP) __syncthreads();
 
     Triple me{-INFINITY, 0, 0};
-    uint32_t above = 0, listed = 0;
+    uint32_t above = 0;
+    unsigned long long from = 0;          // what is larger enters the list
     for (uint32_t at = begin; at < end; at += FOURS * THREADS) {
         if (at + FOURS * THREADS < end) load(next, at + FOURS * THREADS);
         // ---- the largest, and the others ----
@@ -168,55 +185,72 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
         }
         // ---- the list ----
         if (TOP) {
-            const unsigned long long bound = listed == a.top ? sh.top[a.top - 1] : 0ull;
-            // the thread's largest with its place; what is past the row is no logit
-            unsigned long long mine = 0;
-            auto place = [&](int i) { return (long long)(at + (i >> 2) * THREADS + tid) * 4 - skip + (i & 3); };
-            auto key = [&](int i) {
-                const long long e = place(i);
+            auto key = [&](int i) {          // what is past the row is no logit
+                const long long e = (long long)(at + (i >> 2) * THREADS + tid) * 4 - skip + (i & 3);
                 return at + (i >> 2) * THREADS + tid < end && e >= 0 && e < (long long)a.vocab ? logit_key(x[i], (uint32_t)e) : 0ull;
             };
-            const bool reach = listed < a.top || big >= key_logit(bound);
-            if (reach) {
-#pragma unroll
-                for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); mine = k > mine ? k : mine; }
-            }
-            const uint32_t over = __syncthreads_count(mine > bound);
+            const bool reach = from == 0 || big >= key_logit(from);
+            const uint32_t over = __syncthreads_count(reach);
             if (over) {
-                unsigned long long from = bound;                 // what is larger enters
-                if (over > a.top) {
-                    // the top-th largest of the threads' largest: by its bits, from the highest
-                    sh.most[tid] = mine;
-                    __syncthreads();
-                    if (warp == 0) {
-                        unsigned long long k[THREADS / 32], found = 0;
-#pragma unroll
-                        for (int i = 0; i < THREADS / 32; i++) k[i] = sh.most[lane + 32 * i];
-                        for (int bit = 63; bit >= 0; bit--) {
-                            const unsigned long long trial = found | 1ull << bit;
-                            uint32_t n = 0;
-#pragma unroll
-                            for (int i = 0; i < THREADS / 32; i++) n += k[i] >= trial;
-                            n = __reduce_add_sync(0xffffffffu, n);
-                            if (n >= a.top) found = trial;
-                            if (n == a.top) break;
-                        }
-                        if (lane == 0) sh.bound = found - 1;
+                uint32_t n = sh.entering;
+                if (n + over * EACH > CAP) {
+                    if (n > a.top) {             // the list without those that are out of it
+                        put_in_order(sh, n, a.top);
+                        __syncthreads();
+                        if (tid < a.top) sh.cand[tid] = sh.top[tid];
+                        if (tid == 0) sh.entering = a.top;
+                        n = a.top;
+                        from = sh.top[a.top - 1];
                     }
-                    __syncthreads();
-                    from = sh.bound > bound ? sh.bound : bound;
+                    if (over > REACH) {
+                        sh.most[tid] = logit_key(big, 0);
+                        __syncthreads();
+                        if (warp == 0) {         // by the bits in which they differ, from the highest
+                            uint32_t k[THREADS / 32], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+                            for (int i = 0; i < THREADS / 32; i++) { k[i] = (uint32_t)(sh.most[lane + 32 * i] >> 32); lo = min(lo, k[i]); hi = max(hi, k[i]); }
+                            lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
+                            const int bits = 32 - __clz(lo ^ hi);
+                            uint32_t found = bits == 32 ? 0u : hi >> bits << bits, at_least = THREADS;
+                            for (int bit = bits - 1; bit >= 0 && at_least > REACH; bit--) {
+                                const uint32_t trial = found | 1u << bit;
+                                uint32_t c = 0;
+#pragma unroll
+                                for (int i = 0; i < THREADS / 32; i++) c += k[i] >= trial;
+                                c = __reduce_add_sync(0xffffffffu, c);
+                                if (c >= a.top) { found = trial; at_least = c; }
+                            }
+                            if (lane == 0) sh.bound = at_least <= REACH ? (unsigned long long)found << 32 : ~0ull;
+                        }
+                        __syncthreads();
+                        unsigned long long bound = sh.bound;
+                        if (bound == ~0ull) {    // too many that are equal: by their places too
+                            unsigned long long mine = 0;
+#pragma unroll
+                            for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); mine = k > mine ? k : mine; }
+                            sh.most[tid] = mine;
+                            __syncthreads();
+                            if (warp == 0) {
+                                unsigned long long found = 0;
+                                for (int bit = 63; bit >= 0; bit--) {
+                                    const unsigned long long trial = found | 1ull << bit;
+                                    uint32_t c = 0;
+                                    for (int i = 0; i < THREADS / 32; i++) c += sh.most[lane + 32 * i] >= trial;
+                                    if (__reduce_add_sync(0xffffffffu, c) >= a.top) found = trial;
+                                }
+                                if (lane == 0) sh.bound = found;
+                            }
+                            __syncthreads();
+                            bound = sh.bound;    // the top-th largest, or 0 where there are not so many
+                        }
+                        if (bound > from) from = bound - 1;
+                    }
                 }
-                if (mine > from) {
+                __syncthreads();
+                if (from == 0 || big >= key_logit(from)) {
 #pragma unroll
                     for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); if (k > from) sh.cand[atomicAdd(&sh.entering, 1u)] = k; }
                 }
-                if (tid < listed) sh.cand[atomicAdd(&sh.entering, 1u)] = sh.top[tid];
-                __syncthreads();
-                const uint32_t n = sh.entering;
-                listed = put_in_order(sh, n, a.top);
-                __syncthreads();
-                if (tid == 0) sh.entering = 0;
-                __syncthreads();
             }
         }
 #pragma unroll
@@ -224,29 +258,36 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     }
 
     // ---- threads, warps, CTAs ----
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Triple you;
-        you.m = __shfl_down_sync(0xffffffffu, me.m, o); you.s = __shfl_down_sync(0xffffffffu, me.s, o); you.w = __shfl_down_sync(0xffffffffu, me.w, o);
-        me.join(you);
-    }
+    { uint32_t zero = 0; join_lanes<32>(me, zero); }
     above = __reduce_add_sync(0xffffffffu, above);
     if (lane == 0) { sh.part[warp] = me; sh.above[warp] = above; }
     __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-        for (int i = 1; i < WARPS; i++) { me.join(sh.part[i]); above += sh.above[i]; }
-        sh.all = me; sh.all_above = above; sh.listed = listed;
+    uint32_t listed = 0;
+    if (TOP) listed = put_in_order(sh, sh.entering, a.top);
+    if (warp == 0) {
+        me = lane < WARPS ? sh.part[lane] : Triple{-INFINITY, 0, 0};
+        above = lane < WARPS ? sh.above[lane] : 0u;
+        join_lanes<WARPS>(me, above);
+        if (lane == 0) { sh.all = me; sh.all_above = above; sh.listed = listed; }
     }
     cluster_sync();
     if (part == 0) {
-        // each thread of the first CTA joins the triples of all, in order; its threads bring the lists together
-        me = sh.all; above = sh.all_above;
-        for (uint32_t c = 1; c < parts; c++) {
-            const uint32_t p = there(&sh.all, c);
-            me.join(Triple{far_f32(p), far_f32(p + 4), far_f32(p + 8)});
-            above += far_u32(there(&sh.all_above, c));
+        if (TOP && parts > 1) {
+            if (tid == 0) sh.entering = 0;
+            __syncthreads();
+            for (uint32_t i = tid; i < parts * a.top; i += THREADS) {
+                const uint32_t c = i / a.top, j = i % a.top;
+                const unsigned long long k = far_u64(there(&sh.top[j], c));
+                if (j < far_u32(there(&sh.listed, c))) sh.cand[atomicAdd(&sh.entering, 1u)] = k;
+            }
         }
+        // each warp joins the triples of all CTAs, a lane each
+        const uint32_t p = there(&sh.all, min(lane, parts - 1));
+        me = Triple{far_f32(p), far_f32(p + 4), far_f32(p + 8)};
+        above = far_u32(there(&sh.all_above, min(lane, parts - 1)));
+        if (lane >= parts) { me = Triple{-INFINITY, 0, 0}; above = 0; }
+        join_lanes<MAX_CLUSTER>(me, above);
+        me.m = __shfl_sync(0xffffffffu, me.m, 0); me.s = __shfl_sync(0xffffffffu, me.s, 0);       // one value for all
         const bool none = !(me.m > -INFINITY && me.m < INFINITY);
         const float l = log1pf(me.s), nan = __uint_as_float(0x7fc00000u);
         if (tid == 0) {
@@ -256,10 +297,6 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
         }
         if (TOP) {
             if (parts > 1) {
-                for (uint32_t i = tid; i < parts * a.top; i += THREADS) {
-                    const uint32_t c = i / a.top, j = i % a.top;
-                    if (j < far_u32(there(&sh.listed, c))) sh.cand[atomicAdd(&sh.entering, 1u)] = far_u64(there(&sh.top[j], c));
-                }
                 __syncthreads();
                 put_in_order(sh, sh.entering, a.top);
                 __syncthreads();
