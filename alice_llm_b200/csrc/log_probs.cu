@@ -6,10 +6,12 @@
 // a warp or a CTA, is a triple (m, s, w) in which the 1 of its own largest term is left out.
 //
 // One pass: a thread takes 16 logits at a time, splits them into their largest and the 15 others by minima and maxima and adds them to its
-// triple. The alternatives come from the same registers: a bound that at least k of the threads' maxima reach and few more is found by
-// halving; logits above it go to a list in shared memory, later ones too, and the list is put in order by counting, at the end or when it
-// is full (the bound then rises to its k-th). A row is cut among the CTAs of a cluster, as many as keep the chip busy, and joined through distributed shared memory: no scratch,
+// triple. The alternatives come from the same registers: a bound that at least k of the threads' first maxima reach and few more is found by
+// halving; logits above it go to a list in shared memory, later ones too, without a barrier, and now and then the list is put in order and
+// the bound rises to its k-th. Should it overflow all the same (logits that keep rising), the part is listed again, 16 logits a thread
+// and a barrier at a time. A row is cut among the CTAs of a cluster, as many as keep the chip busy, and joined through distributed shared memory: no scratch,
 // nothing that calls or graphs could share, and the same order of sums at every call.
+#include <algorithm>
 #include <cmath>
 
 #include "abi_internal.cuh"
@@ -156,6 +158,80 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     Triple me{-INFINITY, 0, 0};
     uint32_t above = 0;
     unsigned long long from = 0;          // what is larger enters the list
+    auto key = [&](int i, uint32_t at) {          // what is past the row is no logit
+        const long long e = (long long)(at + (i >> 2) * THREADS + tid) * 4 - skip + (i & 3);
+        return at + (i >> 2) * THREADS + tid < end && e >= 0 && e < (long long)a.vocab ? logit_key(x[i], (uint32_t)e) : 0ull;
+    };
+    // the list's first, in order, and nothing else of it
+    auto compact = [&](uint32_t n) {
+        put_in_order(sh, n, a.top);
+        __syncthreads();
+        if (tid < a.top) sh.cand[tid] = sh.top[tid];
+        if (tid == 0) sh.entering = a.top;
+        from = sh.top[a.top - 1];
+    };
+    // 16 logits a thread into the list, all threads together
+    auto enter = [&](uint32_t at, float big) {
+            const bool reach = from == 0 || big >= key_logit(from);
+            const uint32_t over = __syncthreads_count(reach);
+            if (over) {
+                uint32_t n = sh.entering;
+                if (n + over * EACH > CAP) {
+                    if (n > a.top) { compact(n); n = a.top; }
+                    if (over > REACH) {
+                        sh.most[tid] = logit_key(big, 0);
+                        __syncthreads();
+                        if (warp == 0) {         // by the bits in which they differ, from the highest
+                            uint32_t k[THREADS / 32], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+                            for (int i = 0; i < THREADS / 32; i++) { k[i] = (uint32_t)(sh.most[lane + 32 * i] >> 32); lo = min(lo, k[i]); hi = max(hi, k[i]); }
+                            lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
+                            const int bits = 32 - __clz(lo ^ hi);
+                            uint32_t found = bits == 32 ? 0u : hi >> bits << bits, at_least = THREADS;
+                            for (int bit = bits - 1; bit >= 0 && at_least > a.top + a.top / 4 + 1; bit--) {
+                                const uint32_t trial = found | 1u << bit;
+                                uint32_t c = 0;
+#pragma unroll
+                                for (int i = 0; i < THREADS / 32; i++) c += k[i] >= trial;
+                                c = __reduce_add_sync(0xffffffffu, c);
+                                if (c >= a.top) { found = trial; at_least = c; }
+                            }
+                            if (lane == 0) sh.bound = at_least <= REACH ? (unsigned long long)found << 32 : ~0ull;
+                        }
+                        __syncthreads();
+                        unsigned long long bound = sh.bound;
+                        if (bound == ~0ull) {    // too many that are equal: by their places too
+                            unsigned long long mine = 0;
+#pragma unroll
+                            for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i, at); mine = k > mine ? k : mine; }
+                            sh.most[tid] = mine;
+                            __syncthreads();
+                            if (warp == 0) {
+                                unsigned long long found = 0;
+                                for (int bit = 63; bit >= 0; bit--) {
+                                    const unsigned long long trial = found | 1ull << bit;
+                                    uint32_t c = 0;
+                                    for (int i = 0; i < THREADS / 32; i++) c += sh.most[lane + 32 * i] >= trial;
+                                    if (__reduce_add_sync(0xffffffffu, c) >= a.top) found = trial;
+                                }
+                                if (lane == 0) sh.bound = found;
+                            }
+                            __syncthreads();
+                            bound = sh.bound;    // the top-th largest, or 0 where there are not so many
+                        }
+                        if (bound > from) from = bound - 1;
+                    }
+                }
+                __syncthreads();
+                const float least = from == 0 ? -INFINITY : key_logit(from);
+                if (big >= least) {
+#pragma unroll
+                    for (int i = 0; i < EACH; i++)
+                        if (x[i] >= least) { const unsigned long long k = key(i, at); if (k > from) sh.cand[atomicAdd(&sh.entering, 1u)] = k; }
+                }
+            }
+    };
+    uint32_t round = 0;
     for (uint32_t at = begin; at < end; at += FOURS * THREADS) {
         if (at + FOURS * THREADS < end) load(next, at + FOURS * THREADS);
         // ---- the largest, and the others ----
@@ -185,71 +261,22 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
         }
         // ---- the list ----
         if (TOP) {
-            auto key = [&](int i) {          // what is past the row is no logit
-                const long long e = (long long)(at + (i >> 2) * THREADS + tid) * 4 - skip + (i & 3);
-                return at + (i >> 2) * THREADS + tid < end && e >= 0 && e < (long long)a.vocab ? logit_key(x[i], (uint32_t)e) : 0ull;
-            };
-            const bool reach = from == 0 || big >= key_logit(from);
-            const uint32_t over = __syncthreads_count(reach);
-            if (over) {
-                uint32_t n = sh.entering;
-                if (n + over * EACH > CAP) {
-                    if (n > a.top) {             // the list without those that are out of it
-                        put_in_order(sh, n, a.top);
-                        __syncthreads();
-                        if (tid < a.top) sh.cand[tid] = sh.top[tid];
-                        if (tid == 0) sh.entering = a.top;
-                        n = a.top;
-                        from = sh.top[a.top - 1];
-                    }
-                    if (over > REACH) {
-                        sh.most[tid] = logit_key(big, 0);
-                        __syncthreads();
-                        if (warp == 0) {         // by the bits in which they differ, from the highest
-                            uint32_t k[THREADS / 32], lo = 0xffffffffu, hi = 0;
-#pragma unroll
-                            for (int i = 0; i < THREADS / 32; i++) { k[i] = (uint32_t)(sh.most[lane + 32 * i] >> 32); lo = min(lo, k[i]); hi = max(hi, k[i]); }
-                            lo = __reduce_min_sync(0xffffffffu, lo); hi = __reduce_max_sync(0xffffffffu, hi);
-                            const int bits = 32 - __clz(lo ^ hi);
-                            uint32_t found = bits == 32 ? 0u : hi >> bits << bits, at_least = THREADS;
-                            for (int bit = bits - 1; bit >= 0 && at_least > REACH; bit--) {
-                                const uint32_t trial = found | 1u << bit;
-                                uint32_t c = 0;
-#pragma unroll
-                                for (int i = 0; i < THREADS / 32; i++) c += k[i] >= trial;
-                                c = __reduce_add_sync(0xffffffffu, c);
-                                if (c >= a.top) { found = trial; at_least = c; }
-                            }
-                            if (lane == 0) sh.bound = at_least <= REACH ? (unsigned long long)found << 32 : ~0ull;
-                        }
-                        __syncthreads();
-                        unsigned long long bound = sh.bound;
-                        if (bound == ~0ull) {    // too many that are equal: by their places too
-                            unsigned long long mine = 0;
-#pragma unroll
-                            for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); mine = k > mine ? k : mine; }
-                            sh.most[tid] = mine;
-                            __syncthreads();
-                            if (warp == 0) {
-                                unsigned long long found = 0;
-                                for (int bit = 63; bit >= 0; bit--) {
-                                    const unsigned long long trial = found | 1ull << bit;
-                                    uint32_t c = 0;
-                                    for (int i = 0; i < THREADS / 32; i++) c += sh.most[lane + 32 * i] >= trial;
-                                    if (__reduce_add_sync(0xffffffffu, c) >= a.top) found = trial;
-                                }
-                                if (lane == 0) sh.bound = found;
-                            }
-                            __syncthreads();
-                            bound = sh.bound;    // the top-th largest, or 0 where there are not so many
-                        }
-                        if (bound > from) from = bound - 1;
-                    }
+            if (at == begin) enter(at, big);
+            else {
+                if ((++round & (round - 1)) == 0 && round > 1) {      // 2, 4, 8, ...: as many logits again as there were. The same for all threads
+                    __syncthreads();
+                    const uint32_t n = sh.entering;
+                    if (n > a.top && n <= CAP) compact(n);
+                    __syncthreads();
                 }
-                __syncthreads();
-                if (from == 0 || big >= key_logit(from)) {
+                const float least = from == 0 ? -INFINITY : key_logit(from);
+                if (big >= least) {
 #pragma unroll
-                    for (int i = 0; i < EACH; i++) { const unsigned long long k = key(i); if (k > from) sh.cand[atomicAdd(&sh.entering, 1u)] = k; }
+                    for (int i = 0; i < EACH; i++)
+                        if (x[i] >= least) {
+                            const unsigned long long k = key(i, at);
+                            if (k > from) { const uint32_t to = atomicAdd(&sh.entering, 1u); if (to < CAP) sh.cand[to] = k; }
+                        }
                 }
             }
         }
@@ -263,7 +290,23 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     if (lane == 0) { sh.part[warp] = me; sh.above[warp] = above; }
     __syncthreads();
     uint32_t listed = 0;
-    if (TOP) listed = put_in_order(sh, sh.entering, a.top);
+    if (TOP) {
+        if (sh.entering > CAP) {
+            __syncthreads();
+            if (tid == 0) sh.entering = 0;
+            __syncthreads();
+            from = 0;
+            for (uint32_t at = begin; at < end; at += FOURS * THREADS) {
+                load(x, at);
+                float big = x[0];
+#pragma unroll
+                for (int i = 1; i < EACH; i++) big = max_nan(big, x[i]);
+                enter(at, big);
+            }
+            __syncthreads();
+        }
+        listed = put_in_order(sh, sh.entering, a.top);
+    }
     if (warp == 0) {
         me = lane < WARPS ? sh.part[lane] : Triple{-INFINITY, 0, 0};
         above = lane < WARPS ? sh.above[lane] : 0u;
@@ -273,12 +316,16 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     cluster_sync();
     if (part == 0) {
         if (TOP && parts > 1) {
+            // of every list at least this many reach the least of their places: together no fewer than are wanted
+            const uint32_t place = (a.top + parts - 1) / parts - 1, of = min(lane, parts - 1);
+            const unsigned long long mark = place < far_u32(there(&sh.listed, of)) ? far_u64(there(&sh.top[place], of)) : 0ull;
+            const uint32_t hi = __reduce_min_sync(0xffffffffu, (uint32_t)(mark >> 32));      // by the logits alone
             if (tid == 0) sh.entering = 0;
             __syncthreads();
             for (uint32_t i = tid; i < parts * a.top; i += THREADS) {
                 const uint32_t c = i / a.top, j = i % a.top;
                 const unsigned long long k = far_u64(there(&sh.top[j], c));
-                if (j < far_u32(there(&sh.listed, c))) sh.cand[atomicAdd(&sh.entering, 1u)] = k;
+                if (j < far_u32(there(&sh.listed, c)) && (uint32_t)(k >> 32) >= hi) sh.cand[atomicAdd(&sh.entering, 1u)] = k;
             }
         }
         // each warp joins the triples of all CTAs, a lane each
@@ -336,9 +383,15 @@ cudaError_t launch(const LogProbArgs& a, uint32_t parts, cudaStream_t st, bool p
 
 cudaError_t launch_log_probs(const LogProbArgs& a, int num_sms, cudaStream_t st, bool pdl) {
     if (!a.rows) return cudaSuccess;
-    // Twice as many CTAs as an SM holds at a time, as long as each has logits for all its threads.
+    // The number of parts by what the busiest SM has to do, in logits: a CTA costs about 6000 besides its own, fewer than three do
+    // not keep an SM's loads going, and more than are resident at a time (four) cost about 15 %. Measured beside fixed numbers: 64 rows of 128256 11.6 us in 8 parts and 17.3 in 16, 256 of
+    // 151643 35.4 in 2 and 37.9 in 4, 300 of 128256 53 in 1 and 38 in 2 or 4.
     uint32_t parts = 1;
-    while (parts < MAX_CLUSTER && (uint64_t)a.rows * parts < 8ull * num_sms && (uint64_t)parts * THREADS * EACH < a.vocab) parts *= 2;
+    double least = 0;
+    for (uint32_t p = 1; p <= MAX_CLUSTER; p *= 2) {
+        const double ctas = (double)a.rows * p, per_sm = ctas / num_sms, cost = (ctas <= 4.0 * num_sms ? std::max(3.0, std::ceil(per_sm)) : 1.15 * per_sm) * (6000.0 + (double)a.vocab / p);
+        if (p == 1 || cost < least) { least = cost; parts = p; }
+    }
     return a.top ? launch<true>(a, parts, st, pdl) : launch<false>(a, parts, st, pdl);
 }
 

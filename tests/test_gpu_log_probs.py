@@ -103,6 +103,15 @@ def test_ties_go_to_the_lowest_index(engine):
     check(engine, np.ascontiguousarray(x[:, ::-1]), rng.integers(0, 9001, 7), 32)
 
 
+@pytest.mark.parametrize("top", [1, 7, 32])
+def test_logits_that_keep_rising(engine, top):
+    """Every logit is above all before it: a list of what exceeds an earlier bound would not end. Rows enough that a CTA has many rounds of one."""
+    x = np.arange(60001, dtype=np.float32)[None] * np.linspace(1e-4, 1e-3, 200, dtype=np.float32)[:, None]
+    x[1::3] = np.floor(x[1::3] * 4) / 4
+    x[2::3] = x[2::3, ::-1]
+    check(engine, x, np.arange(200) * 300, top)
+
+
 def test_tokens_that_are_ruled_out(engine):
     rng = np.random.default_rng(4)
     x = (rng.normal(size=(5, 6000)) * 4).astype(np.float32)
