@@ -53,10 +53,15 @@ struct alignas(32) Kv4Job {
     uint32_t tile0, tile1;       // of the tiles of all jobs of a key / value head
     uint32_t unused;
 };
+struct alignas(16) Kv4Token {
+    uint32_t tile;               // of its page's first head, counted through the pool
+    uint32_t row;                // in the tile
+    uint32_t pos;                // position: row of the rotation table
+    uint32_t unused;
+};
 struct Kv4Plan {
     const Kv4Head* head;
-    const uint32_t* tok_slot;    // [tokens] page * page_tokens + place in it
-    const uint32_t* tok_pos;     // [tokens] row of the rotation table: the position
+    const Kv4Token* token;       // [tokens]
     const Kv4Job* job;           // [jobs]
     const uint32_t* job_tile;    // [jobs] their tile0 by themselves
     const uint32_t* table;       // [seqs][table_ld] pages
@@ -78,6 +83,7 @@ struct Kv4RowsArgs {             // append: k, v read; read: k, v written
     float *k, *v;
     size_t k_ld, v_ld;           // floats from token to token
     uint32_t most_tokens;        // that k and v have room for
+    uint32_t heads;              // key / value heads a warp takes (the launcher's)
     Kv4Rope rope;
     int* status;
 };

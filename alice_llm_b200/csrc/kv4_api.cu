@@ -124,8 +124,8 @@ int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t
     alice_engine_retain(e);
     size_t at = 0;
     auto take = [&](size_t words) { const size_t o = at; at += (words * 4 + 15) & ~size_t(15); return o; };
-    const size_t o_job = take((size_t)b->max_jobs * (sizeof(Kv4Job) / 4)), o_head = take(sizeof(Kv4Head) / 4), o_jtile = take(b->max_jobs), o_slot = take(max_tokens),
-                 o_pos = take(max_tokens), o_table = take((size_t)max_seqs * max_pages);
+    const size_t o_job = take((size_t)b->max_jobs * (sizeof(Kv4Job) / 4)), o_head = take(sizeof(Kv4Head) / 4), o_jtile = take(b->max_jobs), o_token = take((size_t)max_tokens * 4),
+                 o_table = take((size_t)max_seqs * max_pages);
     cudaError_t err = cudaSetDevice(e->device);
     if (err == cudaSuccess) err = cudaMalloc(reinterpret_cast<void**>(&b->blob), at);
     if (err == cudaSuccess) err = cudaMalloc(reinterpret_cast<void**>(&b->part), kv4_part_floats(s.dim, e->num_sms) * sizeof(float));
@@ -135,7 +135,7 @@ int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t
     if (err != cudaSuccess) { alice_kv4_batch_free(b); return alice_cuda_fail(err, who); }
     auto u32 = [&](size_t o) { return reinterpret_cast<const uint32_t*>(b->blob + o); };
     b->plan.head = reinterpret_cast<const Kv4Head*>(b->blob + o_head);
-    b->plan.tok_slot = u32(o_slot); b->plan.tok_pos = u32(o_pos);
+    b->plan.token = reinterpret_cast<const Kv4Token*>(b->blob + o_token);
     b->plan.job = reinterpret_cast<const Kv4Job*>(b->blob + o_job); b->plan.job_tile = u32(o_jtile);
     b->plan.table = u32(o_table); b->plan.table_ld = max_pages;
     *out = b;
@@ -175,7 +175,7 @@ int32_t alice_kv4_batch_set(alice_kv4_batch* b, uint32_t seqs, const uint32_t* p
         CU(cudaStreamIsCapturing(st, &capturing));
         if (capturing != cudaStreamCaptureStatusNone) return alice_cuda_fail(cudaErrorStreamCaptureUnsupported, "alice_kv4_batch_set: lengths and pages of a captured stream");
         Kv4HostPlan h;
-        const bool fits = kv4_make_plan(h, b->shape.dim, b->shape.page_tokens, b->group, seqs, past, tokens, tables, table_ld, b->max_pages);
+        const bool fits = kv4_make_plan(h, b->shape.dim, b->shape.kv_heads, b->shape.page_tokens, b->group, seqs, past, tokens, tables, table_ld, b->max_pages);
         if (!fits || (uint64_t)h.head.tiles * b->shape.kv_heads > 0x7fffffffull)     // tiles of all heads are numbered in 32 bits
             return alice_fail(ALICE_E_SHAPE, "%s: too many tokens over too many positions for one step", who);
         // copies from pageable memory: the vectors have been read when a call returns
@@ -183,7 +183,7 @@ int32_t alice_kv4_batch_set(alice_kv4_batch* b, uint32_t seqs, const uint32_t* p
             return src.empty() ? cudaSuccess : cudaMemcpyAsync(const_cast<void*>(static_cast<const void*>(dst)), src.data(), src.size() * sizeof(src[0]), cudaMemcpyHostToDevice, st);
         };
         CU(up(b->plan.job, h.job)); CU(up(b->plan.job_tile, h.job_tile));
-        CU(up(b->plan.tok_slot, h.slot)); CU(up(b->plan.tok_pos, h.pos)); CU(up(b->plan.table, h.table));
+        CU(up(b->plan.token, h.token)); CU(up(b->plan.table, h.table));
         CU(cudaMemcpyAsync(const_cast<Kv4Head*>(b->plan.head), &h.head, sizeof(Kv4Head), cudaMemcpyHostToDevice, st));
         b->now = h.head;
     } catch (const std::exception&) {

@@ -13,7 +13,8 @@ inline int kv4_check_shape(const char* who, uint32_t pages, uint32_t page_tokens
     if (dim != 64 && dim != 128 && dim != 256) return alice_fail(ALICE_E_SHAPE, "%s: heads of %u; 64, 128 and 256 are built", who, dim);
     if (!page_tokens || page_tokens % KV4_TILE || page_tokens > 4096) return alice_fail(ALICE_E_SHAPE, "%s: pages of %u positions; a multiple of 16 up to 4096 is wanted", who, page_tokens);
     if (kv_heads > 65535) return alice_fail(ALICE_E_SHAPE, "%s: %u key / value heads", who, kv_heads);
-    if ((uint64_t)pages * page_tokens > 0xffffffffull) return alice_fail(ALICE_E_SHAPE, "%s: more than 2^32 positions", who);
+    if ((uint64_t)pages * page_tokens > 0xffffffffull || (uint64_t)pages * kv_heads * (page_tokens / KV4_TILE) > 0xffffffffull)      // places are 32 bits
+        return alice_fail(ALICE_E_SHAPE, "%s: more than 2^32 positions, or pieces of 16 positions of a head", who);
     return ALICE_OK;
 }
 
@@ -61,12 +62,13 @@ inline int kv4_check_batch(const char* who, uint32_t pages, uint32_t page_tokens
 
 struct Kv4HostPlan {
     Kv4Head head{};
-    std::vector<uint32_t> job_tile, slot, pos, table;
+    std::vector<uint32_t> job_tile, table;
+    std::vector<Kv4Token> token;
     std::vector<Kv4Job> job;
 };
 
 // Of checked arguments. Rows of one job see up to `last` keys, those of its last token. false: more than 2^31 tiles.
-inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t page_tokens, uint32_t group, uint32_t seqs, const uint32_t* past, const uint32_t* tokens, const uint32_t* tables,
+inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t kv_heads, uint32_t page_tokens, uint32_t group, uint32_t seqs, const uint32_t* past, const uint32_t* tokens, const uint32_t* tables,
                           uint32_t table_ld, uint32_t max_pages) {
     uint32_t most = 0, total = 0;
     uint64_t tiles = 0;
@@ -84,8 +86,7 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t page_tokens, ui
         h.head.end = std::max(h.head.end, end);
         for (uint32_t i = 0; i < tokens[s]; i++) {
             const uint32_t at = past[s] + i;
-            h.pos.push_back(at);
-            h.slot.push_back(t[at / page_tokens] * page_tokens + at % page_tokens);
+            h.token.push_back({t[at / page_tokens] * kv_heads * (page_tokens / KV4_TILE) + at % page_tokens / KV4_TILE, at % KV4_TILE, at, 0});
         }
         for (uint32_t r = 0; r < tokens[s] * group; r += rows) {
             const uint32_t n = std::min(rows, tokens[s] * group - r), last = past[s] + (r + n - 1) / group + 1, tile0 = (uint32_t)tiles;
