@@ -72,6 +72,8 @@ SIGNATURES = {
     "alice_kv4_attention": (C.c_int32, [_vp, _vp, _vp, _vp, C.c_size_t, _vp, C.c_size_t, _vp, C.c_uint32, C.c_uint32, C.c_float]),
     "alice_log_probs": (C.c_int32, [_vp, _vp, C.c_uint32, C.c_uint32, C.c_size_t, _vp, _vp, _vp, _vp, C.c_uint32, _vp, _vp]),
     "alice_model_create": (C.c_int32, [_vp, _vp, _vp, _vp, _vp, _vp, _pp]),
+    "alice_model_create_kv4": (C.c_int32, [_vp, _vp, _vp, _vp, _vp, _vp, _pp]),
+    "alice_model_log_probs": (C.c_int32, [_vp, _vp, C.c_uint32, _vp, C.c_uint32, _vp, _vp, _vp, _vp, _vp]),
     "alice_model_destroy": (C.c_int32, [_vp]),
     "alice_model_forward": (C.c_int32, [_vp, C.c_uint32]),
     "alice_model_forward_read": (C.c_int32, [_vp, C.c_uint32, _vp]),

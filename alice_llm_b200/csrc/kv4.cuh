@@ -114,6 +114,8 @@ __device__ __forceinline__ bool kv4_fits(const Kv4Head& h, uint32_t most_tokens,
 
 // Rows a job may have, by the most rows a sequence has: 4, 8 or 16 (8 of 256 dims, whose operands would not fit the registers).
 inline uint32_t kv4_job_rows(uint32_t most, uint32_t dim) { return most <= 4 ? 4 : most <= 8 || dim == 256 ? 8 : 16; }
+// Writes `plan` for one sequence's n tokens from position *pos on (or pos0, where pos is null), its pages in order. A single CTA.
+cudaError_t launch_kv4_plan(const Kv4Plan& plan, const Kv4Shape& shape, uint32_t group, uint32_t n, const int* pos, uint32_t pos0, cudaStream_t st, bool pdl);
 size_t kv4_part_floats(uint32_t dim, int num_sms);
 // `tokens`, `jobs`: how many the host knows of; the kernels take the numbers of plan.head and stride over them.
 cudaError_t launch_kv4_append(const Kv4RowsArgs& a, uint32_t tokens, int num_sms, cudaStream_t st, bool pdl);

@@ -151,7 +151,7 @@ __device__ __forceinline__ float half_of(const Words<N>& x, int i) { return i & 
 // (sin, cos) of the pairs that dims dim0 .. dim0 + 3 are in: of two pairs, or (pairs half a head apart) of four.
 struct Turn { float4 a, b; };
 __device__ __forceinline__ Turn turn_at(const float* turn, uint32_t dim0, const Kv4Rope& rope) {
-    auto at = [](const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); };
+    auto at = [](const float* p) { return *reinterpret_cast<const float4*>(p); };
     Turn w{};
     if (dim0 < rope.dims) {
         const uint32_t half = rope.dims / 2, j = rope.neox ? 2 * (dim0 < half ? dim0 : dim0 - half) : dim0;
@@ -187,7 +187,7 @@ __device__ __forceinline__ uint32_t find_job(const uint32_t* job_tile, uint32_t 
     uint32_t lo = 0, n = jobs;
     while (n > 1) {
         const uint32_t step = (n + 31) / 32, i = lo + lane * step;
-        const uint32_t hit = __ballot_sync(0xffffffffu, lane * step < n && __ldg(job_tile + i) <= x);
+        const uint32_t hit = __ballot_sync(0xffffffffu, lane * step < n && job_tile[i] <= x);
         const uint32_t k = 31 - __clz(hit);
         n = min(step, n - k * step);
         lo += k * step;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             p_n = i / per_page; p_in = i - p_n * per_page;
             if (p_base == 0xffffffffu || p_n >= p_base + 32) {
                 p_base = p_n;
-                p_pages = __ldg(pl.table + (size_t)p_seq * pl.table_ld + min(p_n + lane, (p_end - 1 - p_tile0) / per_page));
+                p_pages = pl.table[(size_t)p_seq * pl.table_ld + min(p_n + lane, (p_end - 1 - p_tile0) / per_page)];
             }
         };
         auto found = [&]() {         // and has it
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 for (uint32_t c = 0; c < CH; c++) {
                     const uint32_t at_c = c * 128 + lane * 4, row = at_c / DIM, dim0 = at_c % DIM;
                     const uint32_t r = jb.row + min(row, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
-                    x[c] = __ldg(reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0));
+                    x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0);
                     of[c] = a.rope.by_token ? at_tok : jb.past + tok;
                 }
                 if (a.rope.dims) {

@@ -25,7 +25,7 @@ struct Walk {
         end = min(head + heads, s.kv_heads);
         head += lane / 4 / NB;
         dim0 = block * KV4_BLOCK + sub * 8;
-        const uint4 t = __ldg(reinterpret_cast<const uint4*>(plan.token + tok));
+        const uint4 t = *reinterpret_cast<const uint4*>(plan.token + tok);
         pos = t.z;
         per_head = (size_t)s.tiles() * kv4_tile_bytes(DIM);
         const size_t tile = (size_t)t.x * kv4_tile_bytes(DIM);
@@ -51,7 +51,7 @@ __device__ __forceinline__ T max4(T v, uint32_t mask) {
 
 struct Eight { float v[8]; };
 __device__ __forceinline__ Eight load8(const float* p) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = *reinterpret_cast<const float4*>(p), b = reinterpret_cast<const float4*>(p)[1];
     return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
 struct Held { uint32_t codes; __half d, m; };
@@ -240,6 +240,34 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
             }
         }
     }
+}
+
+// A model's one sequence: what the host works out for a batch (csrc/kv4_plan.cuh), from the position on the device.
+__global__ void __launch_bounds__(256) kv4_plan_kernel(Kv4Plan plan, Kv4Shape s, uint32_t group, uint32_t rows, uint32_t n, const int* pos, uint32_t pos0) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t past = pos ? (uint32_t)*pos : pos0, total = n * group, jobs = (total + rows - 1) / rows, tid = threadIdx.x;
+    auto tiles_of = [&](uint32_t j) { return (past + (min((j + 1) * rows, total) - 1) / group + 1 + KV4_TILE - 1) / KV4_TILE; };
+    for (uint32_t i = tid; i < n; i += blockDim.x) {
+        const uint32_t at = past + i;       // pages in order: page at / page_tokens
+        const_cast<Kv4Token*>(plan.token)[i] = Kv4Token{at / s.page_tokens * s.kv_heads * s.tiles() + at % s.page_tokens / KV4_TILE, at % KV4_TILE, at, 0};
+    }
+    for (uint32_t j = tid; j < jobs; j += blockDim.x) {
+        uint32_t before = 0;
+        for (uint32_t i = 0; i < j; i++) before += tiles_of(i);
+        const_cast<Kv4Job*>(plan.job)[j] = Kv4Job{0, j * rows, min(rows, total - j * rows), 0, past, before, before + tiles_of(j), 0};
+        const_cast<uint32_t*>(plan.job_tile)[j] = before;
+        if (j == jobs - 1) *const_cast<Kv4Head*>(plan.head) = Kv4Head{1, n, jobs, rows, before + tiles_of(j), past + n, (past + n - 1) / s.page_tokens};
+    }
+}
+
+cudaError_t launch_kv4_plan(const Kv4Plan& plan, const Kv4Shape& shape, uint32_t group, uint32_t n, const int* pos, uint32_t pos0, cudaStream_t st, bool pdl) {
+    cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[1];
+    lc.gridDim = dim3(1); lc.blockDim = dim3(256); lc.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at; lc.numAttrs = pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&lc, kv4_plan_kernel, plan, shape, group, kv4_job_rows(n * group, shape.dim), n, pos, pos0);
 }
 
 namespace {

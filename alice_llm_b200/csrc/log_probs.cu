@@ -149,9 +149,9 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     };
     float x[EACH], next[EACH];
     load(x, begin);
-    const uint32_t t = a.target ? __ldg(a.target + r) : 0u;
+    const uint32_t t = a.target ? a.target[r] : 0u;
     const bool aimed = a.target && t < a.vocab;
-    const float xt = aimed ? __ldg(row + t) : INFINITY;
+    const float xt = aimed ? row[t] : INFINITY;
     if (tid == 0) { sh.listed = 0; sh.entering = 0; }
     if (TOP) __syncthreads();
 

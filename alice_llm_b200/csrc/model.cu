@@ -14,6 +14,8 @@
 #include "gemv_blocks.cuh"
 #include "gemv_planes.cuh"
 #include "glue.cuh"
+#include "kv4.cuh"
+#include "kv4_plan.cuh"
 #include "model_base.cuh"
 #include "tp.cuh"
 
@@ -37,6 +39,11 @@ struct LlamaModel final : alice_model {
     // activations, each for up to `cap` tokens: [k][dim]; logits for MAX_BATCH
     float *hidden = nullptr, *qkv = nullptr, *attn_out = nullptr, *ffn_h = nullptr;   // and the base's logits
     float *kcache = nullptr, *vcache = nullptr;  // [layer][max_seq][kv_dim]
+    // or the same in 4 bits (csrc/kv4.cuh): a pool a layer, pages in order, and the plan of a step, written on the device from the position
+    bool kv4 = false;
+    Kv4Shape kv4_shape{};
+    Kv4Plan kv4_plan{};
+    uint8_t* kv4_pool = nullptr;
     float* attn_part = nullptr;
     uint32_t part_vectors = 0;   // vectors of head_dim + 4 it holds
     float* rope_freq = nullptr;  // 1 / theta^(2j / head_dim), j < 64, computed on the host (libm powf, as the CPU path)
@@ -70,9 +77,9 @@ struct LlamaModel final : alice_model {
     uint32_t piece_tokens() const override { return cap; }
     int enqueue_step(uint32_t batch, bool greedy_feed) override { return step(batch, greedy_feed, nullptr, 0, nullptr); }
     // rows == nullptr: logits of the whole batch (at most MAX_BATCH tokens) stay on the device. Else those of rows[0 .. nrows) are
-    // copied to host_logits; the last run of up to MAX_BATCH consecutive rows stays in `logits`.
-    int step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uint32_t nrows, float* host_logits);
-    int enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, float* host_logits) override;
+    // handed to `to`; the last run of up to MAX_BATCH consecutive rows stays in `logits`.
+    int step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uint32_t nrows, LogitsTo* to);
+    int enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, LogitsTo& to) override;
     int clear_state() override;
 };
 
@@ -135,7 +142,7 @@ void fill_dst(PublishDst& d, const Need& nd, uint8_t* q8_base, float* xn, uint32
 // rows into every peer's copy, with one flag per vector that a one-CTA kernel behind it raises on the peers and waits for
 // here before it prepares the vector for the next op. Attention runs on the rank's own KV heads (its q, k, v rows), so
 // only its output needs exchanging (it is the input of the output projection).
-int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uint32_t nrows, float* host_logits) {
+int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uint32_t nrows, LogitsTo* to) {
     LlamaModel* const m = this;
     const alice_model_config& c = m->cfg;
     cudaStream_t st = m->e->stream;
@@ -230,11 +237,12 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
         if (nd0.xn) ea.pub = p;
     }
     MCU(launch_embed_q8_0(ea, st, pdl));
+    if (m->kv4) MCU(launch_kv4_plan(m->kv4_plan, m->kv4_shape, shape.num_heads / shape.num_kv_heads, batch, m->d_pos, 0, st, pdl));
 
     for (uint32_t l = 0; l < L_n; l++) {
         const LlamaModel::Layer& L = m->layers[l];
-        float* kc = m->kcache + (size_t)l * c.max_seq_len * lkv;
-        float* vc = m->vcache + (size_t)l * c.max_seq_len * lkv;
+        float* kc = m->kv4 ? nullptr : m->kcache + (size_t)l * c.max_seq_len * lkv;
+        float* vc = m->kv4 ? nullptr : m->vcache + (size_t)l * c.max_seq_len * lkv;
         const uint32_t qkv_stride = lq + 2 * lkv;
         // attention norm (already applied: hid_q8 / hid_xn) + q, k, v projections (src/llama3.rs:14178-14217)
         if (L.q.fmt == L.k.fmt && L.q.fmt == L.v.fmt) {
@@ -268,7 +276,7 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
         // a K-quant output projection takes the attention output as Q8_K: written by the attention kernel itself when a
         // KV head's outputs are whole blocks, else quantized in the projection's own prologue
         const bool o_q8 = format_uses_q8k(L.o.fmt) && n == 1 && q_dim % 256 == 0 && (batch > 1 || group % 2 == 0);
-        if (o_q8 && batch == 1) {
+        if (o_q8 && batch == 1 && !m->kv4) {
             const Q8KView v = q8_view(m->attn_q8, q_dim, m->cap);
             aa.q8.qs = const_cast<int8_t*>(v.qs); aa.q8.d = const_cast<float*>(v.d); aa.q8.bsums = const_cast<int16_t*>(v.bsums);
         }
@@ -280,7 +288,20 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
             aa.npeers = m->npeers;
             for (uint32_t q = 0; q < m->npeers; q++) aa.peer_out[q] = reinterpret_cast<float*>(on_peer(q, m->attn_out)) + (size_t)r * lq;
         }
-        if (batch == 1) {
+        if (m->kv4) {        // append, then attention over the pages; the vectors as for several tokens
+            Kv4RowsArgs ra{};
+            ra.plan = m->kv4_plan; ra.shape = m->kv4_shape; ra.pool = m->kv4_pool + l * m->kv4_shape.bytes();
+            ra.k = m->qkv + lq; ra.v = m->qkv + lq + lkv; ra.k_ld = ra.v_ld = qkv_stride; ra.most_tokens = m->cap; ra.status = m->e->status;
+            ra.rope = Kv4Rope{m->rope_tab, c.head_dim, c.neox_rope, 1, m->cap};
+            MCU(launch_kv4_append(ra, batch, m->e->num_sms, st, pdl));
+            Kv4AttnArgs ta{};
+            ta.plan = ra.plan; ta.shape = ra.shape; ta.pool = ra.pool; ta.q = m->qkv; ta.q_ld = qkv_stride; ta.out = m->attn_out; ta.out_ld = q_dim;
+            ta.most_tokens = m->cap; ta.group = group; ta.scale = 1.0f / std::sqrt((float)c.head_dim); ta.rope = ra.rope; ta.part = m->attn_part; ta.tickets = m->attn_tickets;
+            ta.status = m->e->status;
+            const uint32_t rows_of = kv4_job_rows(batch * group, c.head_dim);
+            MCU(launch_kv4_attention(ta, rows_of, (batch * group + rows_of - 1) / rows_of, m->e->num_sms, st, pdl));
+            if (o_q8) { launch_quantize_q8k(m->attn_out, q_dim, batch, m->attn_q8, st, pdl, m->cap); MCU(cudaGetLastError()); }
+        } else if (batch == 1) {
             aa.nsplit = std::max<uint32_t>(1, std::min(m->nsplit, (uint32_t)m->e->num_sms / shape.num_kv_heads));      // a CTA an SM
             MCU(launch_attention(aa, st, pdl));
         } else {
@@ -368,7 +389,7 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
             if ((rc = tp_all_gather(m->e, m->logits, (size_t)m->lV * sizeof(float)))) return rc;
             if ((rc = tp_all_gather(m->e, m->argmax_keys, sizeof(unsigned long long)))) return rc;
         }
-        if (rows) MCU(cudaMemcpyAsync(host_logits + (size_t)i * V, m->logits, (size_t)len * V * 4, cudaMemcpyDeviceToHost, st));
+        if (rows && (rc = to->take(m, m->logits, i, len))) return rc;
         i += rows ? len : 1;
     }
     MCU(launch_finish_step(m->argmax_keys, m->tp_n, m->d_token, m->d_pos, m->d_trace, greedy_feed ? 1 : 0, batch,
@@ -378,15 +399,18 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
 }
 
 // A single token always has its logits (and its argmax) left on the device.
-int LlamaModel::enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, float* host_logits) {
+int LlamaModel::enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, LogitsTo& to) {
     static const uint32_t none = 0;
-    if (n > 1) return step(n, false, rows ? rows : &none, nrows, host_logits);
+    if (n > 1) return step(n, false, rows ? rows : &none, nrows, &to);
     const int rc = step(1, false, nullptr, 0, nullptr);
-    if (!rc && nrows) MCU(cudaMemcpyAsync(host_logits, logits, (size_t)cfg.vocab_size * 4, cudaMemcpyDeviceToHost, e->stream));
-    return rc;
+    return !rc && nrows ? to.take(this, logits, 0, 1) : rc;
 }
 
 int LlamaModel::clear_state() {
+    if (kv4) {
+        MCU(cudaMemsetAsync(kv4_pool, 0, kv4_shape.bytes() * cfg.num_layers, e->stream));
+        return ALICE_OK;
+    }
     const size_t kv_bytes = (size_t)cfg.num_layers * cfg.max_seq_len * lkv * 4;
     MCU(cudaMemsetAsync(kcache, 0, kv_bytes, e->stream));
     MCU(cudaMemsetAsync(vcache, 0, kv_bytes, e->stream));
@@ -399,10 +423,8 @@ bool same_shape(const WeightDesc& w, uint32_t rows, uint32_t cols) { return w.ro
 
 extern "C" {
 
-int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const alice_layer_weights* layers,
-                           const alice_weights* embedding, const float* output_norm, const alice_weights* output,
-                           alice_model** out) {
-    const char* who = "alice_model_create";
+static int create(const char* who, bool kv4, alice_engine* e, const alice_model_config* cfg, const alice_layer_weights* layers, const alice_weights* embedding,
+                  const float* output_norm, const alice_weights* output, alice_model** out) {
     if (!e || !cfg || !layers || !embedding || !output_norm || !output || !out) return alice_fail(ALICE_E_INVALID, "%s: null argument", who);
     *out = nullptr;
     const alice_model_config& c = *cfg;
@@ -416,6 +438,7 @@ int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const
     const uint32_t q_dim = c.num_heads * c.head_dim, kv_dim = c.num_kv_heads * c.head_dim;
     // tensor-parallel group of the engine: the weight handles are this rank's row shards
     const uint32_t n = e->tp_world;
+    if (kv4 && n > 1) return alice_fail(ALICE_E_UNSUPPORTED, "%s: the 4-bit cache is single-GPU only", who);
     if (c.num_kv_heads % n || c.hidden_dim % n || c.intermediate_dim % n || c.vocab_size % n)
         return alice_fail(ALICE_E_SHAPE, "%s: kv heads %u, hidden %u, ffn %u and vocab %u must all divide by the group size %u", who,
                           c.num_kv_heads, c.hidden_dim, c.intermediate_dim, c.vocab_size, n);
@@ -476,11 +499,37 @@ int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const
         }
     }
     if (!rc) rc = dev_alloc(m, &m->qkv, (size_t)B * (lq + 2 * lkv));
-    if (!rc) rc = dev_alloc(m, &m->kcache, kv_elems);
-    if (!rc) rc = dev_alloc(m, &m->vcache, kv_elems);
+    m->kv4 = kv4;
+    if (!kv4) {
+        if (!rc) rc = dev_alloc(m, &m->kcache, kv_elems);
+        if (!rc) rc = dev_alloc(m, &m->vcache, kv_elems);
+    } else {
+        constexpr uint32_t PAGE = 64;
+        const uint32_t pages = (uint32_t)(((uint64_t)c.max_seq_len + PAGE - 1) / PAGE);
+        if (!rc) rc = kv4_check_shape(who, pages, PAGE, c.num_kv_heads, c.head_dim);
+        if (!rc) rc = kv4_check_limits(who, c.num_kv_heads, c.head_dim, c.num_heads, 1, B, pages);
+        m->kv4_shape = Kv4Shape{pages, PAGE, c.num_kv_heads, c.head_dim};
+        const uint32_t jobs = kv4_max_jobs(1, B, group, c.head_dim);
+        Kv4Head* head = nullptr; Kv4Token* token = nullptr; Kv4Job* job = nullptr;
+        uint32_t *tile = nullptr, *table = nullptr;
+        if (!rc) rc = dev_alloc(m, &m->kv4_pool, m->kv4_shape.bytes() * c.num_layers);
+        if (!rc) rc = dev_alloc(m, &head, 1);
+        if (!rc) rc = dev_alloc(m, &token, B);
+        if (!rc) rc = dev_alloc(m, &job, jobs);
+        if (!rc) rc = dev_alloc(m, &tile, jobs);
+        if (!rc) rc = dev_alloc(m, &table, pages);
+        if (!rc) {
+            std::vector<uint32_t> order(pages);
+            for (uint32_t p = 0; p < pages; p++) order[p] = p;
+            const cudaError_t err = cudaMemcpy(table, order.data(), (size_t)pages * 4, cudaMemcpyHostToDevice);
+            if (err != cudaSuccess) rc = alice_cuda_fail(err, who);
+        }
+        m->kv4_plan = Kv4Plan{head, token, job, tile, table, pages};
+    }
     m->part_vectors = MAX_BATCH * m->nsplit * (c.num_heads / n);
-    if (!rc) rc = dev_alloc(m, &m->attn_part, (size_t)m->part_vectors * (c.head_dim + 4));
-    if (!rc) rc = dev_alloc(m, &m->attn_tickets, c.num_kv_heads / n);
+    const uint32_t tickets = kv4 ? (uint32_t)e->num_sms : c.num_kv_heads / n;
+    if (!rc) rc = dev_alloc(m, &m->attn_part, kv4 ? kv4_part_floats(c.head_dim, e->num_sms) : (size_t)m->part_vectors * (c.head_dim + 4));
+    if (!rc) rc = dev_alloc(m, &m->attn_tickets, tickets);
     if (!rc) rc = dev_alloc(m, &m->rope_tab, (size_t)B * 128);
     if (!rc) rc = dev_alloc(m, &m->rope_freq, 64);
     if (!rc) rc = dev_alloc(m, &m->hid_q8, Q8KLayout::make((c.hidden_dim + 255) / 256, B).total);
@@ -500,10 +549,11 @@ int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const
         float freq[64];
         for (int j = 0; j < 64; j++) freq[j] = 1.0f / std::pow(c.rope_theta, (float)(2 * j) / (float)c.head_dim);
         cudaError_t err = cudaMemcpy(m->rope_freq, freq, sizeof freq, cudaMemcpyHostToDevice);
-        if (err == cudaSuccess) err = cudaMemsetAsync(m->kcache, 0, kv_elems * 4, e->stream);
-        if (err == cudaSuccess) err = cudaMemsetAsync(m->vcache, 0, kv_elems * 4, e->stream);
+        if (err == cudaSuccess && kv4) err = cudaMemsetAsync(m->kv4_pool, 0, m->kv4_shape.bytes() * c.num_layers, e->stream);
+        if (err == cudaSuccess && !kv4) err = cudaMemsetAsync(m->kcache, 0, kv_elems * 4, e->stream);
+        if (err == cudaSuccess && !kv4) err = cudaMemsetAsync(m->vcache, 0, kv_elems * 4, e->stream);
         if (err == cudaSuccess) err = cudaMemsetAsync(m->d_pos, 0, 4, e->stream);
-        if (err == cudaSuccess) err = cudaMemsetAsync(m->attn_tickets, 0, (size_t)(c.num_kv_heads / n) * 4, e->stream);
+        if (err == cudaSuccess) err = cudaMemsetAsync(m->attn_tickets, 0, (size_t)tickets * 4, e->stream);
         if (err == cudaSuccess) err = cudaMemsetAsync(m->d_token, 0, 4 * B, e->stream);
         if (err == cudaSuccess) err = cudaMemsetAsync(m->d_trace, 0, (size_t)c.max_seq_len * 4, e->stream);
         if (err == cudaSuccess) err = cudaStreamSynchronize(e->stream);
@@ -513,6 +563,17 @@ int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const
     if (rc) { alice_model_destroy(m); return rc; }
     *out = m;
     return ALICE_OK;
+}
+
+int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const alice_layer_weights* layers,
+                           const alice_weights* embedding, const float* output_norm, const alice_weights* output,
+                           alice_model** out) {
+    return create("alice_model_create", false, e, cfg, layers, embedding, output_norm, output, out);
+}
+
+int32_t alice_model_create_kv4(alice_engine* e, const alice_model_config* cfg, const alice_layer_weights* layers, const alice_weights* embedding,
+                               const float* output_norm, const alice_weights* output, alice_model** out) {
+    return create("alice_model_create_kv4", true, e, cfg, layers, embedding, output_norm, output, out);
 }
 
 int32_t alice_model_tp_export(alice_model* base, void* out, size_t nbytes) {
@@ -569,6 +630,27 @@ static int kv_copy(alice_model* base, uint32_t layer, uint32_t pos0, uint32_t np
     const size_t off = ((size_t)layer * c.max_seq_len + pos0) * kv_dim, bytes = (size_t)npos * kv_dim * 4;
     cudaStream_t st = m->e->stream;
     MCU(cudaSetDevice(m->e->device));
+    if (m->kv4) {        // rows as they are (keys rotated by the caller), a step's worth at a time through the place of q, k, v
+        for (uint32_t lo = 0; lo < npos; lo += m->cap) {
+            const uint32_t k_n = std::min(m->cap, npos - lo);
+            const size_t part = (size_t)k_n * kv_dim;
+            Kv4RowsArgs ra{};
+            ra.plan = m->kv4_plan; ra.shape = m->kv4_shape; ra.pool = m->kv4_pool + layer * m->kv4_shape.bytes();
+            ra.k = m->qkv; ra.v = m->qkv + part; ra.k_ld = ra.v_ld = kv_dim; ra.most_tokens = k_n; ra.status = m->e->status;
+            MCU(launch_kv4_plan(m->kv4_plan, m->kv4_shape, c.num_heads / c.num_kv_heads, k_n, nullptr, pos0 + lo, st, m->e->pdl));
+            if (to_device) {
+                MCU(cudaMemcpyAsync(ra.k, k + (size_t)lo * kv_dim, part * 4, cudaMemcpyHostToDevice, st));
+                MCU(cudaMemcpyAsync(ra.v, v + (size_t)lo * kv_dim, part * 4, cudaMemcpyHostToDevice, st));
+                MCU(launch_kv4_append(ra, k_n, m->e->num_sms, st, m->e->pdl));
+            } else {
+                MCU(launch_kv4_read(ra, k_n, m->e->num_sms, st, m->e->pdl));
+                MCU(cudaMemcpyAsync(k + (size_t)lo * kv_dim, ra.k, part * 4, cudaMemcpyDeviceToHost, st));
+                MCU(cudaMemcpyAsync(v + (size_t)lo * kv_dim, ra.v, part * 4, cudaMemcpyDeviceToHost, st));
+            }
+        }
+        MCU(cudaStreamSynchronize(st));
+        return ALICE_OK;
+    }
     if (to_device) {
         MCU(cudaMemcpyAsync(m->kcache + off, k, bytes, cudaMemcpyHostToDevice, st));
         MCU(cudaMemcpyAsync(m->vcache + off, v, bytes, cudaMemcpyHostToDevice, st));

@@ -1,8 +1,10 @@
 // The alice_model_* entry points that are the same for every model family (include/alice_cuda.h): stepping, greedy decoding
 // from a captured graph, logits, position. GpuModel of ALICE-LLM src/gpu.rs:5010-6094.
 #include <cstring>
+#include <exception>
 #include <vector>
 
+#include "log_probs.cuh"
 #include "model_base.cuh"
 
 namespace {
@@ -31,7 +33,25 @@ int set_tokens(alice_model* m, const uint32_t* tokens, uint32_t n) {
     return to_device(m, m->d_token, tokens, n);
 }
 
+// What is asked of each row of logits, worked out where they are.
+struct LogitsToScores final : LogitsTo {
+    alice::LogProbArgs args;
+    int take(alice_model* m, const float* logits, uint32_t first, uint32_t k) override {
+        alice::LogProbArgs a = args;
+        a.x = logits; a.ld = a.vocab = m->vocab; a.rows = k;
+        a.target += first; a.lp += first; a.entropy += first; a.rank += first;
+        if (a.top) { a.top_ids += (size_t)first * a.top; a.top_lp += (size_t)first * a.top; }
+        MCU(alice::launch_log_probs(a, m->e->num_sms, m->e->stream, m->e->pdl));
+        return ALICE_OK;
+    }
+};
+
 }  // namespace
+
+int LogitsToHost::take(alice_model* m, const float* logits, uint32_t first, uint32_t k) {
+    MCU(cudaMemcpyAsync(host + (size_t)first * m->vocab, logits, (size_t)k * m->vocab * 4, cudaMemcpyDeviceToHost, m->e->stream));
+    return ALICE_OK;
+}
 
 void alice_model::make_stage() {
     if (cudaMallocHost(&stage, (size_t)STAGE_ROWS * vocab * 4) != cudaSuccess) { stage = nullptr; cudaGetLastError(); }
@@ -92,7 +112,8 @@ int32_t alice_model_forward_rows(alice_model* m, const uint32_t* tokens, uint32_
         local.clear();
         while (done + local.size() < nrows && rows[done + local.size()] < lo + k) local.push_back(rows[done + local.size()] - lo);
         rc = set_tokens(m, tokens + lo, k);
-        if (!rc) rc = m->enqueue_rows(k, local.data(), (uint32_t)local.size(), to + (size_t)done * m->vocab);
+        LogitsToHost host(to + (size_t)done * m->vocab);
+        if (!rc) rc = m->enqueue_rows(k, local.data(), (uint32_t)local.size(), host);
         if (!rc) m->pos += k;
         done += (uint32_t)local.size();
         lo += k;
@@ -101,6 +122,52 @@ int32_t alice_model_forward_rows(alice_model* m, const uint32_t* tokens, uint32_
     rc = alice_sync(m->e);
     if (to != logits && nrows) memcpy(logits, to, (size_t)nrows * m->vocab * 4);
     return rc;
+}
+
+int32_t alice_model_log_probs(alice_model* m, const uint32_t* tokens, uint32_t n, const uint32_t* targets, uint32_t top, float* log_probs, float* entropy,
+                              uint32_t* rank, uint32_t* top_ids, float* top_log_probs) {
+    const char* who = "alice_model_log_probs";
+    if (!m || (n && (!tokens || !targets || !log_probs))) return alice_fail(ALICE_E_INVALID, "%s: null argument", who);
+    if (top > alice::LOGP_MAX_TOP || top > m->vocab) return alice_fail(ALICE_E_SHAPE, "%s: %u alternatives; up to %u, and no more than %u tokens", who, top, alice::LOGP_MAX_TOP, m->vocab);
+    if (n && top && (!top_ids || !top_log_probs)) return alice_fail(ALICE_E_INVALID, "%s: %u alternatives without room for them", who, top);
+    if (n == 0) return ALICE_OK;
+    for (uint32_t i = 0; i < n; i++)
+        if (targets[i] >= m->vocab) return alice_fail(ALICE_E_INVALID, "%s: target %u >= vocab %u", who, targets[i], m->vocab);
+    MCU(cudaSetDevice(m->e->device));
+    int rc = check_room(m, n, who);
+    if (rc) return rc;
+    const uint32_t piece = m->piece_tokens();
+    constexpr uint32_t MOST = 2048;                  // tokens a piece may have in any family
+    if (piece > MOST) return alice_fail(ALICE_E_SHAPE, "%s: pieces of %u tokens", who, piece);
+    if (!m->scores && (rc = dev_alloc(m, &m->scores, (size_t)MOST * (4 + 2 * alice::LOGP_MAX_TOP)))) return rc;
+    uint32_t* const at = m->scores;
+    LogitsToScores to;
+    to.args = alice::LogProbArgs{};
+    to.args.target = at; to.args.lp = reinterpret_cast<float*>(at + MOST); to.args.entropy = reinterpret_cast<float*>(at + 2 * MOST); to.args.rank = at + 3 * MOST;
+    to.args.top = top; to.args.top_ids = at + 4 * MOST; to.args.top_lp = reinterpret_cast<float*>(at + (4 + alice::LOGP_MAX_TOP) * MOST);
+    cudaStream_t st = m->e->stream;
+    try {
+        std::vector<uint32_t> rows(std::min(piece, n));
+        for (uint32_t i = 0; i < rows.size(); i++) rows[i] = i;
+        for (uint32_t lo = 0; lo < n; lo += piece) {
+            const uint32_t k = std::min(piece, n - lo);
+            if ((rc = set_tokens(m, tokens + lo, k))) return rc;
+            if ((rc = to_device(m, reinterpret_cast<int*>(at), targets + lo, k))) return rc;
+            if ((rc = m->enqueue_rows(k, rows.data(), k, to))) return rc;
+            m->pos += k;
+            // pageable memory: the next piece does not overwrite what has not been read
+            MCU(cudaMemcpyAsync(log_probs + lo, to.args.lp, (size_t)k * 4, cudaMemcpyDeviceToHost, st));
+            if (entropy) MCU(cudaMemcpyAsync(entropy + lo, to.args.entropy, (size_t)k * 4, cudaMemcpyDeviceToHost, st));
+            if (rank) MCU(cudaMemcpyAsync(rank + lo, to.args.rank, (size_t)k * 4, cudaMemcpyDeviceToHost, st));
+            if (top) {
+                MCU(cudaMemcpyAsync(top_ids + (size_t)lo * top, to.args.top_ids, (size_t)k * top * 4, cudaMemcpyDeviceToHost, st));
+                MCU(cudaMemcpyAsync(top_log_probs + (size_t)lo * top, to.args.top_lp, (size_t)k * top * 4, cudaMemcpyDeviceToHost, st));
+            }
+        }
+    } catch (const std::exception&) {
+        return alice_fail(ALICE_E_NOMEM, "%s: host allocation failed", who);
+    }
+    return alice_sync(m->e);
 }
 
 int32_t alice_model_forward_batch_read(alice_model* m, const uint32_t* tokens, uint32_t n, float* logits) {

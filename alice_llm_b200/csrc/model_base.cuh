@@ -6,6 +6,18 @@
 
 #include "abi_internal.cuh"
 
+struct alice_model;
+// Where rows of logits go as a forward pass makes them: `k` rows on the device, the wanted ones from `first` on. Queues work only.
+struct LogitsTo {
+    virtual ~LogitsTo() = default;
+    virtual int take(alice_model* m, const float* logits, uint32_t first, uint32_t k) = 0;
+};
+struct LogitsToHost final : LogitsTo {
+    float* host;
+    explicit LogitsToHost(float* h) : host(h) {}
+    int take(alice_model* m, const float* logits, uint32_t first, uint32_t k) override;
+};
+
 struct alice_model {
     alice_engine* e = nullptr;
     uint32_t vocab = 0, max_seq = 0;
@@ -22,6 +34,7 @@ struct alice_model {
     // could be had: the copies then go straight to the caller.
     static constexpr uint32_t STAGE_ROWS = 8;
     float* stage = nullptr;
+    uint32_t* scores = nullptr;                  // of alice_model_log_probs: targets and results of a piece, from the first call on
 
     virtual ~alice_model() = default;
     // Most consecutive tokens enqueue_step takes, and the pieces a prompt is cut into for enqueue_rows.
@@ -30,8 +43,8 @@ struct alice_model {
     // Queues n consecutive tokens (read from d_token) at the current position: leaves logits and advances *d_pos. With
     // greedy_feed (n == 1) the argmax becomes the next token and is recorded in d_trace.
     virtual int enqueue_step(uint32_t n, bool greedy_feed) = 0;
-    // The same n tokens with the logits of rows[0 .. nrows) (ascending, < n) copied to host_logits [nrows][vocab].
-    virtual int enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, float* host_logits) = 0;
+    // The same n tokens with the logits of rows[0 .. nrows) (ascending, < n) handed to `to`.
+    virtual int enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, LogitsTo& to) = 0;
     // Queues clearing of everything a sequence leaves behind.
     virtual int clear_state() = 0;
     void make_stage();                           // at the end of creation

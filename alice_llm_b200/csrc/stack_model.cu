@@ -78,7 +78,7 @@ struct StackModel final : alice_model {
     uint32_t runs() const { return cfg.num_layers + (cfg.loop_times ? (cfg.loop_times - 1) * (cfg.loop_stop - cfg.loop_start) : 0); }
     uint32_t max_tokens() const override { return tracing ? std::min(chunk, TRACE_TOKENS) : chunk; }
     int enqueue_step(uint32_t n, bool greedy_feed) override;
-    int enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, float* host_logits) override;
+    int enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, LogitsTo& to) override;
     int clear_state() override;
     bool can_return_to(uint32_t p) const override {
         if (p == pos || p == 0) return true;
@@ -425,12 +425,12 @@ int StackModel::enqueue_step(uint32_t n, bool greedy_feed) {
     return ALICE_OK;
 }
 
-int StackModel::enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, float* host_logits) {
+int StackModel::enqueue_rows(uint32_t n, const uint32_t* rows, uint32_t nrows, LogitsTo& to) {
     int rc = body(n);
     for (uint32_t i = 0; i < nrows && !rc; i += MAX_NORM_ROWS) {
         const uint32_t k = std::min(MAX_NORM_ROWS, nrows - i);
         rc = head(n, rows + i, k, false);
-        if (!rc) MCU(cudaMemcpyAsync(host_logits + (size_t)i * vocab, logits, (size_t)k * vocab * 4, cudaMemcpyDeviceToHost, e->stream));
+        if (!rc) rc = to.take(this, logits, i, k);
     }
     if (rc) return rc;
     MCU(launch_finish_step(argmax_keys, 1, d_token, d_pos, d_trace, 0, n, nullptr, e->stream, e->pdl));

@@ -595,7 +595,10 @@ class GpuModel:
         engine._children.add(self)
 
     @classmethod
-    def load(cls, engine: GpuEngine, model: dict, config: GpuModelConfig | None = None) -> "GpuModel":
+    def load(cls, engine: GpuEngine, model: dict, config: GpuModelConfig | None = None, kv_cache: str = "f32") -> "GpuModel":
+        """kv_cache "q4": keys and values in 4 bits with a step and a minimum for every 32 (single GPU)."""
+        if kv_cache not in ("f32", "q4"):
+            raise AliceError(_lib.E_INVALID, f"GpuModel.load: kv_cache {kv_cache!r} is neither \"f32\" nor \"q4\"")
         cfg = config or GpuModelConfig.from_dict(model["config"])
         q_dim, kv_dim = cfg.num_heads * cfg.head_dim, cfg.num_kv_heads * cfg.head_dim
         H, F = cfg.hidden_dim, cfg.intermediate_dim
@@ -646,24 +649,24 @@ class GpuModel:
         c = _lib.ModelConfig(cfg.num_layers, H, F, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim, cfg.vocab_size,
                              cfg.max_seq_len, cfg.rope_theta, cfg.eps, int(cfg.neox_rope))
         h = C.c_void_p()
-        check(engine._lib.alice_model_create(engine._h, C.byref(c), C.byref(layers), emb._h, _ptr(onorm), out._h,
-                                             C.byref(h)))
+        create = engine._lib.alice_model_create_kv4 if kv_cache == "q4" else engine._lib.alice_model_create
+        check(create(engine._h, C.byref(c), C.byref(layers), emb._h, _ptr(onorm), out._h, C.byref(h)))
         return cls(engine, h, cfg, keep)
 
     @classmethod
-    def load_shared(cls, engine: GpuEngine, model: dict, config: GpuModelConfig | None = None) -> "GpuModel":
+    def load_shared(cls, engine: GpuEngine, model: dict, config: GpuModelConfig | None = None, kv_cache: str = "f32") -> "GpuModel":
         """GpuModel::load_shared (src/gpu.rs:2837): a model on an engine other models already use (draft and target of
         speculative decoding share device, stream and scratch). Engines here are shared by reference, so this is
         ``load``; the models' steps run in the order they are queued on the engine's stream."""
-        return cls.load(engine, model, config)
+        return cls.load(engine, model, config, kv_cache)
 
     @classmethod
-    def load_gguf(cls, engine: GpuEngine, path, max_seq_len=None) -> "GpuModel":
+    def load_gguf(cls, engine: GpuEngine, path, max_seq_len=None, kv_cache: str = "f32") -> "GpuModel":
         """GpuModel::load (src/gpu.rs:2831) from a GGUF file: the file is mapped, the raw blocks of every tensor of
         the name table go to the device as they are (this rank's row shards on a tensor-parallel engine)."""
         from .gguf_file import GgufFile
         gf = GgufFile.open(path)
-        gm = cls.load(engine, gf.load_model(max_seq_len))
+        gm = cls.load(engine, gf.load_model(max_seq_len), kv_cache=kv_cache)
         gm._keep.append(gf)
         return gm
 
@@ -739,6 +742,23 @@ class GpuModel:
         out = np.empty((r.size, self._config.vocab_size), np.float32)
         check(self.engine._lib.alice_model_forward_rows(self._h, _ptr(t), t.size, _ptr(r), r.size, _ptr(out)))
         return out
+
+    def log_probs(self, token_ids, targets=None, top: int = 0) -> dict:
+        """Consecutive tokens from the present position and, behind each, what the model gives its target: {"log_probs", "entropy", "rank"}
+        and with `top` > 0 "top_ids", "top_log_probs" [tokens, top]. Without targets a text is scored: all but its last token are fed, each
+        with the next one as its target."""
+        t = _np(token_ids, np.uint32).reshape(-1)
+        if targets is None:
+            t, g = _np(t[:-1], np.uint32), _np(t[1:], np.uint32)
+        else:
+            g = _np(targets, np.uint32).reshape(-1)
+        if t.size != g.size:
+            raise AliceError(_lib.E_SHAPE, f"log_probs: {t.size} tokens and {g.size} targets")
+        n, k = t.size, min(max(int(top), 0), 1024)     # more than there may be is refused by the call
+        out = {"log_probs": np.empty(n, np.float32), "entropy": np.empty(n, np.float32), "rank": np.empty(n, np.uint32),
+               "top_ids": np.empty((n, k), np.uint32), "top_log_probs": np.empty((n, k), np.float32)}
+        check(self.engine._lib.alice_model_log_probs(self._h, _ptr(t), n, _ptr(g), int(top), *(_ptr(out[x]) for x in ("log_probs", "entropy", "rank", "top_ids", "top_log_probs"))))
+        return out if top else {x: out[x] for x in ("log_probs", "entropy", "rank")}
 
     def generate(self, prompt, n: int) -> np.ndarray:
         """n greedy tokens after `prompt` from the present position (Llama3Model::generate, src/llama3.rs:16084): the prompt

@@ -203,7 +203,8 @@ int32_t alice_kv4_free(alice_kv4* c);
  * a sequence needs are not looked at, and of a sequence without new tokens none. Sequences may share pages, but none that this step
  * writes into may occur twice among the written ones. Set is not possible in a stream capture; a captured append, read or attention
  * works at its replay on what the batch was set to last, provided that asks for as many rows a job (up to 4, up to 8, or more
- * (token, head) rows of the sequence with most; else alice_sync reports ALICE_E_KERNEL) and fits the buffers and tables of the capture.
+ * (token, head) rows of the sequence with most) and fits the buffers and tables of the capture; else it does nothing and alice_sync reports
+ * ALICE_E_KERNEL.
  * alice_kv4_batch_check: the checks of set alone, on the host. */
 typedef struct alice_kv4_batch alice_kv4_batch;
 int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t heads, uint32_t max_seqs, uint32_t max_tokens, uint32_t max_pages,
@@ -280,6 +281,10 @@ typedef struct {                       /* one transformer layer; norms are host 
 int32_t alice_model_create(alice_engine* e, const alice_model_config* cfg, const alice_layer_weights* layers,
                            const alice_weights* embedding, const float* output_norm, const alice_weights* output,
                            alice_model** out);
+/* The same model with its keys and values in 4 bits (the format of alice_kv4, in one pool a layer): 160 bytes a position and key / value
+ * head instead of 1024. alice_model_kv_write rounds to the format, alice_model_kv_read gives what is held. Single GPU only. */
+int32_t alice_model_create_kv4(alice_engine* e, const alice_model_config* cfg, const alice_layer_weights* layers,
+                               const alice_weights* embedding, const float* output_norm, const alice_weights* output, alice_model** out);
 int32_t alice_model_destroy(alice_model* m);
 /* GpuModel::forward / forward_and_read (src/gpu.rs:5010, 5033): one token at the current position. */
 int32_t alice_model_forward(alice_model* m, uint32_t token);
@@ -303,6 +308,11 @@ int32_t alice_model_read_logits(alice_model* m, float* logits);
  * (ascending places among these tokens, possibly none) written to logits[i * vocab + v]. Blocks. The prompt phase of
  * Llama3Model::generate (src/llama3.rs:16084), which looks at the last token's logits only. */
 int32_t alice_model_forward_rows(alice_model* m, const uint32_t* tokens, uint32_t n, const uint32_t* rows, uint32_t nrows, float* logits);
+/* n consecutive tokens like alice_model_forward_rows, and of the logits behind each of them what alice_log_probs says about targets[i]
+ * (the text's next token, to score a text): log_probs[n]; entropy[n], rank[n] (either may be null); top_ids, top_log_probs [n][top]. The
+ * logits stay on the device. Blocks. */
+int32_t alice_model_log_probs(alice_model* m, const uint32_t* tokens, uint32_t n, const uint32_t* targets, uint32_t top, float* log_probs, float* entropy,
+                              uint32_t* rank, uint32_t* top_ids, float* top_log_probs);
 /* Tensor parallel without collective calls: after every rank has created its model, each exports a handle to its
  * exchange region (ALICE_TP_HANDLE_BYTES; CUDA IPC, same node), the host gathers the handles of all ranks in rank
  * order and every rank connects. From then on the kernel that produces a sharded vector stores its rows straight
