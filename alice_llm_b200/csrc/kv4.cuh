@@ -23,6 +23,7 @@
 namespace alice {
 
 constexpr uint32_t KV4_BLOCK = 32, KV4_TILE = 16;
+constexpr uint32_t KV4_PROMPT_ROWS = 128;      // of a job of csrc/kv4_prompt.cu
 
 __host__ __device__ constexpr uint32_t kv4_tile_bytes(uint32_t dim) { return 20 * dim; }
 __host__ __device__ constexpr uint32_t kv4_v_codes(uint32_t dim) { return 8 * dim; }
@@ -44,6 +45,7 @@ struct Kv4Head {
     uint32_t seqs, tokens, jobs, rows;   // rows: (token, query head) rows of a job
     uint32_t tiles;                      // of all jobs of one key / value head
     uint32_t end, top_page;              // positions of the longest sequence, highest page of a table
+    uint32_t prompt_jobs;                // behind the others, of sequences with many rows
 };
 
 // A job: up to `rows` of Kv4Head consecutive (token, query head of the group) rows of a sequence, against the keys the last of them sees.
@@ -97,6 +99,7 @@ struct Kv4AttnArgs {
     size_t q_ld, out_ld;
     uint32_t most_tokens;
     uint32_t group;              // query heads a key / value head
+    uint32_t rows, prompt_jobs;  // of what is launched: rows of a job, 0: only prompts; prompt jobs at most
     float scale;
     Kv4Rope rope;
     float* part;                 // scratch of the joins, kv4_part_floats
@@ -105,14 +108,19 @@ struct Kv4AttnArgs {
 };
 
 // A captured call meets what the batch is at its replay: whether that stays within the buffers, tables and pages of the call.
-__device__ __forceinline__ bool kv4_fits(const Kv4Head& h, uint32_t most_tokens, const Kv4Rope& rope, const Kv4Shape& shape, uint32_t rows, int* status) {
-    const bool ok = h.tokens <= most_tokens && (!rope.table || (rope.by_token ? h.tokens : h.end) <= rope.rows) && (!h.tokens || h.top_page < shape.pages) &&
-                    (!rows || !h.tokens || h.rows == rows);
+__device__ __forceinline__ bool kv4_fits(const Kv4Head& h, uint32_t most_tokens, const Kv4Rope& rope, const Kv4Shape& shape, int* status, bool launched = true) {
+    const bool ok = launched && h.tokens <= most_tokens && (!rope.table || (rope.by_token ? h.tokens : h.end) <= rope.rows) && (!h.tokens || h.top_page < shape.pages);
     if (!ok && threadIdx.x == 0) atomicCAS(status, 0, KERR_KV4_BATCH);
     return ok;
 }
 
-// Rows a job may have, by the most rows a sequence has: 4, 8 or 16 (8 of 256 dims, whose operands would not fit the registers).
+__device__ __forceinline__ bool kv4_fits(const Kv4Head& h, const Kv4AttnArgs& a) {
+    return kv4_fits(h, a.most_tokens, a.rope, a.shape, a.status, (!h.jobs || h.rows == a.rows) && h.prompt_jobs <= a.prompt_jobs);
+}
+
+// Whether a sequence's (token, query head) rows are jobs of csrc/kv4_prompt.cu.
+inline bool kv4_is_prompt(uint32_t rows, uint32_t dim) { return rows >= 64 && dim != 256; }
+// Rows a job may have else, by the most rows a sequence has: 4, 8 or 16 (8 of 256 dims, whose operands would not fit the registers).
 inline uint32_t kv4_job_rows(uint32_t most, uint32_t dim) { return most <= 4 ? 4 : most <= 8 || dim == 256 ? 8 : 16; }
 // Writes `plan` for one sequence's n tokens from position *pos on (or pos0, where pos is null), its pages in order. A single CTA.
 cudaError_t launch_kv4_plan(const Kv4Plan& plan, const Kv4Shape& shape, uint32_t group, uint32_t n, const int* pos, uint32_t pos0, cudaStream_t st, bool pdl);
@@ -120,6 +128,7 @@ size_t kv4_part_floats(uint32_t dim, int num_sms);
 // `tokens`, `jobs`: how many the host knows of; the kernels take the numbers of plan.head and stride over them.
 cudaError_t launch_kv4_append(const Kv4RowsArgs& a, uint32_t tokens, int num_sms, cudaStream_t st, bool pdl);
 cudaError_t launch_kv4_read(const Kv4RowsArgs& a, uint32_t tokens, int num_sms, cudaStream_t st, bool pdl);
-cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, uint32_t rows, uint32_t jobs, int num_sms, cudaStream_t st, bool pdl);
+cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl);
+cudaError_t launch_kv4_prompt(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl);
 
 }  // namespace alice

@@ -247,7 +247,9 @@ int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4
     a.plan = b->plan; a.shape = c->shape; a.pool = c->pool; a.q = q->p; a.out = out->p; a.q_ld = q_stride; a.out_ld = out_stride;
     a.most_tokens = std::min(room(q, q_stride, dim), room(out, out_stride, dim));
     a.group = b->group; a.scale = scale; a.part = b->part; a.tickets = b->tickets; a.status = e->status;
-    CU(launch_kv4_attention(a, b->now.rows, b->now.jobs, e->num_sms, e->stream, e->pdl));
+    a.rows = b->now.prompt_jobs && !b->now.jobs ? 0 : std::max(b->now.rows, 4u);      // a capture of an empty batch is one of single tokens
+    a.prompt_jobs = b->now.prompt_jobs;
+    CU(launch_kv4_attention(a, e->num_sms, e->stream, e->pdl));
     return ALICE_OK;
 }
 

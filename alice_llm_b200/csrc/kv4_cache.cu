@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const __grid_constan
     pdl_launch_dependents();
     pdl_wait();
     const Kv4Head all = *a.plan.head;
-    if (!kv4_fits(all, a.most_tokens, a.rope, a.shape, 0, a.status)) return;
+    if (!kv4_fits(all, a.most_tokens, a.rope, a.shape, a.status)) return;
     const uint32_t units = W::units(all.tokens, a.heads, a.shape.kv_heads), lane = threadIdx.x & 31, mask = 0xfu << (lane & 28);
     for (uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += gridDim.x * 8) {
         W w(u, a.heads, a.plan, a.shape);
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
     pdl_launch_dependents();
     pdl_wait();
     const Kv4Head all = *a.plan.head;
-    if (!kv4_fits(all, a.most_tokens, a.rope, a.shape, 0, a.status)) return;
+    if (!kv4_fits(all, a.most_tokens, a.rope, a.shape, a.status)) return;
     const uint32_t units = W::units(all.tokens, a.heads, a.shape.kv_heads);
     for (uint32_t u = blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += gridDim.x * 8) {
         W w(u, a.heads, a.plan, a.shape);
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 }
 
 // A model's one sequence: what the host works out for a batch (csrc/kv4_plan.cuh), from the position on the device.
-__global__ void __launch_bounds__(256) kv4_plan_kernel(Kv4Plan plan, Kv4Shape s, uint32_t group, uint32_t rows, uint32_t n, const int* pos, uint32_t pos0) {
+__global__ void __launch_bounds__(256) kv4_plan_kernel(Kv4Plan plan, Kv4Shape s, uint32_t group, uint32_t rows, uint32_t n, const int* pos, uint32_t pos0, bool prompt) {
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t past = pos ? (uint32_t)*pos : pos0, total = n * group, jobs = (total + rows - 1) / rows, tid = threadIdx.x;
@@ -255,9 +255,10 @@ __global__ void __launch_bounds__(256) kv4_plan_kernel(Kv4Plan plan, Kv4Shape s,
     for (uint32_t j = tid; j < jobs; j += blockDim.x) {
         uint32_t before = 0;
         for (uint32_t i = 0; i < j; i++) before += tiles_of(i);
-        const_cast<Kv4Job*>(plan.job)[j] = Kv4Job{0, j * rows, min(rows, total - j * rows), 0, past, before, before + tiles_of(j), 0};
+        const_cast<Kv4Job*>(plan.job)[prompt ? jobs - 1 - j : j] = Kv4Job{0, j * rows, min(rows, total - j * rows), 0, past, before, before + tiles_of(j), 0};
         const_cast<uint32_t*>(plan.job_tile)[j] = before;
-        if (j == jobs - 1) *const_cast<Kv4Head*>(plan.head) = Kv4Head{1, n, jobs, rows, before + tiles_of(j), past + n, (past + n - 1) / s.page_tokens};
+        if (j == jobs - 1)
+            *const_cast<Kv4Head*>(plan.head) = Kv4Head{1, n, prompt ? 0 : jobs, rows, prompt ? 0 : before + tiles_of(j), past + n, (past + n - 1) / s.page_tokens, prompt ? jobs : 0};
     }
 }
 
@@ -267,19 +268,19 @@ cudaError_t launch_kv4_plan(const Kv4Plan& plan, const Kv4Shape& shape, uint32_t
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at; lc.numAttrs = pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&lc, kv4_plan_kernel, plan, shape, group, kv4_job_rows(n * group, shape.dim), n, pos, pos0);
+    const bool prompt = kv4_is_prompt(n * group, shape.dim);      // jobs that see most first
+    return cudaLaunchKernelEx(&lc, kv4_plan_kernel, plan, shape, group, prompt ? KV4_PROMPT_ROWS : kv4_job_rows(n * group, shape.dim), n, pos, pos0, prompt);
 }
 
 namespace {
 template <int NB, class K>
 cudaError_t launch_rows(K kernel, Kv4RowsArgs a, uint32_t tokens, int num_sms, cudaStream_t st, bool pdl) {
-    if (!tokens) return cudaSuccess;
     cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[1];
     // Heads a warp takes one after the other: as many as leave sixteen warps an SM. They share the token's place and angles, but a step of
     // few tokens wants its rows side by side.
     a.heads = Walk<NB>::AT_ONCE;
     while (a.heads < a.shape.kv_heads && a.heads < 8 && Walk<NB>::units(tokens, 2 * a.heads, a.shape.kv_heads) >= 16u * num_sms) a.heads *= 2;
-    const uint32_t ctas = (Walk<NB>::units(tokens, a.heads, a.shape.kv_heads) + 7) / 8, most = (uint32_t)num_sms * 32;
+    const uint32_t ctas = max((Walk<NB>::units(tokens, a.heads, a.shape.kv_heads) + 7) / 8, 1u), most = (uint32_t)num_sms * 32;
     lc.gridDim = dim3(ctas < most ? ctas : most); lc.blockDim = dim3(256); lc.stream = st;
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;

@@ -72,7 +72,9 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t kv_heads, uint3
                           uint32_t table_ld, uint32_t max_pages) {
     uint32_t most = 0, total = 0;
     uint64_t tiles = 0;
-    for (uint32_t s = 0; s < seqs; s++) most = std::max(most, tokens[s] * group);
+    std::vector<Kv4Job> prompts;
+    for (uint32_t s = 0; s < seqs; s++)
+        if (!kv4_is_prompt(tokens[s] * group, dim)) most = std::max(most, tokens[s] * group);
     const uint32_t rows = kv4_job_rows(most, dim);
     h.table.assign((size_t)seqs * max_pages, 0);
     for (uint32_t s = 0; s < seqs; s++) {
@@ -88,6 +90,10 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t kv_heads, uint3
             const uint32_t at = past[s] + i;
             h.token.push_back({t[at / page_tokens] * kv_heads * (page_tokens / KV4_TILE) + at % page_tokens / KV4_TILE, at % KV4_TILE, at, 0});
         }
+        if (kv4_is_prompt(tokens[s] * group, dim)) {
+            for (uint32_t r = 0; r < tokens[s] * group; r += KV4_PROMPT_ROWS) prompts.push_back({s, r, std::min(KV4_PROMPT_ROWS, tokens[s] * group - r), first, past[s], 0, 0, 0});
+            continue;
+        }
         for (uint32_t r = 0; r < tokens[s] * group; r += rows) {
             const uint32_t n = std::min(rows, tokens[s] * group - r), last = past[s] + (r + n - 1) / group + 1, tile0 = (uint32_t)tiles;
             tiles += (last + KV4_TILE - 1) / KV4_TILE;
@@ -95,7 +101,12 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t kv_heads, uint3
             h.job_tile.push_back(tile0);
         }
     }
+    // prompts are started in this order: those that see most first
+    auto keys = [&](const Kv4Job& j) { return j.past + (j.row + j.rows - 1) / group; };
+    std::stable_sort(prompts.begin(), prompts.end(), [&](const Kv4Job& x, const Kv4Job& y) { return keys(x) > keys(y); });
+    h.head.prompt_jobs = (uint32_t)prompts.size();
     h.head.seqs = seqs; h.head.tokens = total; h.head.jobs = (uint32_t)h.job.size(); h.head.rows = rows; h.head.tiles = (uint32_t)tiles;
+    h.job.insert(h.job.end(), prompts.begin(), prompts.end());
     return tiles <= 0x7fffffffull;
 }
 

@@ -1,0 +1,558 @@
+// Attention of many new tokens over the 4-bit cache (csrc/kv4.cuh): 128 (token, query head) rows of a key head against 64 keys at a time, both
+// products on the fifth-generation tensor cores.
+//
+// With a block's step d and minimum m a number is d * (code - 8) + (m + 8 d). Every factor is a pair of half-precision numbers (value and
+// remainder, 22 bits; d * (code - 8) has 15) and a product three of them: value value, value remainder, remainder value. The second part is the same for
+// the 32 dims of a block, so it is a few more columns of the operand, against the sums of a block's queries in one product and with sums of its
+// own in the other. Of 64 keys both are scaled by a power of two into the middle of the range.
+//
+// Sixteen warps: one brings tiles of the pool (bulk copies, a ring of four blocks), two look them over (largest magnitude, NaN), eight turn codes into
+// operands in shared memory (2 instructions a number in half precision; in f32 it was 7, and 667 us instead of 252 with loads of their own for a
+// prompt of 2048 tokens x 32 heads of 128 behind 1021), one issues the products, and four turn scores into weights, a row a lane. Queries and
+// weights lie in tensor memory, the weights where the scores were. Scores of the next keys run while weights are made. A block's sums
+// start from zero and are added to the row's in registers, in f32: over a long chain the tensor cores' sums would be further off than
+// f32's. The reference of the weights moves as in csrc/kv4_attn.cu.
+//
+// A cluster's CTAs share the keys of a job where there are fewer jobs than SMs, and join through distributed shared memory. A key or value
+// that is NaN enters as zero, and rows that see it are NaN: those whose keys reach past the first such position.
+//
+// Every wait is bounded; tensor memory is given back, and products and copies are waited for, on all ways out.
+#include "common.cuh"
+#include "kv4.cuh"
+#include "kv4_query.cuh"
+#include "tc_dev.cuh"
+
+#include <cuda_fp16.h>
+
+namespace alice {
+namespace {
+
+constexpr uint32_t ROWS = KV4_PROMPT_ROWS, KEYS = 64, THREADS = 512;
+constexpr uint32_t RING = 4;                // blocks of keys as they lie in the pool
+constexpr uint32_t SLOTS = 8;               // of a block's scales: RING blocks to come, the operands', the products' and those the rows take up
+constexpr int KERR_ATTN_WAIT = 9;           // a wait inside the tensor-core attention
+constexpr float ROOM = 8.0f, LIFT = 7.0f;   // as in csrc/kv4_attn.cu
+constexpr uint32_t NEVER = 0xffffffffu;
+
+template <int NB>
+struct Lay {
+    // An operand: 64 columns of 64 keys a box; the values' boxes, a box for what codes are less than the numbers, the remainders' boxes.
+    static constexpr uint32_t DIM = 32 * NB, BOXES = DIM / 64, BOX = KEYS * 128, BASE = BOXES * BOX, LEFT = BASE + BOX, OPERAND = LEFT + BASE;
+    static constexpr uint32_t SUMS = 2 * KEYS, QUERIES = SUMS + DIM + 16, TMEM = 512;      // columns: scores and weights, sums (and those of the bases), queries
+    static_assert(QUERIES + DIM + 8 <= TMEM, "");
+    static constexpr uint32_t TILE = kv4_tile_bytes(DIM);
+    static constexpr uint32_t K = 0, V = 2 * OPERAND, TILES = 4 * OPERAND;                 // in shared memory; two operands each
+    static constexpr uint32_t PLACE = V;                                                   // of the queries on their way to tensor memory
+    static_assert(ROWS * DIM * 4 <= 2 * OPERAND, "");
+    struct Smem {
+        alignas(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_empty, done;
+        uint64_t came[RING], seen[RING], taken[RING];                                      // a block of the ring: is there; looked over; free
+        uint32_t tmem;
+        float to[SLOTS][2], from[SLOTS][2];                                                // keys' and values' power of two, and its inverse
+        uint32_t k_nan, v_nan[NB];                                                         // first positions
+        float2 ml[ROWS];
+        float factor[ROWS], q_sum[ROWS][NB];
+    };
+    static constexpr size_t BYTES = sizeof(Smem) + 1024 + TILES + RING * 4 * TILE;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// f16 x f16 -> f32, M x N
+__host__ __device__ constexpr uint32_t f16_desc(uint32_t m, uint32_t n, bool b_rows_k) { return (1u << 4) | ((uint32_t)b_rows_k << 16) | ((n / 8) << 17) | ((m / 16) << 24); }
+__device__ __forceinline__ void pair_of(float a, float b, uint32_t& value, uint32_t& left) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    value = half2_bits(h); left = half2_bits(__floats2half2_rn(a - f.x, b - f.y));
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t there(uint32_t a, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 far_f4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 far_f2(uint32_t a) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t far_u32(uint32_t a) { uint32_t v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory"); return v; }
+// four lanes' or warps' arrivals in one
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+__device__ __forceinline__ void tmem_put8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::
+          "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(float (&v)[8], uint32_t addr) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\ntcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(addr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void sts16(uint32_t a, __half h) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(h)) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// The place of 8 columns (a 16-byte piece) of a row of a box.
+__device__ __forceinline__ uint32_t piece_at(uint32_t row, uint32_t piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+}  // namespace
+
+// grid (key / value heads of jobs, 1, parts of the keys), clusters along z.
+template <int NB>
+__global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttnArgs a) {
+    using L = Lay<NB>;
+    constexpr uint32_t DIM = L::DIM, F4 = DIM / 4;
+    extern __shared__ uint8_t raw[];
+    auto& sh = *reinterpret_cast<typename L::Smem*>(raw);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, part = blockIdx.z, parts = gridDim.z;
+    const uint32_t job = blockIdx.x / a.shape.kv_heads, head = blockIdx.x - job * a.shape.kv_heads;      // all heads of the longest job go first
+    const uint32_t smem = (smem_u32(raw) + (uint32_t)sizeof(typename L::Smem) + 1023u) & ~1023u;
+    auto bar = [](uint64_t& b) { return smem_u32(&b); };
+    if (tid == 0) {
+        mbar_init(bar(sh.q_full), 4);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar(sh.k_full[i]), 8); mbar_init(bar(sh.v_full[i]), 8); mbar_init(bar(sh.k_empty[i]), 1); mbar_init(bar(sh.v_empty[i]), 1);
+            mbar_init(bar(sh.s_full[i]), 1); mbar_init(bar(sh.p_full[i]), 4);
+        }
+        mbar_init(bar(sh.o_full), 1); mbar_init(bar(sh.o_empty), 4);
+        for (uint32_t i = 0; i < RING; i++) { mbar_init(bar(sh.came[i]), 1); mbar_init(bar(sh.seen[i]), 2); mbar_init(bar(sh.taken[i]), 8); }
+        mbar_init(bar(sh.done), 1);
+        mbar_fence_init();
+        fence_proxy_async();
+        sh.k_nan = NEVER;
+        for (int b = 0; b < NB; b++) sh.v_nan[b] = NEVER;
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(L::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sh.tmem;
+    pdl_launch_dependents();      // not before the tensor memory is had: a later kernel's CTA could hold it and wait for this one
+    pdl_wait();
+
+    const Kv4Head hd = *a.plan.head;
+    const bool here = kv4_fits(hd, a) && job < hd.prompt_jobs;
+    Kv4Job jb{};
+    if (here) jb = a.plan.job[hd.jobs + job];
+    const uint32_t keys = here ? jb.past + (jb.row + jb.rows - 1) / a.group + 1 : 0, blocks = (keys + KEYS - 1) / KEYS;
+    const uint32_t b0 = blocks * part / parts, n = blocks * (part + 1) / parts - b0;
+    const long long limit_cycles = WAIT_CYCLE_LIMIT;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
+        // ---- rows: queries, weights, sums ----
+        float sums[DIM], base[NB], l = 0, ref = -INFINITY;      // weighted codes, weighted bases; of weights
+        const uint32_t row = warp * 32 + lane, lane_at = tmem + ((warp * 32) << 16);
+        const uint32_t see = here && row < jb.rows ? jb.past + (jb.row + row) / a.group + 1 : 0;
+        float factor = 0;
+        if (n) {
+            // A row's dims lie 4 a lane to be read, rotated and cut into pairs, and go through shared memory into the lane of the row.
+            constexpr uint32_t PER = DIM / 4, AT_ONCE = 8;
+            const uint32_t place = smem + L::PLACE + warp * 32 * DIM * 4;
+            const uint32_t dim0 = lane % PER * 4;
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < 32 * DIM / 128; c0 += AT_ONCE) {
+                float4 x[AT_ONCE];
+                Turn w[AT_ONCE];
+#pragma unroll
+                for (uint32_t c = 0; c < AT_ONCE; c++) {
+                    const uint32_t own = (c0 + c) * (128 / DIM) + lane / PER, r = jb.row + min(warp * 32 + own, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
+                    x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0);
+                    if (a.rope.dims) w[c] = turn_at(a.rope.table + (size_t)(a.rope.by_token ? at_tok : jb.past + tok) * a.rope.dims, dim0, a.rope);
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < AT_ONCE; c++) {
+                    const uint32_t own = (c0 + c) * (128 / DIM) + lane / PER;
+                    if (a.rope.dims) { const float4 one[1] = {x[c]}; x[c] = rotated4(one, 0, dim0, w[c], a.rope); }
+                    const float f = warp * 32 + own < jb.rows ? a.scale : 0.0f;
+                    const float v[4] = {x[c].x * f, x[c].y * f, x[c].z * f, x[c].w * f};
+                    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+                    for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    int e2 = (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 9;     // the largest into 2^9 .. 2^10
+                    e2 = min(max(e2, -100), 120);
+                    const float down = pow2(-e2);
+                    uint32_t hi[2], lo[2];
+                    pair_of(v[0] * down, v[1] * down, hi[0], lo[0]);
+                    pair_of(v[2] * down, v[3] * down, hi[1], lo[1]);
+                    // 16-byte pieces of a row in an order that lets the rows' lanes read theirs side by side
+                    const uint32_t to = place + own * DIM * 4, piece = dim0 / 8, in = dim0 % 8 * 2;
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + ((piece ^ (own & 7)) << 4) + in), "r"(hi[0]), "r"(hi[1]) : "memory");
+                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + ((piece + DIM / 8 ^ (own & 7)) << 4) + in), "r"(lo[0]), "r"(lo[1]) : "memory");
+                    float sum = (v[0] + v[1] + v[2] + v[3]) * down;
+#pragma unroll
+                    for (uint32_t o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane % 8 == 0) sh.q_sum[warp * 32 + own][dim0 / 32] = sum;
+                    if (dim0 == 0) sh.factor[warp * 32 + own] = pow2(e2) * 1.44269504088896341f;
+                }
+            }
+            __syncwarp();
+            factor = sh.factor[row];
+#pragma unroll
+            for (uint32_t c = 0; c < DIM; c += 16) {
+                uint32_t w[16];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {      // in the order of a word's unpacked codes: 0 4 1 5 2 6 3 7
+                    const uint4 v = lds128(place + lane * DIM * 4 + ((c / 4 + i ^ (lane & 7)) << 4));
+                    w[4 * i] = __byte_perm(v.x, v.z, 0x5410); w[4 * i + 1] = __byte_perm(v.x, v.z, 0x7632);
+                    w[4 * i + 2] = __byte_perm(v.y, v.w, 0x5410); w[4 * i + 3] = __byte_perm(v.y, v.w, 0x7632);
+                }
+                tmem_put16(lane_at + L::QUERIES + c, w);
+            }
+            // sums of a block's queries, against the bases: values, values, remainders
+            uint32_t w[8] = {};
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) pair_of(sh.q_sum[row][b], sh.q_sum[row][b + 1], w[b / 2], w[4 + b / 2]);
+            w[2] = w[0]; w[3] = w[1];
+            tmem_put8(lane_at + L::QUERIES + DIM, w);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(bar(sh.q_full));
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < DIM; c++) sums[c] = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b++) base[b] = 0;
+        const uint32_t all_see = here ? jb.past + jb.row / a.group + 1 : 0;      // keys that every row sees
+        bool ok = true;
+        float carried = 1.0f;          // what the reference's last move makes of the block before
+        // the sums of block j join the row's
+        auto drain = [&](uint32_t j) {
+            ok = warp_wait(bar(sh.o_full), j & 1, limit_cycles);
+            if (!ok) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float f = carried * sh.from[j % SLOTS][1];
+#pragma unroll
+            for (uint32_t c = 0; c < DIM; c += 32) {
+                float v[32];
+                tmem_ld32(v, lane_at + L::SUMS + c);
+#pragma unroll
+                for (int i = 0; i < 32; i++) sums[c + i] = fmaf(v[i], f, sums[c + i]);
+            }
+            float v[8];
+            tmem_ld8(v, lane_at + L::SUMS + DIM);
+#pragma unroll
+            for (int b = 0; b < NB; b++) base[b] = fmaf(v[b] + v[4 + b], f, base[b]);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(bar(sh.o_empty));
+        };
+        for (uint32_t j = 0; j < n; j++) {
+            if (!(ok = warp_wait(bar(sh.s_full[j & 1]), (j >> 1) & 1, limit_cycles))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = lane_at + (j & 1) * KEYS, key0 = (b0 + j) * KEYS;
+            const float f = factor * sh.from[j % SLOTS][0];
+            float s[64];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float v[32];
+                tmem_ld32(v, at + c * 32);
+#pragma unroll
+                for (int i = 0; i < 32; i++) s[c * 32 + i] = v[i];
+            }
+            const bool edge = key0 + KEYS > all_see;
+            const int left = (int)see - (int)key0;       // keys of the block that the row sees
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 64; i++) if (i >= left) s[i] = -INFINITY;
+            }
+            float m = s[0];
+#pragma unroll
+            for (int i = 1; i < 64; i++) m = fmaxf(m, s[i]);
+            carried = 1.0f;
+            if (__any_sync(0xffffffffu, m * f > ref + ROOM)) {
+                const float next = m * f > ref + ROOM ? m * f : ref;
+                carried = next == ref ? 1.0f : ex2(ref - next);
+                ref = next;
+                l *= carried;
+#pragma unroll
+                for (uint32_t c = 0; c < DIM; c++) sums[c] *= carried;
+#pragma unroll
+                for (int b = 0; b < NB; b++) base[b] *= carried;
+            }
+            const float lift = LIFT - ref;
+            float add[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t out[32];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float p0 = ex2(fmaf(s[c * 32 + 2 * i], f, lift)), p1 = ex2(fmaf(s[c * 32 + 2 * i + 1], f, lift));
+                    if (edge) {
+                        if (c * 32 + 2 * i >= left) p0 = 0;
+                        if (c * 32 + 2 * i + 1 >= left) p1 = 0;
+                    }
+                    add[0] += p0; add[1] += p1;
+                    pair_of(p0, p1, out[i], out[16 + i]);
+                }
+                tmem_put32(at + c * 32, out);
+            }
+            l += add[0] + add[1];
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(bar(sh.p_full[j & 1]));
+            if (j) drain(j - 1);
+            if (!ok) break;
+        }
+        carried = 1.0f;
+        if (ok && n) drain(n - 1);
+        if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
+        // the last products are over: the place of their operands is free
+#pragma unroll
+        for (uint32_t i = 0; i < F4; i++) {
+            const uint32_t o = smem + (row * F4 + (i ^ (row & (F4 - 1)))) * 16, c = i / 2 * 8 + i % 2;      // columns in the order of unpacked codes
+            const float x = base[i / 8];
+            asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o), "f"(sums[c] + x), "f"(sums[c + 2] + x), "f"(sums[c + 4] + x), "f"(sums[c + 6] + x) : "memory");
+        }
+        sh.ml[row] = make_float2(ref, l);
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        // ---- operands: a (position, block of 32 dims) a thread ----
+        const uint32_t t = tid - 128, pos = (t >> 5) * 8 + (t & 7), b = t >> 3 & (NB - 1);
+        const bool for_k = NB == 4 || !(t >> 4 & 1), for_v = NB == 4 || !for_k;      // heads of 64: keys or values
+        const uint32_t tile = smem + L::TILES + pos / KV4_TILE * L::TILE, pr = kv4_row(pos % KV4_TILE);
+        const uint32_t k_row = tile + pr * (DIM / 2) + b * 4, v_row = tile + kv4_v_codes(DIM) + pos % KV4_TILE * (DIM / 2) + b * 2;
+        const uint32_t k_dm = tile + kv4_k_scales(DIM) + pr * (4 * NB) + b * 2, v_dm = tile + kv4_v_scales(DIM) + pr * (4 * NB) + b * 2;
+        // The columns that the bases do not fill are zero once and for all: of both operands, those of the warp's own rows.
+        auto clear = [&](uint32_t operand) {
+            sts128(smem + operand + (lane >> 4) * L::OPERAND + L::BASE + piece_at((t >> 5) * 8 + (lane & 7), lane >> 3 & 1), 0, 0, 0, 0);
+            __syncwarp();
+        };
+        // One row's 32 dims: step * (code - 8) as values and remainders (of 15 bits: exact), minimum + 8 * step beside them
+        auto put = [&](uint32_t operand, const uint32_t (&codes)[4], uint32_t d16, uint32_t m16, float to, bool key) {
+            float d = f16_bits_to_f32(d16), m = f16_bits_to_f32(m16);
+            if (m != m) d = m = 0;
+            const __half2 step = __half2half2(__float2half_rn(d * to));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const Codes c = unpack<8>(codes[i]);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const __half2 h = __hmul2(bits_half2(c.v[k]), step);
+                    hi[k] = half2_bits(h); lo[k] = half2_bits(__hfma2(bits_half2(c.v[k]), step, __hneg2(h)));
+                }
+                const uint32_t o = smem + operand + b / 2 * L::BOX + piece_at(pos, (b & 1) * 4 + i);
+                sts128(o, hi[0], hi[1], hi[2], hi[3]);
+                sts128(o + L::LEFT, lo[0], lo[1], lo[2], lo[3]);
+            }
+            const float base = fmaf(8.0f, d, m) * to;
+            const __half h = __float2half_rn(base);
+            const uint32_t o = smem + operand + L::BASE + b * 2;
+            sts16(o + piece_at(pos, 0), h);
+            sts16(o + piece_at(pos, 0) + 8, __float2half_rn(base - __half2float(h)));
+            if (key) sts16(o + piece_at(pos, 1), h);
+        };
+        bool ok = true;
+        clear(L::K);
+        for (uint32_t j = 0; j < n; j++) {
+            const uint32_t st = j & 1, free = ((j >> 1) & 1) ^ 1, at = j % RING * 4 * L::TILE;
+            if (!(ok = warp_wait(bar(sh.came[j % RING]), (j / RING) & 1, limit_cycles) && warp_wait(bar(sh.seen[j % RING]), (j / RING) & 1, limit_cycles))) break;
+            const bool valid = (b0 + j) * KEYS + pos < keys;      // what lies behind the last key is anything
+            uint32_t kc[4], vc[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                kc[i] = lds32(k_row + at + i * (NB * 4));
+                vc[i] = lds16(v_row + at + 2 * i * (NB * 2)) | lds16(v_row + at + (2 * i + 1) * (NB * 2)) << 16;
+            }
+            const uint32_t kd = valid ? lds16(k_dm + at) : 0, km = valid ? lds16(k_dm + at + 2 * NB) : 0, vd = valid ? lds16(v_dm + at) : 0, vm = valid ? lds16(v_dm + at + 2 * NB) : 0;
+            const float k_to = sh.to[j % SLOTS][0], v_to = sh.to[j % SLOTS][1];
+            warp_arrive(bar(sh.taken[j % RING]));
+            if (!(ok = warp_wait(bar(sh.k_empty[st]), free, limit_cycles))) break;
+            if (for_k) put(L::K + st * L::OPERAND, kc, kd, km, k_to, true);
+            fence_proxy_async();
+            warp_arrive(bar(sh.k_full[st]));
+            if (j == 0) {       // the queries have left the place
+                if (!(ok = warp_wait(bar(sh.q_full), 0, limit_cycles))) break;
+                clear(L::V);
+            }
+            if (!(ok = warp_wait(bar(sh.v_empty[st]), free, limit_cycles))) break;
+            if (for_v) put(L::V + st * L::OPERAND, vc, vd, vm, v_to, false);
+            fence_proxy_async();
+            warp_arrive(bar(sh.v_full[st]));
+        }
+        if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        bool ok = true;
+        if (warp == 12 && n) {
+            // ---- products ----
+            ok = warp_wait(bar(sh.q_full), 0, limit_cycles);
+            constexpr uint32_t s_desc = f16_desc(ROWS, KEYS, false), o_desc = f16_desc(ROWS, DIM, true), both_desc = f16_desc(ROWS, DIM + 16, true);
+            auto scores = [&](uint32_t j) {
+                if (!(ok = ok && warp_wait(bar(sh.k_full[j & 1]), (j >> 1) & 1, limit_cycles))) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_lane()) {
+                    const uint32_t kv = smem + L::K + (j & 1) * L::OPERAND, to = tmem + (j & 1) * KEYS, q = tmem + L::QUERIES;
+                    auto keys16 = [&](uint32_t from, uint32_t kk) { return smem_desc(kv + from + kk / 4 * L::BOX) + 2 * (kk % 4); };
+                    // small products first: fewer steps of a sum that is large already
+#pragma unroll
+                    for (uint32_t kk = 0; kk < DIM / 16; kk++) {
+                        mma_f16_ta(to, q + kk * 8, keys16(L::LEFT, kk), s_desc, kk > 0);
+                        mma_f16_ta(to, q + DIM / 2 + kk * 8, keys16(0, kk), s_desc, true);
+                    }
+#pragma unroll
+                    for (uint32_t kk = 0; kk < DIM / 16; kk++) mma_f16_ta(to, q + kk * 8, keys16(0, kk), s_desc, true);
+                    mma_f16_ta(to, q + DIM, smem_desc(kv + L::BASE), s_desc, true);
+                    mma_commit(bar(sh.s_full[j & 1]));
+                    mma_commit(bar(sh.k_empty[j & 1]));
+                }
+                __syncwarp();
+            };
+            scores(0);
+            for (uint32_t j = 0; j < n && ok; j++) {
+                if (j + 1 < n) scores(j + 1);      // where the weights of block j - 1 were, whose products are ahead of these
+                ok = ok && warp_wait(bar(sh.v_full[j & 1]), (j >> 1) & 1, limit_cycles) && warp_wait(bar(sh.p_full[j & 1]), (j >> 1) & 1, limit_cycles) &&
+                     warp_wait(bar(sh.o_empty), (j & 1) ^ 1, limit_cycles);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_lane()) {
+                    const uint32_t va = smem + L::V + (j & 1) * L::OPERAND, pa = tmem + (j & 1) * KEYS, to = tmem + L::SUMS;
+                    auto weights = [&](uint32_t c) { return pa + c / 2 * 32 + c % 2 * 8; };      // of sixteen keys: values; remainders 16 columns on
+                    auto keys16 = [&](uint32_t from, uint32_t c) { return smem_desc_n(va + from + c * 16 * 128, L::BOX); };
+#pragma unroll
+                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c) + 16, keys16(0, c), both_desc, c > 0);
+#pragma unroll
+                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c), keys16(L::LEFT, c), o_desc, true);
+#pragma unroll
+                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c), keys16(0, c), both_desc, true);
+                    mma_commit(bar(sh.o_full));
+                    mma_commit(bar(sh.v_empty[j & 1]));
+                }
+                __syncwarp();
+            }
+            if (elect_lane()) mma_commit(bar(sh.done));
+            __syncwarp();
+            ok = warp_wait(bar(sh.done), 0, limit_cycles) && ok;      // nothing runs any more
+        } else if (warp == 13) {
+            // ---- the ring: a block is four tiles, a lane each ----
+            const uint32_t per_page = a.shape.tiles();
+            uint32_t j = 0;
+            for (; j < n; j++) {
+                const uint32_t tile = (b0 + j) * 4 + lane, s = j % RING;
+                const bool mine = lane < 4 && tile * KV4_TILE < keys;
+                const uint32_t pg = mine ? tile / per_page : 0, page = mine ? a.plan.table[(size_t)jb.seq * a.plan.table_ld + pg] : 0;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * L::TILE;
+                if (!(ok = warp_wait(bar(sh.taken[s]), ((j / RING) & 1) ^ 1, limit_cycles))) break;
+                if (lane == 0) mbar_arrive_expect_tx(bar(sh.came[s]), bytes);
+                __syncwarp();
+                if (mine)
+                    bulk_g2s(smem + L::TILES + (s * 4 + lane) * L::TILE, a.pool + (((size_t)page * a.shape.kv_heads + head) * per_page + (tile - pg * per_page)) * L::TILE, L::TILE, bar(sh.came[s]));
+                __syncwarp();
+            }
+            for (uint32_t i = j < RING ? 0 : j - RING; i < j; i++) ok = warp_wait(bar(sh.came[i % RING]), (i / RING) & 1, limit_cycles) && ok;      // no copy is on its way any more
+        } else if (warp > 13) {
+            // ---- warp 14 the keys', warp 15 the values' largest magnitude in a block and first NaN ----
+            const uint32_t which = warp - 14, scales = smem + L::TILES + (which ? kv4_v_scales(DIM) : kv4_k_scales(DIM));
+            for (uint32_t j = 0; j < n; j++) {
+                const uint32_t s = j % RING;
+                if (!(ok = warp_wait(bar(sh.came[s]), (j / RING) & 1, limit_cycles))) break;
+                float most = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < KEYS * NB / 32; i++) {
+                    const uint32_t at = i * 32 + lane, pos = at / NB, b = at % NB, key = (b0 + j) * KEYS + pos;
+                    const uint32_t o = scales + (s * 4 + pos / KV4_TILE) * L::TILE + kv4_row(pos % KV4_TILE) * (4 * NB) + b * 2;
+                    if (key < keys) {
+                        const float d = f16_bits_to_f32(lds16(o)), m = f16_bits_to_f32(lds16(o + 2 * NB));
+                        if (m != m) atomicMin(which ? &sh.v_nan[b] : &sh.k_nan, key);
+                        else most = fmaxf(most, fmaxf(8.0f * d, fabsf(fmaf(8.0f, d, m))));
+                    }
+                }
+                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));      // below 2^8 with this exponent
+                const int e = top ? 7 - ((int)(top >> 23) - 127) : 0;
+                if (lane == 0) { sh.to[j % SLOTS][which] = pow2(e); sh.from[j % SLOTS][which] = pow2(-e); }
+                warp_arrive(bar(sh.seen[s]));
+            }
+        }
+        if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
+    }
+    // ---- parts of the keys joined, out ----
+    if (parts > 1) cluster_sync(); else __syncthreads();
+    if (here) {
+        const uint32_t rows_each = ROWS / parts;
+        uint32_t k_nan = NEVER;
+        for (uint32_t c = 0; c < parts; c++) k_nan = min(k_nan, far_u32(there(smem_u32(&sh.k_nan), c)));
+        for (uint32_t i = tid; i < rows_each * F4; i += THREADS) {
+            const uint32_t row = part * rows_each + i / F4, f4 = i % F4;
+            if (row >= jb.rows) continue;
+            const uint32_t r = jb.row + row, tok = r / a.group, see = jb.past + tok + 1, mine = (row * F4 + (f4 ^ (row & (F4 - 1)))) * 16;
+            float m = -INFINITY, sum = 0;
+            uint32_t v_nan = NEVER;
+            for (uint32_t c = 0; c < parts; c++) {
+                m = fmaxf(m, far_f2(there(smem_u32(&sh.ml[row]), c)).x);
+                v_nan = min(v_nan, far_u32(there(smem_u32(&sh.v_nan[f4 / 8]), c)));
+            }
+            float4 o = make_float4(0, 0, 0, 0);
+            for (uint32_t c = 0; c < parts; c++) {
+                const float2 ml = far_f2(there(smem_u32(&sh.ml[row]), c));
+                const float4 x = far_f4(there(smem + mine, c));
+                const float f = ml.x == m ? 1.0f : ex2(ml.x - m);
+                sum = fmaf(ml.y, f, sum);
+                o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
+            }
+            const float inv = see > k_nan || see > v_nan ? __uint_as_float(0x7fc00000u) : 1.0f / sum;
+            *reinterpret_cast<float4*>(a.out + (size_t)(jb.first + tok) * a.out_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + 4 * f4) =
+                make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+    }
+    if (parts > 1) cluster_sync();      // what the others read stays until they have
+    if (warp == 12) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::TMEM));
+    }
+}
+
+namespace {
+template <int NB>
+cudaError_t launch(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl) {
+    using L = Lay<NB>;
+    static bool done[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    constexpr size_t smem = L::BYTES > 120 * 1024 ? L::BYTES : 120 * 1024;      // one CTA an SM: each takes all of the tensor memory
+    static_assert(smem <= 227 * 1024, "");
+    if (dev >= 64 || !done[dev]) {
+        err = cudaFuncSetAttribute(kv4_prompt_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+        if (dev < 64) done[dev] = true;
+    }
+    // As many parts of the keys as leave every CTA an SM of its own.
+    uint32_t parts = 1;
+    while (parts < 8 && 2ull * parts * a.prompt_jobs * a.shape.kv_heads <= (uint32_t)num_sms) parts *= 2;
+    cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[2];
+    lc.gridDim = dim3(a.prompt_jobs * a.shape.kv_heads, 1, parts); lc.blockDim = dim3(THREADS); lc.dynamicSmemBytes = smem; lc.stream = st;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = parts;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at; lc.numAttrs = pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&lc, kv4_prompt_kernel<NB>, a);
+}
+}  // namespace
+
+cudaError_t launch_kv4_prompt(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl) {
+    switch (a.shape.dim) {
+        case 64: return launch<2>(a, num_sms, st, pdl);
+        case 128: return launch<4>(a, num_sms, st, pdl);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace alice

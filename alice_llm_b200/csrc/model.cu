@@ -298,8 +298,10 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
             ta.plan = ra.plan; ta.shape = ra.shape; ta.pool = ra.pool; ta.q = m->qkv; ta.q_ld = qkv_stride; ta.out = m->attn_out; ta.out_ld = q_dim;
             ta.most_tokens = m->cap; ta.group = group; ta.scale = 1.0f / std::sqrt((float)c.head_dim); ta.rope = ra.rope; ta.part = m->attn_part; ta.tickets = m->attn_tickets;
             ta.status = m->e->status;
-            const uint32_t rows_of = kv4_job_rows(batch * group, c.head_dim);
-            MCU(launch_kv4_attention(ta, rows_of, (batch * group + rows_of - 1) / rows_of, m->e->num_sms, st, pdl));
+            const bool prompt = kv4_is_prompt(batch * group, c.head_dim);
+            ta.rows = prompt ? 0 : kv4_job_rows(batch * group, c.head_dim);
+            ta.prompt_jobs = prompt ? (batch * group + KV4_PROMPT_ROWS - 1) / KV4_PROMPT_ROWS : 0;
+            MCU(launch_kv4_attention(ta, m->e->num_sms, st, pdl));
             if (o_q8) { launch_quantize_q8k(m->attn_out, q_dim, batch, m->attn_q8, st, pdl, m->cap); MCU(cudaGetLastError()); }
         } else if (batch == 1) {
             aa.nsplit = std::max<uint32_t>(1, std::min(m->nsplit, (uint32_t)m->e->num_sms / shape.num_kv_heads));      // a CTA an SM

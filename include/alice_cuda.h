@@ -203,8 +203,8 @@ int32_t alice_kv4_free(alice_kv4* c);
  * a sequence needs are not looked at, and of a sequence without new tokens none. Sequences may share pages, but none that this step
  * writes into may occur twice among the written ones. Set is not possible in a stream capture; a captured append, read or attention
  * works at its replay on what the batch was set to last, provided that asks for as many rows a job (up to 4, up to 8, or more
- * (token, head) rows of the sequence with most) and fits the buffers and tables of the capture; else it does nothing and alice_sync reports
- * ALICE_E_KERNEL.
+ * (token, query head of a key head) rows of the sequence with most, sequences of 64 and more apart) and no more jobs of 128 rows of those, and
+ * fits the buffers and tables of the capture; else it does nothing and alice_sync reports ALICE_E_KERNEL.
  * alice_kv4_batch_check: the checks of set alone, on the host. */
 typedef struct alice_kv4_batch alice_kv4_batch;
 int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t heads, uint32_t max_seqs, uint32_t max_tokens, uint32_t max_pages,
