@@ -27,9 +27,11 @@
 namespace alice {
 namespace {
 
-constexpr uint32_t ROWS = KV4_PROMPT_ROWS, KEYS = 64, THREADS = 512;
+constexpr uint32_t ROWS = KV4_PROMPT_ROWS, KEYS = 64, THREADS = 640;
+constexpr uint32_t SCORES = 3;              // blocks whose scores or weights are in tensor memory
 constexpr uint32_t RING = 4;                // blocks of keys as they lie in the pool
-constexpr uint32_t SLOTS = 8;               // of a block's scales: RING blocks to come, the operands', the products' and those the rows take up
+constexpr uint32_t GROUP = 4;               // blocks that share powers of two and whose sums add up in tensor memory
+constexpr uint32_t SLOTS = 4;               // groups whose powers of two are there
 constexpr int KERR_ATTN_WAIT = 9;           // a wait inside the tensor-core attention
 constexpr float ROOM = 8.0f, LIFT = 7.0f;   // as in csrc/kv4_attn.cu
 constexpr uint32_t NEVER = 0xffffffffu;
@@ -38,19 +40,20 @@ template <int NB>
 struct Lay {
     // An operand: 64 columns of 64 keys a box; the values' boxes, a box for what codes are less than the numbers, the remainders' boxes.
     static constexpr uint32_t DIM = 32 * NB, BOXES = DIM / 64, BOX = KEYS * 128, BASE = BOXES * BOX, LEFT = BASE + BOX, OPERAND = LEFT + BASE;
-    static constexpr uint32_t SUMS = 2 * KEYS, QUERIES = SUMS + DIM + 16, TMEM = 512;      // columns: scores and weights, sums (and those of the bases), queries
+    static constexpr uint32_t SUMS = SCORES * KEYS, QUERIES = SUMS + DIM + 16, TMEM = 512;      // columns: scores and weights, sums (and those of the bases), queries
     static_assert(QUERIES + DIM + 8 <= TMEM, "");
+    static_assert(SUMS + DIM + 16 == QUERIES, "");
     static constexpr uint32_t TILE = kv4_tile_bytes(DIM);
     static constexpr uint32_t K = 0, V = 2 * OPERAND, TILES = 4 * OPERAND;                 // in shared memory; two operands each
     static constexpr uint32_t PLACE = V;                                                   // of the queries on their way to tensor memory
     static_assert(ROWS * DIM * 4 <= 2 * OPERAND, "");
     struct Smem {
-        alignas(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full, o_empty, done;
-        uint64_t came[RING], seen[RING], taken[RING];                                      // a block of the ring: is there; looked over; free
+        alignas(8) uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[SCORES], p_full[SCORES], p_empty[SCORES], o_empty, done[2];
+        uint64_t came[RING], taken[RING], seen[SLOTS], over[SLOTS];                        // a block of the ring: is there, free; a group: looked over, over
         uint32_t tmem;
         float to[SLOTS][2], from[SLOTS][2];                                                // keys' and values' power of two, and its inverse
         uint32_t k_nan, v_nan[NB];                                                         // first positions
-        float2 ml[ROWS];
+        float ref[ROWS], l[ROWS], top[2][2][ROWS];                                         // largest score of either half of the keys, blocks in turn
         float factor[ROWS], q_sum[ROWS][NB];
     };
     static constexpr size_t BYTES = sizeof(Smem) + 1024 + TILES + RING * 4 * TILE;
@@ -80,12 +83,17 @@ __device__ __forceinline__ float4 far_f4(uint32_t a) {
     asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
     return v;
 }
-__device__ __forceinline__ float2 far_f2(uint32_t a) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint32_t far_u32(uint32_t a) { uint32_t v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory"); return v; }
+__device__ __forceinline__ float far_f32(uint32_t a) { return __uint_as_float(far_u32(a)); }
+// A warp waits where it is blocks ahead: asleep between its questions, which would take issue slots from those that work.
+__device__ __forceinline__ bool warp_rests(uint32_t bar, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        __nanosleep(200);
+        if (__any_sync(0xffffffffu, clock64() - t0 > WAIT_CYCLE_LIMIT)) return false;
+    }
+    return true;
+}
 // four lanes' or warps' arrivals in one
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     __syncwarp();
@@ -123,20 +131,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
     const uint32_t smem = (smem_u32(raw) + (uint32_t)sizeof(typename L::Smem) + 1023u) & ~1023u;
     auto bar = [](uint64_t& b) { return smem_u32(&b); };
     if (tid == 0) {
-        mbar_init(bar(sh.q_full), 4);
+        mbar_init(bar(sh.q_full), 8);
         for (int i = 0; i < 2; i++) {
             mbar_init(bar(sh.k_full[i]), 8); mbar_init(bar(sh.v_full[i]), 8); mbar_init(bar(sh.k_empty[i]), 1); mbar_init(bar(sh.v_empty[i]), 1);
-            mbar_init(bar(sh.s_full[i]), 1); mbar_init(bar(sh.p_full[i]), 4);
+            mbar_init(bar(sh.done[i]), 1);
         }
-        mbar_init(bar(sh.o_full), 1); mbar_init(bar(sh.o_empty), 4);
-        for (uint32_t i = 0; i < RING; i++) { mbar_init(bar(sh.came[i]), 1); mbar_init(bar(sh.seen[i]), 2); mbar_init(bar(sh.taken[i]), 8); }
-        mbar_init(bar(sh.done), 1);
+        for (uint32_t i = 0; i < SCORES; i++) { mbar_init(bar(sh.s_full[i]), 1); mbar_init(bar(sh.p_full[i]), 8); mbar_init(bar(sh.p_empty[i]), 1); }
+        mbar_init(bar(sh.o_empty), 8);
+        for (uint32_t i = 0; i < RING; i++) { mbar_init(bar(sh.came[i]), 1); mbar_init(bar(sh.taken[i]), 8); }
+        for (uint32_t i = 0; i < SLOTS; i++) { mbar_init(bar(sh.seen[i]), 1); mbar_init(bar(sh.over[i]), 8); }
         mbar_fence_init();
         fence_proxy_async();
         sh.k_nan = NEVER;
         for (int b = 0; b < NB; b++) sh.v_nan[b] = NEVER;
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(L::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -153,128 +162,139 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
     if (here) jb = a.plan.job[hd.jobs + job];
     const uint32_t keys = here ? jb.past + (jb.row + jb.rows - 1) / a.group + 1 : 0, blocks = (keys + KEYS - 1) / KEYS;
     const uint32_t b0 = blocks * part / parts, n = blocks * (part + 1) / parts - b0;
-    const long long limit_cycles = WAIT_CYCLE_LIMIT;
 
-    if (warp < 4) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
-        // ---- rows: queries, weights, sums ----
-        float sums[DIM], base[NB], l = 0, ref = -INFINITY;      // weighted codes, weighted bases; of weights
-        const uint32_t row = warp * 32 + lane, lane_at = tmem + ((warp * 32) << 16);
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        // ---- rows, a lane each of two warps: queries, the weights of half of the keys each, the sums of half of the dims ----
+        constexpr uint32_t OWN = DIM / 2;
+        const uint32_t quarter = warp & 3, hf = warp >> 2, row = quarter * 32 + lane, lane_at = tmem + ((quarter * 32) << 16);
         const uint32_t see = here && row < jb.rows ? jb.past + (jb.row + row) / a.group + 1 : 0;
+        auto both = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };      // the warps of a row meet, whatever has become of their waits
         float factor = 0;
         if (n) {
             // A row's dims lie 4 a lane to be read, rotated and cut into pairs, and go through shared memory into the lane of the row.
-            constexpr uint32_t PER = DIM / 4, AT_ONCE = 8;
-            const uint32_t place = smem + L::PLACE + warp * 32 * DIM * 4;
-            const uint32_t dim0 = lane % PER * 4;
-#pragma unroll 1
-            for (uint32_t c0 = 0; c0 < 32 * DIM / 128; c0 += AT_ONCE) {
-                float4 x[AT_ONCE];
-                Turn w[AT_ONCE];
+            constexpr uint32_t PER = DIM / 4, CH = 16 * DIM / 128, AT_ONCE = 4;
+            const uint32_t place = smem + L::PLACE + quarter * 32 * DIM * 4, dim0 = lane % PER * 4;
+            float4 x[CH];
+            uint32_t of[CH];       // row of the rotation table
 #pragma unroll
-                for (uint32_t c = 0; c < AT_ONCE; c++) {
-                    const uint32_t own = (c0 + c) * (128 / DIM) + lane / PER, r = jb.row + min(warp * 32 + own, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
-                    x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0);
-                    if (a.rope.dims) w[c] = turn_at(a.rope.table + (size_t)(a.rope.by_token ? at_tok : jb.past + tok) * a.rope.dims, dim0, a.rope);
-                }
+            for (uint32_t c = 0; c < CH; c++) {
+                const uint32_t own = hf * 16 + c * (128 / DIM) + lane / PER, r = jb.row + min(quarter * 32 + own, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
+                x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0);
+                of[c] = a.rope.by_token ? at_tok : jb.past + tok;
+            }
+            if (a.rope.dims) {
 #pragma unroll
-                for (uint32_t c = 0; c < AT_ONCE; c++) {
-                    const uint32_t own = (c0 + c) * (128 / DIM) + lane / PER;
-                    if (a.rope.dims) { const float4 one[1] = {x[c]}; x[c] = rotated4(one, 0, dim0, w[c], a.rope); }
-                    const float f = warp * 32 + own < jb.rows ? a.scale : 0.0f;
-                    const float v[4] = {x[c].x * f, x[c].y * f, x[c].z * f, x[c].w * f};
-                    float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                for (uint32_t c0 = 0; c0 < CH; c0 += AT_ONCE) {
+                    Turn w[AT_ONCE];
 #pragma unroll
-                    for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    int e2 = (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 9;     // the largest into 2^9 .. 2^10
-                    e2 = min(max(e2, -100), 120);
-                    const float down = pow2(-e2);
-                    uint32_t hi[2], lo[2];
-                    pair_of(v[0] * down, v[1] * down, hi[0], lo[0]);
-                    pair_of(v[2] * down, v[3] * down, hi[1], lo[1]);
-                    // 16-byte pieces of a row in an order that lets the rows' lanes read theirs side by side
-                    const uint32_t to = place + own * DIM * 4, piece = dim0 / 8, in = dim0 % 8 * 2;
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + ((piece ^ (own & 7)) << 4) + in), "r"(hi[0]), "r"(hi[1]) : "memory");
-                    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + ((piece + DIM / 8 ^ (own & 7)) << 4) + in), "r"(lo[0]), "r"(lo[1]) : "memory");
-                    float sum = (v[0] + v[1] + v[2] + v[3]) * down;
+                    for (uint32_t c = 0; c < AT_ONCE; c++) w[c] = turn_at(a.rope.table + (size_t)of[c0 + c] * a.rope.dims, dim0, a.rope);
 #pragma unroll
-                    for (uint32_t o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (lane % 8 == 0) sh.q_sum[warp * 32 + own][dim0 / 32] = sum;
-                    if (dim0 == 0) sh.factor[warp * 32 + own] = pow2(e2) * 1.44269504088896341f;
+                    for (uint32_t c = 0; c < AT_ONCE; c++) { const float4 one[1] = {x[c0 + c]}; x[c0 + c] = rotated4(one, 0, dim0, w[c], a.rope); }
                 }
             }
-            __syncwarp();
+#pragma unroll
+            for (uint32_t c = 0; c < CH; c++) {
+                const uint32_t own = hf * 16 + c * (128 / DIM) + lane / PER;
+                const float f = quarter * 32 + own < jb.rows ? a.scale : 0.0f;
+                const float v[4] = {x[c].x * f, x[c].y * f, x[c].z * f, x[c].w * f};
+                float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+                for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                int e2 = (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 9;     // the largest into 2^9 .. 2^10
+                e2 = min(max(e2, -100), 120);
+                const float down = pow2(-e2);
+                uint32_t hi[2], lo[2];
+                pair_of(v[0] * down, v[1] * down, hi[0], lo[0]);
+                pair_of(v[2] * down, v[3] * down, hi[1], lo[1]);
+                // 16-byte pieces of a row in an order that lets the rows' lanes read theirs side by side
+                const uint32_t to = place + own * DIM * 4, piece = dim0 / 8, in = dim0 % 8 * 2;
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + ((piece ^ (own & 7)) << 4) + in), "r"(hi[0]), "r"(hi[1]) : "memory");
+                asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + ((piece + DIM / 8 ^ (own & 7)) << 4) + in), "r"(lo[0]), "r"(lo[1]) : "memory");
+                float sum = (v[0] + v[1] + v[2] + v[3]) * down;
+#pragma unroll
+                for (uint32_t o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane % 8 == 0) sh.q_sum[quarter * 32 + own][dim0 / 32] = sum;
+                if (dim0 == 0) sh.factor[quarter * 32 + own] = pow2(e2) * 1.44269504088896341f;
+            }
+            both();
             factor = sh.factor[row];
 #pragma unroll
-            for (uint32_t c = 0; c < DIM; c += 16) {
+            for (uint32_t c = 0; c < OWN; c += 16) {       // one warp the values, one the remainders
                 uint32_t w[16];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {      // in the order of a word's unpacked codes: 0 4 1 5 2 6 3 7
-                    const uint4 v = lds128(place + lane * DIM * 4 + ((c / 4 + i ^ (lane & 7)) << 4));
+                    const uint4 v = lds128(place + lane * DIM * 4 + ((hf * OWN / 4 + c / 4 + i ^ (lane & 7)) << 4));
                     w[4 * i] = __byte_perm(v.x, v.z, 0x5410); w[4 * i + 1] = __byte_perm(v.x, v.z, 0x7632);
                     w[4 * i + 2] = __byte_perm(v.y, v.w, 0x5410); w[4 * i + 3] = __byte_perm(v.y, v.w, 0x7632);
                 }
-                tmem_put16(lane_at + L::QUERIES + c, w);
+                tmem_put16(lane_at + L::QUERIES + hf * OWN + c, w);
             }
-            // sums of a block's queries, against the bases: values, values, remainders
-            uint32_t w[8] = {};
+            if (hf == 0) {       // sums of a block's queries, against the bases: values, values, remainders
+                uint32_t w[8] = {};
 #pragma unroll
-            for (int b = 0; b < NB; b += 2) pair_of(sh.q_sum[row][b], sh.q_sum[row][b + 1], w[b / 2], w[4 + b / 2]);
-            w[2] = w[0]; w[3] = w[1];
-            tmem_put8(lane_at + L::QUERIES + DIM, w);
+                for (int b = 0; b < NB; b += 2) pair_of(sh.q_sum[row][b], sh.q_sum[row][b + 1], w[b / 2], w[4 + b / 2]);
+                w[2] = w[0]; w[3] = w[1];
+                tmem_put8(lane_at + L::QUERIES + DIM, w);
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             warp_arrive(bar(sh.q_full));
         }
+        float sums[OWN], base[NB / 2], l = 0, ref = -INFINITY;      // weighted codes, weighted bases; of weights
 #pragma unroll
-        for (uint32_t c = 0; c < DIM; c++) sums[c] = 0;
+        for (uint32_t c = 0; c < OWN; c++) sums[c] = 0;
 #pragma unroll
-        for (int b = 0; b < NB; b++) base[b] = 0;
+        for (int b = 0; b < NB / 2; b++) base[b] = 0;
         const uint32_t all_see = here ? jb.past + jb.row / a.group + 1 : 0;      // keys that every row sees
         bool ok = true;
-        float carried = 1.0f;          // what the reference's last move makes of the block before
-        // the sums of block j join the row's
-        auto drain = [&](uint32_t j) {
-            ok = warp_wait(bar(sh.o_full), j & 1, limit_cycles);
-            if (!ok) return;
+        float carried = 1.0f;          // what the reference's last move makes of the sums before it
+        // the products of the block before the one at (place, turn) are over
+        auto behind = [&](uint32_t place, uint32_t turn) { return warp_wait(bar(sh.p_empty[place ? place - 1 : SCORES - 1]), place ? turn : turn ^ 1); };
+        // the sums of group g join the row's
+        auto drain = [&](uint32_t g) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const float f = carried * sh.from[j % SLOTS][1];
+            const float f = carried * sh.from[g % SLOTS][1];
 #pragma unroll
-            for (uint32_t c = 0; c < DIM; c += 32) {
+            for (uint32_t c = 0; c < OWN; c += 32) {
                 float v[32];
-                tmem_ld32(v, lane_at + L::SUMS + c);
+                tmem_ld32(v, lane_at + L::SUMS + hf * OWN + c);
 #pragma unroll
                 for (int i = 0; i < 32; i++) sums[c + i] = fmaf(v[i], f, sums[c + i]);
             }
-            float v[8];
-            tmem_ld8(v, lane_at + L::SUMS + DIM);
+            uint32_t v[16];
+            tmem_get16(v, lane_at + L::SUMS + DIM);
+            tmem_got16(v);
+            auto sum_of = [&](int b) { return __uint_as_float(v[b]) + __uint_as_float(v[4 + b]); };
 #pragma unroll
-            for (int b = 0; b < NB; b++) base[b] = fmaf(v[b] + v[4 + b], f, base[b]);
+            for (int b = 0; b < NB / 2; b++) base[b] = fmaf(hf ? sum_of(NB / 2 + b) : sum_of(b), f, base[b]);
+            l = fmaf(__uint_as_float(v[8]), carried, l);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            warp_arrive(bar(sh.o_empty));
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(bar(sh.o_empty)); mbar_arrive(bar(sh.over[g % SLOTS])); }
         };
+        uint32_t place_j = 0, turn_j = 0;      // j % SCORES, j / SCORES & 1
         for (uint32_t j = 0; j < n; j++) {
-            if (!(ok = warp_wait(bar(sh.s_full[j & 1]), (j >> 1) & 1, limit_cycles))) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = lane_at + (j & 1) * KEYS, key0 = (b0 + j) * KEYS;
-            const float f = factor * sh.from[j % SLOTS][0];
-            float s[64];
+            ok = ok && warp_wait(bar(sh.s_full[place_j]), turn_j);
+            const uint32_t at = lane_at + place_j * KEYS + hf * 32, key0 = (b0 + j) * KEYS + hf * 32;
+            const float f = factor * sh.from[j / GROUP % SLOTS][0];
+            float s[32];
+            if (ok) {
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tmem_ld32(s, at);
+                const int left = (int)see - (int)key0;       // of these keys the row sees
+                if (key0 + 32 > all_see) {
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                float v[32];
-                tmem_ld32(v, at + c * 32);
+                    for (int i = 0; i < 32; i++) if (i >= left) s[i] = -INFINITY;
+                }
+                float most[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 0; i < 32; i++) s[c * 32 + i] = v[i];
+                for (int i = 4; i < 32; i++) most[i % 4] = fmaxf(most[i % 4], s[i]);
+                sh.top[j & 1][hf][row] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
             }
-            const bool edge = key0 + KEYS > all_see;
-            const int left = (int)see - (int)key0;       // keys of the block that the row sees
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 64; i++) if (i >= left) s[i] = -INFINITY;
-            }
-            float m = s[0];
-#pragma unroll
-            for (int i = 1; i < 64; i++) m = fmaxf(m, s[i]);
+            both();
+            if (!ok) continue;
+            const float m = fmaxf(sh.top[j & 1][0][row], sh.top[j & 1][1][row]);
             carried = 1.0f;
             if (__any_sync(0xffffffffu, m * f > ref + ROOM)) {
                 const float next = m * f > ref + ROOM ? m * f : ref;
@@ -282,60 +302,69 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
                 ref = next;
                 l *= carried;
 #pragma unroll
-                for (uint32_t c = 0; c < DIM; c++) sums[c] *= carried;
+                for (uint32_t c = 0; c < OWN; c++) sums[c] *= carried;
 #pragma unroll
-                for (int b = 0; b < NB; b++) base[b] *= carried;
-            }
-            const float lift = LIFT - ref;
-            float add[2] = {0, 0};
+                for (int b = 0; b < NB / 2; b++) base[b] *= carried;
+                if (j % GROUP) {       // and those in tensor memory
+                    if (!(ok = behind(place_j, turn_j))) continue;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (uint32_t c = 0; c <= OWN; c += 16) {
+                        if (c == OWN && hf) break;
+                        const uint32_t sums_at = lane_at + L::SUMS + (c == OWN ? DIM : hf * OWN + c);
+                        uint32_t v[16];
+                        tmem_get16(v, sums_at);
+                        tmem_got16(v);
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                uint32_t out[32];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float p0 = ex2(fmaf(s[c * 32 + 2 * i], f, lift)), p1 = ex2(fmaf(s[c * 32 + 2 * i + 1], f, lift));
-                    if (edge) {
-                        if (c * 32 + 2 * i >= left) p0 = 0;
-                        if (c * 32 + 2 * i + 1 >= left) p1 = 0;
+                        for (int i = 0; i < 16; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * carried);
+                        tmem_put16(sums_at, v);
                     }
-                    add[0] += p0; add[1] += p1;
-                    pair_of(p0, p1, out[i], out[16 + i]);
                 }
-                tmem_put32(at + c * 32, out);
             }
-            l += add[0] + add[1];
+            const float lift = ref == -INFINITY ? 0.0f : LIFT - ref;      // a row that has seen nothing yet: its scores stay -inf
+            uint32_t out[32];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float p0 = ex2(fmaf(s[2 * i], f, lift)), p1 = ex2(fmaf(s[2 * i + 1], f, lift));
+                pair_of(p0, p1, out[i], out[16 + i]);
+            }
+            tmem_put32(at, out);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            warp_arrive(bar(sh.p_full[j & 1]));
-            if (j) drain(j - 1);
-            if (!ok) break;
+            warp_arrive(bar(sh.p_full[place_j]));
+            if (j && j % GROUP == 0 && (ok = behind(place_j, turn_j))) drain(j / GROUP - 1);
+            if (++place_j == SCORES) { place_j = 0; turn_j ^= 1; }
         }
         carried = 1.0f;
-        if (ok && n) drain(n - 1);
+        if (ok && n && (ok = behind(place_j, turn_j))) drain((n - 1) / GROUP);
         if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
         // the last products are over: the place of their operands is free
 #pragma unroll
-        for (uint32_t i = 0; i < F4; i++) {
-            const uint32_t o = smem + (row * F4 + (i ^ (row & (F4 - 1)))) * 16, c = i / 2 * 8 + i % 2;      // columns in the order of unpacked codes
+        for (uint32_t i = 0; i < F4 / 2; i++) {
+            const uint32_t o = smem + (row * F4 + (hf * (F4 / 2) + i ^ (row & (F4 - 1)))) * 16, c = i / 2 * 8 + i % 2;      // columns in the order of unpacked codes
             const float x = base[i / 8];
             asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(o), "f"(sums[c] + x), "f"(sums[c + 2] + x), "f"(sums[c + 4] + x), "f"(sums[c + 6] + x) : "memory");
         }
-        sh.ml[row] = make_float2(ref, l);
-    } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if (hf == 0) { sh.ref[row] = ref; sh.l[row] = l; }
+    } else if (warp < 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         // ---- operands: a (position, block of 32 dims) a thread ----
-        const uint32_t t = tid - 128, pos = (t >> 5) * 8 + (t & 7), b = t >> 3 & (NB - 1);
+        const uint32_t t = tid - 256, pos = (t >> 5) * 8 + (t & 7), b = t >> 3 & (NB - 1);
         const bool for_k = NB == 4 || !(t >> 4 & 1), for_v = NB == 4 || !for_k;      // heads of 64: keys or values
         const uint32_t tile = smem + L::TILES + pos / KV4_TILE * L::TILE, pr = kv4_row(pos % KV4_TILE);
+        // Words of a row in an order of the row's own, so that neither these loads nor the stores of the operand's pieces meet in a bank: word i ^ k_turn of
+        // keys, where the turn is x -> w x in the field of four (a multiplication that plus x is one again), and i ^ v_turn of values.
+        const uint32_t x = pos & 3, k_turn = (x ^ x >> 1) << 1 & 2 | x >> 1, v_turn = pos >> 1 & 3;
         const uint32_t k_row = tile + pr * (DIM / 2) + b * 4, v_row = tile + kv4_v_codes(DIM) + pos % KV4_TILE * (DIM / 2) + b * 2;
         const uint32_t k_dm = tile + kv4_k_scales(DIM) + pr * (4 * NB) + b * 2, v_dm = tile + kv4_v_scales(DIM) + pr * (4 * NB) + b * 2;
-        // The columns that the bases do not fill are zero once and for all: of both operands, those of the warp's own rows.
-        auto clear = [&](uint32_t operand) {
-            sts128(smem + operand + (lane >> 4) * L::OPERAND + L::BASE + piece_at((t >> 5) * 8 + (lane & 7), lane >> 3 & 1), 0, 0, 0, 0);
+        // The columns that the bases do not fill are zero once and for all (of values the ninth is one: the sum of the weights): of both operands,
+        // those of the warp's own rows.
+        auto clear = [&](uint32_t operand, uint32_t first) {
+            sts128(smem + operand + (lane >> 4) * L::OPERAND + L::BASE + piece_at((t >> 5) * 8 + (lane & 7), lane >> 3 & 1), lane & 8 ? first : 0, 0, 0, 0);
             __syncwarp();
         };
         // One row's 32 dims: step * (code - 8) as values and remainders (of 15 bits: exact), minimum + 8 * step beside them
-        auto put = [&](uint32_t operand, const uint32_t (&codes)[4], uint32_t d16, uint32_t m16, float to, bool key) {
+        auto put = [&](uint32_t operand, const uint32_t (&codes)[4], uint32_t turn, uint32_t d16, uint32_t m16, float to, bool key) {
             float d = f16_bits_to_f32(d16), m = f16_bits_to_f32(m16);
             if (m != m) d = m = 0;
             const __half2 step = __half2half2(__float2half_rn(d * to));
@@ -348,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
                     const __half2 h = __hmul2(bits_half2(c.v[k]), step);
                     hi[k] = half2_bits(h); lo[k] = half2_bits(__hfma2(bits_half2(c.v[k]), step, __hneg2(h)));
                 }
-                const uint32_t o = smem + operand + b / 2 * L::BOX + piece_at(pos, (b & 1) * 4 + i);
+                const uint32_t o = smem + operand + b / 2 * L::BOX + piece_at(pos, (b & 1) * 4 + (i ^ turn));
                 sts128(o, hi[0], hi[1], hi[2], hi[3]);
                 sts128(o + L::LEFT, lo[0], lo[1], lo[2], lo[3]);
             }
@@ -360,87 +389,96 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
             if (key) sts16(o + piece_at(pos, 1), h);
         };
         bool ok = true;
-        clear(L::K);
+        clear(L::K, 0);
         for (uint32_t j = 0; j < n; j++) {
             const uint32_t st = j & 1, free = ((j >> 1) & 1) ^ 1, at = j % RING * 4 * L::TILE;
-            if (!(ok = warp_wait(bar(sh.came[j % RING]), (j / RING) & 1, limit_cycles) && warp_wait(bar(sh.seen[j % RING]), (j / RING) & 1, limit_cycles))) break;
+            const uint32_t slot = j / GROUP % SLOTS;
+            if (j % GROUP == 0 && !(ok = warp_wait(bar(sh.seen[slot]), j / GROUP / SLOTS & 1))) break;
+            if (!(ok = warp_wait(bar(sh.came[j % RING]), (j / RING) & 1))) break;
             const bool valid = (b0 + j) * KEYS + pos < keys;      // what lies behind the last key is anything
             uint32_t kc[4], vc[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                kc[i] = lds32(k_row + at + i * (NB * 4));
-                vc[i] = lds16(v_row + at + 2 * i * (NB * 2)) | lds16(v_row + at + (2 * i + 1) * (NB * 2)) << 16;
+                kc[i] = lds32(k_row + at + (i ^ k_turn) * (NB * 4));
+                vc[i] = lds16(v_row + at + (i ^ v_turn) * (NB * 4)) | lds16(v_row + at + (i ^ v_turn) * (NB * 4) + NB * 2) << 16;
             }
             const uint32_t kd = valid ? lds16(k_dm + at) : 0, km = valid ? lds16(k_dm + at + 2 * NB) : 0, vd = valid ? lds16(v_dm + at) : 0, vm = valid ? lds16(v_dm + at + 2 * NB) : 0;
-            const float k_to = sh.to[j % SLOTS][0], v_to = sh.to[j % SLOTS][1];
+            const float k_to = sh.to[slot][0], v_to = sh.to[slot][1];
             warp_arrive(bar(sh.taken[j % RING]));
-            if (!(ok = warp_wait(bar(sh.k_empty[st]), free, limit_cycles))) break;
-            if (for_k) put(L::K + st * L::OPERAND, kc, kd, km, k_to, true);
+            if (!(ok = warp_wait(bar(sh.k_empty[st]), free))) break;
+            if (for_k) put(L::K + st * L::OPERAND, kc, k_turn, kd, km, k_to, true);
             fence_proxy_async();
             warp_arrive(bar(sh.k_full[st]));
             if (j == 0) {       // the queries have left the place
-                if (!(ok = warp_wait(bar(sh.q_full), 0, limit_cycles))) break;
-                clear(L::V);
+                if (!(ok = warp_wait(bar(sh.q_full), 0))) break;
+                clear(L::V, 0x3c00);
             }
-            if (!(ok = warp_wait(bar(sh.v_empty[st]), free, limit_cycles))) break;
-            if (for_v) put(L::V + st * L::OPERAND, vc, vd, vm, v_to, false);
+            if (!(ok = warp_wait(bar(sh.v_empty[st]), free))) break;
+            if (for_v) put(L::V + st * L::OPERAND, vc, v_turn, vd, vm, v_to, false);
             fence_proxy_async();
             warp_arrive(bar(sh.v_full[st]));
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         bool ok = true;
-        if (warp == 12 && n) {
-            // ---- products ----
-            ok = warp_wait(bar(sh.q_full), 0, limit_cycles);
-            constexpr uint32_t s_desc = f16_desc(ROWS, KEYS, false), o_desc = f16_desc(ROWS, DIM, true), both_desc = f16_desc(ROWS, DIM + 16, true);
-            auto scores = [&](uint32_t j) {
-                if (!(ok = ok && warp_wait(bar(sh.k_full[j & 1]), (j >> 1) & 1, limit_cycles))) return;
+        // ---- products: two warps, so that one's waits are filled with the other's ----
+        if (warp == 16 && n) {
+            ok = warp_wait(bar(sh.q_full), 0);
+            constexpr uint32_t desc = f16_desc(ROWS, KEYS, false);
+            uint32_t place_j = 0, turn_j = 0;
+            for (uint32_t j = 0; j < n && ok; j++) {
+                ok = warp_wait(bar(sh.p_empty[place_j]), turn_j ^ 1) && warp_wait(bar(sh.k_full[j & 1]), (j >> 1) & 1);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_lane()) {
-                    const uint32_t kv = smem + L::K + (j & 1) * L::OPERAND, to = tmem + (j & 1) * KEYS, q = tmem + L::QUERIES;
+                    const uint32_t kv = smem + L::K + (j & 1) * L::OPERAND, to = tmem + place_j * KEYS, q = tmem + L::QUERIES;
                     auto keys16 = [&](uint32_t from, uint32_t kk) { return smem_desc(kv + from + kk / 4 * L::BOX) + 2 * (kk % 4); };
                     // small products first: fewer steps of a sum that is large already
 #pragma unroll
                     for (uint32_t kk = 0; kk < DIM / 16; kk++) {
-                        mma_f16_ta(to, q + kk * 8, keys16(L::LEFT, kk), s_desc, kk > 0);
-                        mma_f16_ta(to, q + DIM / 2 + kk * 8, keys16(0, kk), s_desc, true);
+                        mma_f16_ta(to, q + kk * 8, keys16(L::LEFT, kk), desc, kk > 0);
+                        mma_f16_ta(to, q + DIM / 2 + kk * 8, keys16(0, kk), desc, true);
                     }
 #pragma unroll
-                    for (uint32_t kk = 0; kk < DIM / 16; kk++) mma_f16_ta(to, q + kk * 8, keys16(0, kk), s_desc, true);
-                    mma_f16_ta(to, q + DIM, smem_desc(kv + L::BASE), s_desc, true);
-                    mma_commit(bar(sh.s_full[j & 1]));
+                    for (uint32_t kk = 0; kk < DIM / 16; kk++) mma_f16_ta(to, q + kk * 8, keys16(0, kk), desc, true);
+                    mma_f16_ta(to, q + DIM, smem_desc(kv + L::BASE), desc, true);
+                    mma_commit(bar(sh.s_full[place_j]));
                     mma_commit(bar(sh.k_empty[j & 1]));
                 }
                 __syncwarp();
-            };
-            scores(0);
-            for (uint32_t j = 0; j < n && ok; j++) {
-                if (j + 1 < n) scores(j + 1);      // where the weights of block j - 1 were, whose products are ahead of these
-                ok = ok && warp_wait(bar(sh.v_full[j & 1]), (j >> 1) & 1, limit_cycles) && warp_wait(bar(sh.p_full[j & 1]), (j >> 1) & 1, limit_cycles) &&
-                     warp_wait(bar(sh.o_empty), (j & 1) ^ 1, limit_cycles);
+                if (++place_j == SCORES) { place_j = 0; turn_j ^= 1; }
+            }
+            if (elect_lane()) mma_commit(bar(sh.done[0]));
+            __syncwarp();
+            ok = warp_wait(bar(sh.done[0]), 0) && ok;      // nothing of it runs any more
+        } else if (warp == 19 && n) {
+            constexpr uint32_t desc = f16_desc(ROWS, DIM, true), both_desc = f16_desc(ROWS, DIM + 16, true);
+            uint32_t place_j = 0, turn_j = 0;
+            for (uint32_t j = 0; j < n; j++) {
+                ok = warp_wait(bar(sh.v_full[j & 1]), (j >> 1) & 1) && (j % GROUP || warp_wait(bar(sh.o_empty), (j / GROUP & 1) ^ 1)) && warp_wait(bar(sh.p_full[place_j]), turn_j);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_lane()) {
-                    const uint32_t va = smem + L::V + (j & 1) * L::OPERAND, pa = tmem + (j & 1) * KEYS, to = tmem + L::SUMS;
+                    const uint32_t va = smem + L::V + (j & 1) * L::OPERAND, pa = tmem + place_j * KEYS, to = tmem + L::SUMS;
                     auto weights = [&](uint32_t c) { return pa + c / 2 * 32 + c % 2 * 8; };      // of sixteen keys: values; remainders 16 columns on
                     auto keys16 = [&](uint32_t from, uint32_t c) { return smem_desc_n(va + from + c * 16 * 128, L::BOX); };
 #pragma unroll
-                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c) + 16, keys16(0, c), both_desc, c > 0);
+                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c) + 16, keys16(0, c), both_desc, c > 0 || j % GROUP);
 #pragma unroll
-                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c), keys16(L::LEFT, c), o_desc, true);
+                    for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c), keys16(L::LEFT, c), desc, true);
 #pragma unroll
                     for (uint32_t c = 0; c < KEYS / 16; c++) mma_f16_ta(to, weights(c), keys16(0, c), both_desc, true);
-                    mma_commit(bar(sh.o_full));
                     mma_commit(bar(sh.v_empty[j & 1]));
+                    mma_commit(bar(sh.p_empty[place_j]));
                 }
                 __syncwarp();
+                if (++place_j == SCORES) { place_j = 0; turn_j ^= 1; }
             }
-            if (elect_lane()) mma_commit(bar(sh.done));
+            if (elect_lane()) mma_commit(bar(sh.done[1]));
             __syncwarp();
-            ok = warp_wait(bar(sh.done), 0, limit_cycles) && ok;      // nothing runs any more
-        } else if (warp == 13) {
+            ok = warp_wait(bar(sh.done[1]), 0) && ok;
+        } else if (warp == 17) {
             // ---- the ring: a block is four tiles, a lane each ----
             const uint32_t per_page = a.shape.tiles();
             uint32_t j = 0;
@@ -449,35 +487,57 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
                 const bool mine = lane < 4 && tile * KV4_TILE < keys;
                 const uint32_t pg = mine ? tile / per_page : 0, page = mine ? a.plan.table[(size_t)jb.seq * a.plan.table_ld + pg] : 0;
                 const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, mine)) * L::TILE;
-                if (!(ok = warp_wait(bar(sh.taken[s]), ((j / RING) & 1) ^ 1, limit_cycles))) break;
+                if (!(ok = warp_rests(bar(sh.taken[s]), ((j / RING) & 1) ^ 1))) break;
                 if (lane == 0) mbar_arrive_expect_tx(bar(sh.came[s]), bytes);
                 __syncwarp();
                 if (mine)
                     bulk_g2s(smem + L::TILES + (s * 4 + lane) * L::TILE, a.pool + (((size_t)page * a.shape.kv_heads + head) * per_page + (tile - pg * per_page)) * L::TILE, L::TILE, bar(sh.came[s]));
                 __syncwarp();
             }
-            for (uint32_t i = j < RING ? 0 : j - RING; i < j; i++) ok = warp_wait(bar(sh.came[i % RING]), (i / RING) & 1, limit_cycles) && ok;      // no copy is on its way any more
-        } else if (warp > 13) {
-            // ---- warp 14 the keys', warp 15 the values' largest magnitude in a block and first NaN ----
-            const uint32_t which = warp - 14, scales = smem + L::TILES + (which ? kv4_v_scales(DIM) : kv4_k_scales(DIM));
-            for (uint32_t j = 0; j < n; j++) {
-                const uint32_t s = j % RING;
-                if (!(ok = warp_wait(bar(sh.came[s]), (j / RING) & 1, limit_cycles))) break;
+            for (uint32_t i = j < RING ? 0 : j - RING; i < j; i++) ok = warp_wait(bar(sh.came[i % RING]), (i / RING) & 1) && ok;      // no copy is on its way any more
+        } else if (warp == 18) {
+            // ---- the keys' and the values' largest magnitude in a group, and their first NaN: scales of 64 rows a block from the pool, ahead of the ring ----
+            const uint32_t per_page = a.shape.tiles(), which = lane >> 4, row = lane & 15;      // keys, values; a tile at a time
+            for (uint32_t g = 0; g * GROUP < n; g++) {
+                constexpr uint32_t AT_ONCE = GROUP * 2;
+                const uint32_t tile0 = (b0 + g * GROUP) * 4, tiles = min(GROUP * 4, (keys + KV4_TILE - 1) / KV4_TILE - tile0), end = min(GROUP, n - g * GROUP) * 4;
+                const uint32_t own = tile0 + min(row, tiles - 1), pg = own / per_page;
+                const uint32_t own_at = a.plan.table[(size_t)jb.seq * a.plan.table_ld + pg] * a.shape.kv_heads * per_page + head * per_page + (own - pg * per_page);
                 float most = 0;
+#pragma unroll 1
+                for (uint32_t i0 = 0; i0 < GROUP * 4; i0 += AT_ONCE) {
+                    uint2 d[AT_ONCE], m[AT_ONCE];        // of a row (of 64 dims in one word each)
 #pragma unroll
-                for (uint32_t i = 0; i < KEYS * NB / 32; i++) {
-                    const uint32_t at = i * 32 + lane, pos = at / NB, b = at % NB, key = (b0 + j) * KEYS + pos;
-                    const uint32_t o = scales + (s * 4 + pos / KV4_TILE) * L::TILE + kv4_row(pos % KV4_TILE) * (4 * NB) + b * 2;
-                    if (key < keys) {
-                        const float d = f16_bits_to_f32(lds16(o)), m = f16_bits_to_f32(lds16(o + 2 * NB));
-                        if (m != m) atomicMin(which ? &sh.v_nan[b] : &sh.k_nan, key);
-                        else most = fmaxf(most, fmaxf(8.0f * d, fabsf(fmaf(8.0f, d, m))));
+                    for (uint32_t i = 0; i < AT_ONCE; i++) {
+                        const uint32_t at = __shfl_sync(0xffffffffu, own_at, i0 + i);
+                        const uint8_t* const p = a.pool + (size_t)at * L::TILE + (which ? kv4_v_scales(DIM) : kv4_k_scales(DIM)) + row * (4 * NB);
+                        if constexpr (NB == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); d[i] = make_uint2(v.x, v.y); m[i] = make_uint2(v.z, v.w); }
+                        else { const uint2 v = *reinterpret_cast<const uint2*>(p); d[i] = make_uint2(v.x, 0); m[i] = make_uint2(v.y, 0); }
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < AT_ONCE; i++) {
+                        const uint32_t key = (tile0 + i0 + i) * KV4_TILE + ((row & 8) | (row & 1) << 2 | (row >> 1 & 3));      // the position whose scales lie in this row
+                        if (i0 + i >= min(tiles, end) || key >= keys) continue;
+                        auto two = [&](uint32_t dd, uint32_t mm, int b) {
+                            const float2 df = __half22float2(bits_half2(dd)), mf = __half22float2(bits_half2(mm));
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const float dk = k ? df.y : df.x, mk = k ? mf.y : mf.x;
+                                if (mk != mk) atomicMin(which ? &sh.v_nan[b + k] : &sh.k_nan, key);
+                                else most = fmaxf(most, fmaxf(8.0f * dk, fabsf(fmaf(8.0f, dk, mk))));
+                            }
+                        };
+                        two(d[i].x, m[i].x, 0);
+                        if constexpr (NB == 4) two(d[i].y, m[i].y, 2);
                     }
                 }
-                const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));      // below 2^8 with this exponent
+#pragma unroll
+                for (uint32_t o = 1; o < 16; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const uint32_t top = __float_as_uint(most);      // below 2^8 with this exponent
                 const int e = top ? 7 - ((int)(top >> 23) - 127) : 0;
-                if (lane == 0) { sh.to[j % SLOTS][which] = pow2(e); sh.from[j % SLOTS][which] = pow2(-e); }
-                warp_arrive(bar(sh.seen[s]));
+                if (!(ok = warp_rests(bar(sh.over[g % SLOTS]), (g / SLOTS & 1) ^ 1))) break;
+                if (row == 0) { sh.to[g % SLOTS][which] = pow2(e); sh.from[g % SLOTS][which] = pow2(-e); }
+                warp_arrive(bar(sh.seen[g % SLOTS]));
             }
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
@@ -495,15 +555,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
             float m = -INFINITY, sum = 0;
             uint32_t v_nan = NEVER;
             for (uint32_t c = 0; c < parts; c++) {
-                m = fmaxf(m, far_f2(there(smem_u32(&sh.ml[row]), c)).x);
+                m = fmaxf(m, far_f32(there(smem_u32(&sh.ref[row]), c)));
                 v_nan = min(v_nan, far_u32(there(smem_u32(&sh.v_nan[f4 / 8]), c)));
             }
             float4 o = make_float4(0, 0, 0, 0);
             for (uint32_t c = 0; c < parts; c++) {
-                const float2 ml = far_f2(there(smem_u32(&sh.ml[row]), c));
+                const float ref = far_f32(there(smem_u32(&sh.ref[row]), c)), l = far_f32(there(smem_u32(&sh.l[row]), c));
                 const float4 x = far_f4(there(smem + mine, c));
-                const float f = ml.x == m ? 1.0f : ex2(ml.x - m);
-                sum = fmaf(ml.y, f, sum);
+                const float f = ref == m ? 1.0f : ex2(ref - m);
+                sum = fmaf(l, f, sum);
                 o.x = fmaf(x.x, f, o.x); o.y = fmaf(x.y, f, o.y); o.z = fmaf(x.z, f, o.z); o.w = fmaf(x.w, f, o.w);
             }
             const float inv = see > k_nan || see > v_nan ? __uint_as_float(0x7fc00000u) : 1.0f / sum;
@@ -512,7 +572,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
         }
     }
     if (parts > 1) cluster_sync();      // what the others read stays until they have
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(L::TMEM));
     }
