@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
     if (tid == 0) {
         mbar_init(bar(sh.q_full), 8);
         for (int i = 0; i < 2; i++) {
-            mbar_init(bar(sh.k_full[i]), 8); mbar_init(bar(sh.v_full[i]), 8); mbar_init(bar(sh.k_empty[i]), 1); mbar_init(bar(sh.v_empty[i]), 1);
+            mbar_init(bar(sh.k_full[i]), 4); mbar_init(bar(sh.v_full[i]), 4); mbar_init(bar(sh.k_empty[i]), 1); mbar_init(bar(sh.v_empty[i]), 1);
             mbar_init(bar(sh.done[i]), 1);
         }
         for (uint32_t i = 0; i < SCORES; i++) { mbar_init(bar(sh.s_full[i]), 1); mbar_init(bar(sh.p_full[i]), 8); mbar_init(bar(sh.p_empty[i]), 1); }
@@ -348,75 +348,74 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
         if (hf == 0) { sh.ref[row] = ref; sh.l[row] = l; }
     } else if (warp < 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        // ---- operands: a (position, block of 32 dims) a thread ----
-        const uint32_t t = tid - 256, pos = (t >> 5) * 8 + (t & 7), b = t >> 3 & (NB - 1);
-        const bool for_k = NB == 4 || !(t >> 4 & 1), for_v = NB == 4 || !for_k;      // heads of 64: keys or values
-        const uint32_t tile = smem + L::TILES + pos / KV4_TILE * L::TILE, pr = kv4_row(pos % KV4_TILE);
-        // Words of a row in an order of the row's own, so that neither these loads nor the stores of the operand's pieces meet in a bank: word i ^ k_turn of
-        // keys, where the turn is x -> w x in the field of four (a multiplication that plus x is one again), and i ^ v_turn of values.
-        const uint32_t x = pos & 3, k_turn = (x ^ x >> 1) << 1 & 2 | x >> 1, v_turn = pos >> 1 & 3;
-        const uint32_t k_row = tile + pr * (DIM / 2) + b * 4, v_row = tile + kv4_v_codes(DIM) + pos % KV4_TILE * (DIM / 2) + b * 2;
-        const uint32_t k_dm = tile + kv4_k_scales(DIM) + pr * (4 * NB) + b * 2, v_dm = tile + kv4_v_scales(DIM) + pr * (4 * NB) + b * 2;
-        // The columns that the bases do not fill are zero once and for all (of values the ninth is one: the sum of the weights): of both operands,
-        // those of the warp's own rows.
-        auto clear = [&](uint32_t operand, uint32_t first) {
-            sts128(smem + operand + (lane >> 4) * L::OPERAND + L::BASE + piece_at((t >> 5) * 8 + (lane & 7), lane >> 3 & 1), lane & 8 ? first : 0, 0, 0, 0);
-            __syncwarp();
-        };
-        // One row's 32 dims: step * (code - 8) as values and remainders (of 15 bits: exact), minimum + 8 * step beside them
-        auto put = [&](uint32_t operand, const uint32_t (&codes)[4], uint32_t turn, uint32_t d16, uint32_t m16, float to, bool key) {
-            float d = f16_bits_to_f32(d16), m = f16_bits_to_f32(m16);
-            if (m != m) d = m = 0;
-            const __half2 step = __half2half2(__float2half_rn(d * to));
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const Codes c = unpack<8>(codes[i]);
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const __half2 h = __hmul2(bits_half2(c.v[k]), step);
-                    hi[k] = half2_bits(h); lo[k] = half2_bits(__hfma2(bits_half2(c.v[k]), step, __hneg2(h)));
-                }
-                const uint32_t o = smem + operand + b / 2 * L::BOX + piece_at(pos, (b & 1) * 4 + (i ^ turn));
-                sts128(o, hi[0], hi[1], hi[2], hi[3]);
-                sts128(o + L::LEFT, lo[0], lo[1], lo[2], lo[3]);
-            }
-            const float base = fmaf(8.0f, d, m) * to;
-            const __half h = __float2half_rn(base);
-            const uint32_t o = smem + operand + L::BASE + b * 2;
-            sts16(o + piece_at(pos, 0), h);
-            sts16(o + piece_at(pos, 0) + 8, __float2half_rn(base - __half2float(h)));
-            if (key) sts16(o + piece_at(pos, 1), h);
-        };
+        // ---- operands: four warps keys, four warps values; (position, block of 32 dims) by thread ----
+        constexpr int ITEMS = NB / 2;
+        constexpr uint32_t STEP = KEYS / ITEMS;      // positions from one of a thread's items to the next
+        const bool is_v = warp >= 12;
+        const uint32_t t = tid & 127, pos = t / (8 * NB) * 8 + (t & 7), b = t >> 3 & (NB - 1), pr = kv4_row(pos % KV4_TILE);
+        // Words of a row in an order of the row's own, so that neither these loads nor the stores of the operand's pieces meet in a bank: word i ^ turn, of
+        // keys x -> w x in the field of four (a multiplication that plus x is one again).
+        const uint32_t x = pos & 3, turn = is_v ? pos >> 1 & 3 : (x ^ x >> 1) << 1 & 2 | x >> 1;
+        const uint32_t tile = smem + L::TILES + pos / KV4_TILE * L::TILE, codes_at = tile + (is_v ? kv4_v_codes(DIM) + pos % KV4_TILE * (DIM / 2) + b * 2 : pr * (DIM / 2) + b * 4);
+        const uint32_t scales_at = tile + (is_v ? kv4_v_scales(DIM) : kv4_k_scales(DIM)) + pr * (4 * NB) + b * 2, operands = smem + (is_v ? L::V : L::K);
         bool ok = true;
-        clear(L::K, 0);
-        for (uint32_t j = 0; j < n; j++) {
-            const uint32_t st = j & 1, free = ((j >> 1) & 1) ^ 1, at = j % RING * 4 * L::TILE;
-            const uint32_t slot = j / GROUP % SLOTS;
-            if (j % GROUP == 0 && !(ok = warp_wait(bar(sh.seen[slot]), j / GROUP / SLOTS & 1))) break;
-            if (!(ok = warp_wait(bar(sh.came[j % RING]), (j / RING) & 1))) break;
-            const bool valid = (b0 + j) * KEYS + pos < keys;      // what lies behind the last key is anything
-            uint32_t kc[4], vc[4];
+        if (is_v && n) ok = warp_wait(bar(sh.q_full), 0);      // the queries have left the place
+        // The columns that the bases do not fill are zero once and for all (of values the ninth is one: the sum of the weights): of both operands, the rows that this
+        // warp writes.
+        if (ok) {
+            const uint32_t row = NB == 4 ? t / 32 * 8 + (lane & 7) + (lane >> 3 & 1) * 32 : t / 32 * 16 + (lane & 15);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                kc[i] = lds32(k_row + at + (i ^ k_turn) * (NB * 4));
-                vc[i] = lds16(v_row + at + (i ^ v_turn) * (NB * 4)) | lds16(v_row + at + (i ^ v_turn) * (NB * 4) + NB * 2) << 16;
+            for (int i = 0; i < 2; i++) sts128(operands + i * L::OPERAND + L::BASE + piece_at(row, lane >> 4), is_v && lane >> 4 ? 0x3c00 : 0, 0, 0, 0);
+            __syncwarp();
+        }
+        for (uint32_t j = 0; j < n && ok; j++) {
+            const uint32_t st = j & 1, at = j % RING * 4 * L::TILE, slot = j / GROUP % SLOTS;
+            ok = (j % GROUP || warp_wait(bar(sh.seen[slot]), j / GROUP / SLOTS & 1)) && warp_wait(bar(sh.came[j % RING]), (j / RING) & 1);
+            if (!ok) break;
+            uint32_t codes[ITEMS][4], d16[ITEMS], m16[ITEMS];
+#pragma unroll
+            for (int h = 0; h < ITEMS; h++) {
+                const uint32_t from = codes_at + at + h * (STEP / KV4_TILE) * L::TILE, scales = scales_at + at + h * (STEP / KV4_TILE) * L::TILE;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t o = from + (i ^ turn) * (NB * 4);
+                    codes[h][i] = is_v ? lds16(o) | lds16(o + NB * 2) << 16 : lds32(o);
+                }
+                d16[h] = lds16(scales); m16[h] = lds16(scales + 2 * NB);
+                if ((b0 + j) * KEYS + pos + h * STEP >= keys) d16[h] = m16[h] = 0;      // what lies behind the last key is anything
             }
-            const uint32_t kd = valid ? lds16(k_dm + at) : 0, km = valid ? lds16(k_dm + at + 2 * NB) : 0, vd = valid ? lds16(v_dm + at) : 0, vm = valid ? lds16(v_dm + at + 2 * NB) : 0;
-            const float k_to = sh.to[slot][0], v_to = sh.to[slot][1];
+            const float to = sh.to[slot][is_v];
             warp_arrive(bar(sh.taken[j % RING]));
-            if (!(ok = warp_wait(bar(sh.k_empty[st]), free))) break;
-            if (for_k) put(L::K + st * L::OPERAND, kc, k_turn, kd, km, k_to, true);
-            fence_proxy_async();
-            warp_arrive(bar(sh.k_full[st]));
-            if (j == 0) {       // the queries have left the place
-                if (!(ok = warp_wait(bar(sh.q_full), 0))) break;
-                clear(L::V, 0x3c00);
+            if (!(ok = warp_wait(bar(is_v ? sh.v_empty[st] : sh.k_empty[st]), ((j >> 1) & 1) ^ 1))) break;
+            // A row's 32 dims: step * (code - 8) as values and remainders (of 15 bits: exact), minimum + 8 * step beside them
+#pragma unroll
+            for (int h = 0; h < ITEMS; h++) {
+                float d = f16_bits_to_f32(d16[h]), m = f16_bits_to_f32(m16[h]);
+                if (m != m) d = m = 0;
+                const __half2 step = __half2half2(__float2half_rn(d * to));
+                const uint32_t row = operands + st * L::OPERAND + h * STEP * 128;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const Codes c = unpack<8>(codes[h][i]);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const __half2 v = __hmul2(bits_half2(c.v[k]), step);
+                        hi[k] = half2_bits(v); lo[k] = half2_bits(__hfma2(bits_half2(c.v[k]), step, __hneg2(v)));
+                    }
+                    const uint32_t o = row + b / 2 * L::BOX + piece_at(pos, (b & 1) * 4 + (i ^ turn));
+                    sts128(o, hi[0], hi[1], hi[2], hi[3]);
+                    sts128(o + L::LEFT, lo[0], lo[1], lo[2], lo[3]);
+                }
+                const float base = fmaf(8.0f, d, m) * to;
+                const __half v = __float2half_rn(base);
+                const uint32_t o = row + L::BASE + b * 2;
+                sts16(o + piece_at(pos, 0), v);
+                sts16(o + piece_at(pos, 0) + 8, __float2half_rn(base - __half2float(v)));
+                if (!is_v) sts16(o + piece_at(pos, 1), v);
             }
-            if (!(ok = warp_wait(bar(sh.v_empty[st]), free))) break;
-            if (for_v) put(L::V + st * L::OPERAND, vc, v_turn, vd, vm, v_to, false);
             fence_proxy_async();
-            warp_arrive(bar(sh.v_full[st]));
+            warp_arrive(bar(is_v ? sh.v_full[st] : sh.k_full[st]));
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
     } else {
