@@ -45,7 +45,7 @@ struct Kv4Head {
     uint32_t seqs, tokens, jobs, rows;   // rows: (token, query head) rows of a job
     uint32_t tiles;                      // of all jobs of one key / value head
     uint32_t end, top_page;              // positions of the longest sequence, highest page of a table
-    uint32_t prompt_jobs;                // behind the others, of sequences with many rows
+    uint32_t prompt_jobs;                // ahead of the others, of sequences with many rows
 };
 
 // A job: up to `rows` of Kv4Head consecutive (token, query head of the group) rows of a sequence, against the keys the last of them sees.
@@ -64,8 +64,8 @@ struct alignas(16) Kv4Token {
 struct Kv4Plan {
     const Kv4Head* head;
     const Kv4Token* token;       // [tokens]
-    const Kv4Job* job;           // [jobs]
-    const uint32_t* job_tile;    // [jobs] their tile0 by themselves
+    const Kv4Job* job;           // [prompt_jobs], [jobs]
+    const uint32_t* job_tile;    // [jobs] tile0 of the latter by themselves
     const uint32_t* table;       // [seqs][table_ld] pages
     uint32_t table_ld;
 };
@@ -100,6 +100,7 @@ struct Kv4AttnArgs {
     uint32_t most_tokens;
     uint32_t group;              // query heads a key / value head
     uint32_t rows, prompt_jobs;  // of what is launched: rows of a job, 0: only prompts; prompt jobs at most
+    uint32_t end;                // positions of the longest sequence, as far as the host knows
     float scale;
     Kv4Rope rope;
     float* part;                 // scratch of the joins, kv4_part_floats
@@ -118,8 +119,10 @@ __device__ __forceinline__ bool kv4_fits(const Kv4Head& h, const Kv4AttnArgs& a)
     return kv4_fits(h, a.most_tokens, a.rope, a.shape, a.status, (!h.jobs || h.rows == a.rows) && h.prompt_jobs <= a.prompt_jobs);
 }
 
-// Whether a sequence's (token, query head) rows are jobs of csrc/kv4_prompt.cu.
-inline bool kv4_is_prompt(uint32_t rows, uint32_t dim) { return rows >= 64 && dim != 256; }
+// Whether a sequence's (token, query head) rows are jobs of csrc/kv4_prompt.cu: from where its 128 rows a job, mostly empty, are faster than jobs of 16. Measured
+// either way, us (32 x 8 heads of 128): 16 rows behind 4000 positions 21 against 19, 20 rows 21 / 30, 20 rows behind 100 11 / 17, 32 sequences of 20 rows behind 2000
+// 94 / 104, of 64 rows 97 / 184; heads of 64: 32 sequences of 24 rows behind 2000 37 / 38, 64 of 32 rows behind 100 33 / 25, 16 of 64 rows behind 2000 40 / 109.
+inline bool kv4_is_prompt(uint32_t rows, uint32_t dim) { return dim == 128 ? rows > 16 : dim == 64 && rows > 32; }
 // Rows a job may have else, by the most rows a sequence has: 4, 8 or 16 (8 of 256 dims, whose operands would not fit the registers).
 inline uint32_t kv4_job_rows(uint32_t most, uint32_t dim) { return most <= 4 ? 4 : most <= 8 || dim == 256 ? 8 : 16; }
 // Writes `plan` for one sequence's n tokens from position *pos on (or pos0, where pos is null), its pages in order. A single CTA.
@@ -129,6 +132,6 @@ size_t kv4_part_floats(uint32_t dim, int num_sms);
 cudaError_t launch_kv4_append(const Kv4RowsArgs& a, uint32_t tokens, int num_sms, cudaStream_t st, bool pdl);
 cudaError_t launch_kv4_read(const Kv4RowsArgs& a, uint32_t tokens, int num_sms, cudaStream_t st, bool pdl);
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl);
-cudaError_t launch_kv4_prompt(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl);
+cudaError_t launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st, bool pdl);
 
 }  // namespace alice

@@ -248,7 +248,7 @@ int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4
     a.most_tokens = std::min(room(q, q_stride, dim), room(out, out_stride, dim));
     a.group = b->group; a.scale = scale; a.part = b->part; a.tickets = b->tickets; a.status = e->status;
     a.rows = b->now.prompt_jobs && !b->now.jobs ? 0 : std::max(b->now.rows, 4u);      // a capture of an empty batch is one of single tokens
-    a.prompt_jobs = b->now.prompt_jobs;
+    a.prompt_jobs = b->now.prompt_jobs; a.end = b->now.end;
     CU(launch_kv4_attention(a, e->num_sms, e->stream, e->pdl));
     return ALICE_OK;
 }

@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
     const Kv4Plan& pl = a.plan;
     const Kv4Head hd = *pl.head;
     if (!kv4_fits(hd, a)) return;
+    const Kv4Job* const jobs = pl.job + hd.prompt_jobs;
     // Equal parts for the CTAs, those of one job only (a sequence of few new tokens) at the borders of key heads: no CTA has parts of two
     // of them then, and where a CTA can have all of a head there is nothing to join between CTAs.
     const uint32_t tiles = hd.tiles, total = tiles * a.shape.kv_heads, cta = blockIdx.x;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         uint32_t p_n = 0, p_in = 0;
         auto look = [&]() {          // asks for the page of the next tile,
             if (p_new) {
-                const Kv4Job nj = pl.job[p_job];
+                const Kv4Job nj = jobs[p_job];
                 p_seq = nj.seq; p_tile0 = nj.tile0; p_end = nj.tile1;
                 p_base = 0xffffffffu; p_new = false;
             }
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         uint32_t stage = 0, slot = 0;
         for (uint32_t at = w0; at < w1;) {
             // ---- a job, or this warp's part of it ----
-            const Kv4Job jb = pl.job[job];
+            const Kv4Job jb = jobs[job];
             const uint32_t j0 = head * tiles + jb.tile0, j1 = head * tiles + jb.tile1, end = min(j1, w1);
             const bool has_first = at == j0, has_last = end == j1;
 
@@ -738,8 +739,8 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
         else {
             const uint32_t per = total / grid, more = total - per * grid, wide = more * (per + 1);
             auto cta_of = [&](uint32_t x) { return x < wide ? x / (per + 1) : more + (x - wide) / per; };
-            first_cta[k] = cta_of(of.head * tiles + pl.job[of.job].tile0);
-            count[k] = cta_of(of.head * tiles + pl.job[of.job].tile1 - 1) - first_cta[k] + 1;
+            first_cta[k] = cta_of(of.head * tiles + jobs[of.job].tile0);
+            count[k] = cta_of(of.head * tiles + jobs[of.job].tile1 - 1) - first_cta[k] + 1;
         }
         if (tid == 0 && atomicAdd(a.tickets + first_cta[k], 1u) == count[k] - 1) {
             a.tickets[first_cta[k]] = 0;
@@ -798,7 +799,7 @@ cudaError_t launch(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl)
 
 cudaError_t launch_kv4_attention(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl) {
     if (a.prompt_jobs) {
-        const cudaError_t err = launch_kv4_prompt(a, num_sms, st, pdl);
+        const cudaError_t err = launch_kv4_prompt(a, st, pdl);
         if (err != cudaSuccess || !a.rows) return err;
     }
     switch (a.shape.dim * 100 + a.rows) {

@@ -106,7 +106,7 @@ inline bool kv4_make_plan(Kv4HostPlan& h, uint32_t dim, uint32_t kv_heads, uint3
     std::stable_sort(prompts.begin(), prompts.end(), [&](const Kv4Job& x, const Kv4Job& y) { return keys(x) > keys(y); });
     h.head.prompt_jobs = (uint32_t)prompts.size();
     h.head.seqs = seqs; h.head.tokens = total; h.head.jobs = (uint32_t)h.job.size(); h.head.rows = rows; h.head.tiles = (uint32_t)tiles;
-    h.job.insert(h.job.end(), prompts.begin(), prompts.end());
+    h.job.insert(h.job.begin(), prompts.begin(), prompts.end());
     return tiles <= 0x7fffffffull;
 }
 

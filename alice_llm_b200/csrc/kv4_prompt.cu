@@ -157,9 +157,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
     pdl_wait();
 
     const Kv4Head hd = *a.plan.head;
+    Kv4Job jb = a.plan.job[job];      // beside the head: not more than the plan has room for
     const bool here = kv4_fits(hd, a) && job < hd.prompt_jobs;
-    Kv4Job jb{};
-    if (here) jb = a.plan.job[hd.jobs + job];
+    if (!here) jb = Kv4Job{};
     const uint32_t keys = here ? jb.past + (jb.row + jb.rows - 1) / a.group + 1 : 0, blocks = (keys + KEYS - 1) / KEYS;
     const uint32_t b0 = blocks * part / parts, n = blocks * (part + 1) / parts - b0;
 
@@ -177,18 +177,32 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
             const uint32_t place = smem + L::PLACE + quarter * 32 * DIM * 4, dim0 = lane % PER * 4;
             float4 x[CH];
             uint32_t of[CH];       // row of the rotation table
+            // rows one after the other (of 64 dims every other): token and head without a division each; those behind the last are the last
+            const uint32_t last = jb.row + jb.rows - 1, r0 = min(jb.row + quarter * 32 + hf * 16 + lane / PER, last);
+            uint32_t r = r0, tok = r0 / a.group, of_group = r0 - tok * a.group;
 #pragma unroll
             for (uint32_t c = 0; c < CH; c++) {
-                const uint32_t own = hf * 16 + c * (128 / DIM) + lane / PER, r = jb.row + min(quarter * 32 + own, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
-                x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0);
+                const uint32_t at_tok = jb.first + tok;
+                x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + of_group) * DIM + dim0);
                 of[c] = a.rope.by_token ? at_tok : jb.past + tok;
+#pragma unroll
+                for (uint32_t k = 0; k < 128 / DIM; k++)
+                    if (r < last) {
+                        r++;
+                        if (++of_group == a.group) { of_group = 0; tok++; }
+                    }
             }
             if (a.rope.dims) {
+                const uint32_t half = a.rope.dims / 2, turn_at = dim0 >= a.rope.dims ? 0 : a.rope.neox ? 2 * (dim0 < half ? dim0 : dim0 - half) : dim0;
 #pragma unroll
                 for (uint32_t c0 = 0; c0 < CH; c0 += AT_ONCE) {
-                    Turn w[AT_ONCE];
+                    Turn w[AT_ONCE];       // without a branch between the loads
 #pragma unroll
-                    for (uint32_t c = 0; c < AT_ONCE; c++) w[c] = turn_at(a.rope.table + (size_t)of[c0 + c] * a.rope.dims, dim0, a.rope);
+                    for (uint32_t c = 0; c < AT_ONCE; c++) {
+                        const float* const turn = a.rope.table + (size_t)of[c0 + c] * a.rope.dims + turn_at;
+                        w[c].a = *reinterpret_cast<const float4*>(turn);
+                        w[c].b = *reinterpret_cast<const float4*>(turn + (a.rope.neox ? 4 : 0));
+                    }
 #pragma unroll
                     for (uint32_t c = 0; c < AT_ONCE; c++) { const float4 one[1] = {x[c0 + c]}; x[c0 + c] = rotated4(one, 0, dim0, w[c], a.rope); }
                 }
@@ -199,8 +213,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
                 const float f = quarter * 32 + own < jb.rows ? a.scale : 0.0f;
                 const float v[4] = {x[c].x * f, x[c].y * f, x[c].z * f, x[c].w * f};
                 float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+                if constexpr (PER == 32) top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));      // of numbers without a sign
+                else {
 #pragma unroll
-                for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    for (uint32_t o = 1; o < PER; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                }
                 int e2 = (int)((__float_as_uint(top) >> 23) & 0xff) - 127 - 9;     // the largest into 2^9 .. 2^10
                 e2 = min(max(e2, -100), 120);
                 const float down = pow2(-e2);
@@ -544,12 +561,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
     // ---- parts of the keys joined, out ----
     if (parts > 1) cluster_sync(); else __syncthreads();
     if (here) {
-        const uint32_t rows_each = ROWS / parts;
+        const uint32_t rows_each = (ROWS + parts - 1) / parts;
         uint32_t k_nan = NEVER;
         for (uint32_t c = 0; c < parts; c++) k_nan = min(k_nan, far_u32(there(smem_u32(&sh.k_nan), c)));
         for (uint32_t i = tid; i < rows_each * F4; i += THREADS) {
             const uint32_t row = part * rows_each + i / F4, f4 = i % F4;
-            if (row >= jb.rows) continue;
+            if (row >= jb.rows) break;
             const uint32_t r = jb.row + row, tok = r / a.group, see = jb.past + tok + 1, mine = (row * F4 + (f4 ^ (row & (F4 - 1)))) * 16;
             float m = -INFINITY, sum = 0;
             uint32_t v_nan = NEVER;
@@ -578,38 +595,55 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
 }
 
 namespace {
+// Parts of the keys of a job (a cluster): those with which clusters side by side, one after the other, take the least time. A cluster's start and join are as long as
+// eight blocks of keys (2048 tokens of 32 x 8 heads: 9 of 95 us a CTA).
+uint32_t parts_of(uint32_t clusters, uint32_t blocks, const int (&at_once)[9]) {
+    uint32_t best = 1;
+    uint64_t least = ~0ull;
+    for (uint32_t p = 1; p <= 8 && p <= blocks; p++) {
+        if (at_once[p] <= 0) continue;
+        const uint64_t t = ((uint64_t)clusters + at_once[p] - 1) / at_once[p] * (8 + (blocks + p - 1) / p);
+        if (t < least) { least = t; best = p; }
+    }
+    return best;
+}
+
 template <int NB>
-cudaError_t launch(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl) {
+cudaError_t launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
     using L = Lay<NB>;
-    static bool done[64] = {};
+    static int at_once[64][9] = {};      // clusters of .. CTAs that a device holds; [0]: known
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
+    if (dev >= 64) return cudaErrorInvalidDevice;
     constexpr size_t smem = L::BYTES > 120 * 1024 ? L::BYTES : 120 * 1024;      // one CTA an SM: each takes all of the tensor memory
     static_assert(smem <= 227 * 1024, "");
-    if (dev >= 64 || !done[dev]) {
-        err = cudaFuncSetAttribute(kv4_prompt_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return err;
-        if (dev < 64) done[dev] = true;
-    }
-    // As many parts of the keys as leave every CTA an SM of its own.
-    uint32_t parts = 1;
-    while (parts < 8 && 2ull * parts * a.prompt_jobs * a.shape.kv_heads <= (uint32_t)num_sms) parts *= 2;
     cudaLaunchConfig_t lc = {}; cudaLaunchAttribute at[2];
-    lc.gridDim = dim3(a.prompt_jobs * a.shape.kv_heads, 1, parts); lc.blockDim = dim3(THREADS); lc.dynamicSmemBytes = smem; lc.stream = st;
+    lc.blockDim = dim3(THREADS); lc.dynamicSmemBytes = smem; lc.stream = st;
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = parts;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
-    lc.attrs = at; lc.numAttrs = pdl ? 2 : 1;
+    lc.attrs = at;
+    if (!at_once[dev][0]) {
+        err = cudaFuncSetAttribute(kv4_prompt_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+        for (uint32_t p = 1; p <= 8; p++) {
+            lc.gridDim = dim3(1, 1, p); at[0].val.clusterDim.z = p; lc.numAttrs = 1;
+            if ((err = cudaOccupancyMaxActiveClusters(&at_once[dev][p], kv4_prompt_kernel<NB>, &lc)) != cudaSuccess) return err;
+        }
+        at_once[dev][0] = 1;
+    }
+    const uint32_t parts = parts_of(a.prompt_jobs * a.shape.kv_heads, (a.end + KEYS - 1) / KEYS, at_once[dev]);
+    lc.gridDim = dim3(a.prompt_jobs * a.shape.kv_heads, 1, parts); at[0].val.clusterDim.z = parts; lc.numAttrs = pdl ? 2 : 1;
     return cudaLaunchKernelEx(&lc, kv4_prompt_kernel<NB>, a);
 }
 }  // namespace
 
-cudaError_t launch_kv4_prompt(const Kv4AttnArgs& a, int num_sms, cudaStream_t st, bool pdl) {
+cudaError_t launch_kv4_prompt(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
     switch (a.shape.dim) {
-        case 64: return launch<2>(a, num_sms, st, pdl);
-        case 128: return launch<4>(a, num_sms, st, pdl);
+        case 64: return launch<2>(a, st, pdl);
+        case 128: return launch<4>(a, st, pdl);
         default: return cudaErrorInvalidValue;
     }
 }

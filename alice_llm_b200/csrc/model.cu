@@ -301,6 +301,7 @@ int LlamaModel::step(uint32_t batch, bool greedy_feed, const uint32_t* rows, uin
             const bool prompt = kv4_is_prompt(batch * group, c.head_dim);
             ta.rows = prompt ? 0 : kv4_job_rows(batch * group, c.head_dim);
             ta.prompt_jobs = prompt ? (batch * group + KV4_PROMPT_ROWS - 1) / KV4_PROMPT_ROWS : 0;
+            ta.end = m->pos + batch;
             MCU(launch_kv4_attention(ta, m->e->num_sms, st, pdl));
             if (o_q8) { launch_quantize_q8k(m->attn_out, q_dim, batch, m->attn_q8, st, pdl, m->cap); MCU(cudaGetLastError()); }
         } else if (batch == 1) {

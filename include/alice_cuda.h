@@ -202,9 +202,10 @@ int32_t alice_kv4_free(alice_kv4* c);
  * alice_kv4_batch_set takes tables[s * table_ld + p], the page of positions p * page_tokens onward of sequence s; entries past the pages
  * a sequence needs are not looked at, and of a sequence without new tokens none. Sequences may share pages, but none that this step
  * writes into may occur twice among the written ones. Set is not possible in a stream capture; a captured append, read or attention
- * works at its replay on what the batch was set to last, provided that asks for as many rows a job (up to 4, up to 8, or more
- * (token, query head of a key head) rows of the sequence with most, sequences of 64 and more apart) and no more jobs of 128 rows of those, and
- * fits the buffers and tables of the capture; else it does nothing and alice_sync reports ALICE_E_KERNEL.
+ * works at its replay on what the batch was set to last, provided that asks for no other kernels and fits the buffers and tables of the capture;
+ * else it does nothing and alice_sync reports ALICE_E_KERNEL. Kernels differ by the most (token, query head of a key head) rows a sequence has: up
+ * to 4, up to 8, up to 16 (heads of 64: 32); sequences of more rows (not with heads of 256) go by themselves, 128 rows a job and no more jobs than the
+ * capture had.
  * alice_kv4_batch_check: the checks of set alone, on the host. */
 typedef struct alice_kv4_batch alice_kv4_batch;
 int32_t alice_kv4_batch_create(alice_engine* e, const alice_kv4* cache, uint32_t heads, uint32_t max_seqs, uint32_t max_tokens, uint32_t max_pages,
