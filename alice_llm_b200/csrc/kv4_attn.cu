@@ -15,6 +15,9 @@
 //
 // The running maximum m only moves when a score exceeds it by 2^8, and weighted sums go to f32 sums every 8 tiles: products
 // on tensor cores add up with less than f32 rounding, which over a long chain would add up itself.
+//
+// Bound by issue: a product takes 8 clocks of an SM quarter beside which little else runs, and unpacking as long again. Measured, heads of 128: one token of 64 x 8
+// heads behind 131007 positions (168 MB) 66 us, one each of 64 users with 32 x 8 heads behind up to 4095 57 us.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -72,7 +75,8 @@ struct Cfg {
     static constexpr bool SPLIT = R == 4;
     static constexpr int NT = R == 16 ? 2 : 1;                    // eight-column products
     static constexpr int RT = SPLIT ? 1 : 2 * NT;                 // rows a lane has scores and outputs of
-    static constexpr int TP = R == 16 || NB == 8 ? 1 : 2;                    // tiles taken together: as many as the registers hold
+    static constexpr int TP = R == 16 || NB == 8 ? 1 : 2;         // tiles taken together, as many as the registers hold (131008 positions: 65.6 us, one 68.2)
+    // As many as the registers hold; of 4 rows 12 (56.7 us, 16 58.6 where a CTA has more to merge), of 8 as few as keep the products busy (12 no faster).
     static constexpr int WARPS = NB == 8 ? (R == 4 ? 8 : 6) : R == 4 ? 12 : 8;
     static constexpr uint32_t DIM = 32 * NB, TILE = kv4_tile_bytes(DIM);
     static constexpr int NF = NB * RT;                            // float4 of output a lane has

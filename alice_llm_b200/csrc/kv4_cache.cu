@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const __grid_constan
     }
 }
 
+// And out again: m + d * code, one rounding. Bound by what it writes: 5470 tokens of 8 heads of 128 (45 MB) 17.6 us.
 template <int NB>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4RowsArgs a) {
     using W = Walk<NB>;

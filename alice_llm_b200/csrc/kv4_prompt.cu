@@ -6,12 +6,16 @@
 // the 32 dims of a block, so it is a few more columns of the operand, against the sums of a block's queries in one product and with sums of its
 // own in the other. Of 64 keys both are scaled by a power of two into the middle of the range.
 //
-// Sixteen warps: one brings tiles of the pool (bulk copies, a ring of four blocks), two look them over (largest magnitude, NaN), eight turn codes into
-// operands in shared memory (2 instructions a number in half precision; in f32 it was 7, and 667 us instead of 252 with loads of their own for a
-// prompt of 2048 tokens x 32 heads of 128 behind 1021), one issues the products, and four turn scores into weights, a row a lane. Queries and
-// weights lie in tensor memory, the weights where the scores were. Scores of the next keys run while weights are made. A block's sums
-// start from zero and are added to the row's in registers, in f32: over a long chain the tensor cores' sums would be further off than
-// f32's. The reference of the weights moves as in csrc/kv4_attn.cu.
+// Twenty warps: one brings tiles of the pool (bulk copies, a ring of four blocks), one looks their scales over ahead of that (largest magnitude, NaN), four and four
+// turn codes of keys and of values into operands in shared memory (2 instructions a number in half precision), two issue the products of the one and the other kind,
+// so that one's waits are filled with the other's, and eight turn scores into weights, a row by a lane of two warps: half of a block's keys and half of the
+// dims' sums each. Queries and weights lie in tensor memory, the weights where the scores were; scores of the next blocks run while weights are made. Sums of four
+// blocks add up in tensor memory and go to registers then, in f32: over a long chain the tensor cores' sums would be further off than f32's. The
+// reference of the weights moves as in csrc/kv4_attn.cu; what has been summed up in tensor memory moves with it.
+//
+// Measured: 2048 tokens x 32 heads of 128 (8 of keys) behind 1021 positions 229 us (the products alone: 124 at the measured bf16 rate; jobs of 16 rows on
+// mma.sync: 715). A block takes 2600 clocks, the products 1630 of them: what is lost are the hand-overs from warps to warps. With operand warps that load from the pool
+// themselves it was 667 us, with one warp a row, one for all products and every block's sums to registers 252, with warps that make both operands 6 us more.
 //
 // A cluster's CTAs share the keys of a job where there are fewer jobs than SMs, and join through distributed shared memory. A key or value
 // that is NaN enters as zero, and rows that see it are NaN: those whose keys reach past the first such position.

@@ -118,6 +118,8 @@ __device__ __forceinline__ uint32_t put_in_order(Smem& sh, uint32_t n, uint32_t 
 
 }  // namespace
 
+// Measured: 1 row of 128256 without alternatives 4.8 us, with 5 9.8; 777 of 32000 without 24.0 (4.1 TB/s); 256 of 151643 with 20 56.7 (2.7 TB/s: comparisons with the
+// bound and exponentials share the issue slots; without alternatives the loads bound it).
 template <bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_constant__ LogProbArgs a) {
     __shared__ Smem sh;
