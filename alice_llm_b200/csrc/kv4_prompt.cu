@@ -4,7 +4,7 @@
 // With a block's step d and minimum m a number is d * (code - 8) + (m + 8 d). Every factor is a pair of half-precision numbers (value and
 // remainder, 22 bits; d * (code - 8) has 15) and a product three of them: value value, value remainder, remainder value. The second part is the same for
 // the 32 dims of a block, so it is a few more columns of the operand, against the sums of a block's queries in one product and with sums of its
-// own in the other. Of 64 keys both are scaled by a power of two into the middle of the range.
+// own in the other. Of 256 keys both are scaled by a power of two to below 2^15: what is 2^18 and more below the largest of them has fewer than 22 bits, 2^-40 of that largest.
 //
 // Twenty warps: one brings tiles of the pool (bulk copies, a ring of four blocks), one looks their scales over ahead of that (largest magnitude, NaN), four and four
 // turn codes of keys and of values into operands in shared memory (2 instructions a number in half precision), two issue the products of the one and the other kind,
@@ -553,8 +553,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
                 }
 #pragma unroll
                 for (uint32_t o = 1; o < 16; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const uint32_t top = __float_as_uint(most);      // below 2^8 with this exponent
-                const int e = top ? 7 - ((int)(top >> 23) - 127) : 0;
+                const uint32_t top = __float_as_uint(most);      // below 2^15 with this exponent: codes * step and base are as large at most
+                const int e = top ? 14 - ((int)(top >> 23) - 127) : 0;
                 if (!(ok = warp_rests(bar(sh.over[g % SLOTS]), (g / SLOTS & 1) ^ 1))) break;
                 if (row == 0) { sh.to[g % SLOTS][which] = pow2(e); sh.from[g % SLOTS][which] = pow2(-e); }
                 warp_arrive(bar(sh.seen[g % SLOTS]));
