@@ -17,7 +17,7 @@
 // on tensor cores add up with less than f32 rounding, which over a long chain would add up itself.
 //
 // Bound by issue: a product takes 8 clocks of an SM quarter beside which little else runs, and unpacking as long again. Measured, heads of 128: one token of 64 x 8
-// heads behind 131007 positions (168 MB) 66 us, one each of 64 users with 32 x 8 heads behind up to 4095 57 us.
+// heads behind 131007 positions (168 MB) 64 us, one each of 64 users with 32 x 8 heads behind up to 4095 57 us.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -234,6 +234,9 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
 
         look();
         uint32_t stage = 0, slot = 0;
+        // The first tiles are asked for behind the first queries and their angles, which would wait for all of them otherwise; as few as the ring
+        // holds behind the queries alone (24 short sequences of 64 dims 23.1 us, else 23.4; 131008 positions, where only the code differs, 63.6 and 66.2).
+        const bool few = w1 - w0 <= STAGES;
         for (uint32_t at = w0; at < w1;) {
             // ---- a job, or this warp's part of it ----
             const Kv4Job jb = jobs[job];
@@ -257,6 +260,11 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                     const uint32_t r = jb.row + min(row, jb.rows - 1), tok = r / a.group, at_tok = jb.first + tok;
                     x[c] = *reinterpret_cast<const float4*>(a.q + at_tok * a.q_ld + (size_t)(head * a.group + r - tok * a.group) * DIM + dim0);
                     of[c] = a.rope.by_token ? at_tok : jb.past + tok;
+                }
+                if (at == w0 && few) {
+                    found();
+#pragma unroll
+                    for (int i = 0; i < STAGES; i++) ask(i);
                 }
                 if (a.rope.dims) {
                     constexpr uint32_t PER_ROW = DIM > 128 ? DIM / 128 : 1;
@@ -337,8 +345,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 for (int i = 0; i < RT; i++) factor[i] = aside[(SPLIT ? t : (i >> 1) * 8 + 2 * t + (i & 1)) * (NB + 1) + NB];
                 __syncwarp();
             }
-            // the first tiles are asked for behind the first queries, which would wait for all of them otherwise
-            if (at == w0) {
+            if (at == w0 && !few) {
                 found();
 #pragma unroll
                 for (int i = 0; i < STAGES; i++) ask(i);
