@@ -118,7 +118,7 @@ __device__ __forceinline__ uint32_t put_in_order(Smem& sh, uint32_t n, uint32_t 
 
 }  // namespace
 
-// Measured: 1 row of 128256 without alternatives 4.8 us, with 5 9.8; 777 of 32000 without 24.0 (4.1 TB/s); 256 of 151643 with 20 56.7 (2.7 TB/s: comparisons with the
+// Measured: 1 row of 128256 without alternatives 4.8 us, with 5 9.8; 777 of 32000 without 24.0 (4.1 TB/s); 256 of 151643 with 20 50.2 (3.1 TB/s: comparisons with the
 // bound and exponentials share the issue slots; without alternatives the loads bound it).
 template <bool TOP>
 __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_constant__ LogProbArgs a) {
@@ -132,7 +132,18 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const __grid_cons
     const uint32_t skip = (uint32_t)((reinterpret_cast<uintptr_t>(row) >> 2) & 3);
     const float4* const four = reinterpret_cast<const float4*>(row - skip);
     const uint32_t fours = (uint32_t)(((uint64_t)a.vocab + skip + 3) / 4), per = (fours + parts - 1) / parts, begin = min(part * per, fours), end = min(begin + per, fours);
+    const uint32_t whole0 = skip ? 1 : 0, whole1 = min(end, (uint32_t)(((uint64_t)a.vocab + skip) / 4));      // pieces that are the row's own
     auto load = [&](float (&x)[EACH], uint32_t at) {
+        // Without a look at every piece's ends: 256 rows of 151643 with 20 alternatives 56.6 -> 50.2 us, but 777 of 32000 without any 23.9 -> 25.7 (the code of
+        // both ways stands between the loads and their use).
+        if (TOP && at >= whole0 && at + FOURS * THREADS <= whole1) {
+#pragma unroll
+            for (int i = 0; i < FOURS; i++) {
+                const float4 v = __ldcs(four + at + tid + i * THREADS);
+                x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < FOURS; i++) {
             const uint32_t p = at + i * THREADS + tid;
