@@ -249,6 +249,11 @@ int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4
     a.group = b->group; a.scale = scale; a.part = b->part; a.tickets = b->tickets; a.status = e->status;
     a.rows = b->now.prompt_jobs && !b->now.jobs ? 0 : std::max(b->now.rows, 4u);      // a capture of an empty batch is one of single tokens
     a.prompt_jobs = b->now.prompt_jobs; a.end = b->now.end;
+    if (a.prompt_jobs) {      // a captured call meets longer sequences
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        CU(cudaStreamIsCapturing(e->stream, &capturing));
+        if (capturing != cudaStreamCaptureStatusNone) a.end = (uint32_t)std::min<uint64_t>((uint64_t)b->max_pages * b->shape.page_tokens, 0x7fffffffu);
+    }
     CU(launch_kv4_attention(a, e->num_sms, e->stream, e->pdl));
     return ALICE_OK;
 }

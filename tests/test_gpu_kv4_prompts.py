@@ -258,3 +258,28 @@ def test_two_engines_at_once(engine):
         for x in o:
             assert np.array_equal(s.e.read_f32(x).reshape(s.q.shape), w)
     other.close()
+
+
+def test_a_capture_behind_few_positions_replayed_behind_many(engine):
+    import torch
+    from alice_llm_b200.gpu import GpuEngine
+    e = GpuEngine()
+    stream = torch.cuda.Stream()
+    e.set_stream(stream.cuda_stream)
+    s = Step(e, 20, 1, 128, 64, [3000], [2], seed=1)
+    s.fill()
+    want, tol = s.expect()
+    q, o = e.upload_f32(s.q), e.alloc_f32(s.q.size)
+    s.batch.set([3], [2], s.tables)
+    e.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        e.kv4_attention(s.cache, s.batch, q, o, 128 ** -0.5)
+    s.batch.set(s.past, s.tokens, s.tables)
+    with torch.cuda.stream(stream):
+        graph.replay()
+    got = e.read_f32(o).reshape(s.q.shape)
+    assert (np.abs(got - want) <= tol).all()
+    e.sync()
+    del graph
+    e.close()
