@@ -13,7 +13,7 @@
 // blocks add up in tensor memory and go to registers then, in f32: over a long chain the tensor cores' sums would be further off than f32's. The
 // reference of the weights moves as in csrc/kv4_attn.cu; what has been summed up in tensor memory moves with it.
 //
-// Measured: 2048 tokens x 32 heads of 128 (8 of keys) behind 1021 positions 229 us (the products alone: 124 at the measured bf16 rate; jobs of 16 rows on
+// Measured: 2048 tokens x 32 heads of 128 (8 of keys) behind 1021 positions 227 us (the products alone: 124 at the measured bf16 rate; jobs of 16 rows on
 // mma.sync: 715). A block takes 2600 clocks, the products 1630 of them: what is lost are the hand-overs from warps to warps. With operand warps that load from the pool
 // themselves it was 667 us, with one warp a row, one for all products and every block's sums to registers 252, with warps that make both operands 6 us more.
 //
@@ -32,6 +32,9 @@ namespace alice {
 namespace {
 
 constexpr uint32_t ROWS = KV4_PROMPT_ROWS, KEYS = 64, THREADS = 640;
+// Registers by role; together what the launch has (65536 / 640 threads, down to a multiple of eight).
+constexpr uint32_t REGS_ROWS = 136, REGS_OPERANDS = 72, REGS_REST = 64;
+static_assert(256 * REGS_ROWS + 256 * REGS_OPERANDS + 128 * REGS_REST <= THREADS * (65536 / THREADS / 8 * 8), "");
 constexpr uint32_t SCORES = 3;              // blocks whose scores or weights are in tensor memory
 constexpr uint32_t RING = 4;                // blocks of keys as they lie in the pool
 constexpr uint32_t GROUP = 4;               // blocks that share powers of two and whose sums add up in tensor memory
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
     const uint32_t b0 = blocks * part / parts, n = blocks * (part + 1) / parts - b0;
 
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_ROWS));
         // ---- rows, a lane each of two warps: queries, the weights of half of the keys each, the sums of half of the dims ----
         constexpr uint32_t OWN = DIM / 2;
         const uint32_t quarter = warp & 3, hf = warp >> 2, row = quarter * 32 + lane, lane_at = tmem + ((quarter * 32) << 16);
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
         }
         if (hf == 0) { sh.ref[row] = ref; sh.l[row] = l; }
     } else if (warp < 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OPERANDS));
         // ---- operands: four warps keys, four warps values; (position, block of 32 dims) by thread ----
         constexpr int ITEMS = NB / 2;
         constexpr uint32_t STEP = KEYS / ITEMS;      // positions from one of a thread's items to the next
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
         }
         if (!ok && lane == 0) atomicCAS(a.status, 0, KERR_ATTN_WAIT);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_REST));
         bool ok = true;
         // ---- products: two warps, so that one's waits are filled with the other's ----
         if (warp == 16 && n) {
