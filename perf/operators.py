@@ -170,8 +170,8 @@ def prepare(case, seed):
         wrap = lambda t: e.buf_from_device(t.data_ptr(), t.numel())  # noqa: E731
         cache = e.kv4_cache(pages, page, kh, dim)
         batch = e.kv4_batch(cache, case.get("heads", kh), len(past), sum(tokens), wide)
-        batch.set(past, tokens, table.cpu().numpy())
-        st.update(engine=e, cache=cache, batch=batch, rope_buf=wrap(st["rope"]) if rot else None)
+        # a server keeps lengths and page tables on the host; each step hands them over
+        st.update(engine=e, cache=cache, batch=batch, step=(past, tokens, table.cpu().numpy().astype(np.uint32)), rope_buf=wrap(st["rope"]) if rot else None)
         if case["kind"] == "append":
             st["k_out"], st["v_out"] = torch.empty_like(st["k"]), torch.empty_like(st["v"])
             st.update({n + "_buf": wrap(st[n]) for n in ("k", "v", "k_out", "v_out")})
@@ -300,6 +300,8 @@ def run(st):
     c = st["case"]
     if not own:
         return {"append": _plain_append, "attend": _plain_attend, "log_probs": _plain_log_probs}[c["kind"]](st)
+    elif "step" in st:
+        st["batch"].set(*st["step"])      # the places of its tokens and its jobs are worked out within the step
     e = st["engine"]
     if c["kind"] == "append":
         e.kv4_append(st["cache"], st["batch"], st["k_buf"], st["v_buf"], rope=st["rope_buf"], rot_dims=c["rot"], neox=c["neox"])
