@@ -7,6 +7,7 @@
 #include "abi_internal.cuh"
 #include "kv4.cuh"
 #include "kv4_plan.cuh"
+#include "rows.cuh"
 
 using namespace alice;
 
@@ -37,15 +38,12 @@ namespace {
 
 bool apart(const alice_buf* x, size_t nx, const alice_buf* y, size_t ny) { return x->p + nx <= y->p || y->p + ny <= x->p; }
 
-// floats that `tokens` rows of `dim` span, `ld` apart
-size_t span(uint32_t tokens, size_t ld, size_t dim) { return tokens ? (size_t)(tokens - 1) * ld + dim : 0; }
-
 int check_rows(const char* who, const char* name, const alice_engine* e, const alice_buf* x, uint32_t tokens, size_t& ld, size_t dim) {
     if (!x) return alice_fail(ALICE_E_INVALID, "%s: %s is null", who, name);
     if (x->e != e) return alice_fail(ALICE_E_INVALID, "%s: %s belongs to another engine", who, name);
     if (ld == 0) ld = dim;
     if (ld < dim || ld % 4 || ld > ((size_t)1 << 40)) return alice_fail(ALICE_E_SHAPE, "%s: rows of %s are %zu floats apart; a multiple of 4 of at least %zu is wanted", who, name, ld, dim);
-    if (x->len < span(tokens, ld, dim)) return alice_fail(ALICE_E_SHAPE, "%s: %s holds %zu floats, %u rows need %zu", who, name, x->len, tokens, span(tokens, ld, dim));
+    if (!rows_fit(x->len, tokens, ld, dim)) return alice_fail(ALICE_E_SHAPE, "%s: %s holds %zu floats, less than %u rows of %zu that are %zu apart", who, name, x->len, tokens, dim, ld);
     return ALICE_OK;
 }
 
@@ -223,7 +221,7 @@ int32_t alice_kv4_read(alice_engine* e, const alice_kv4* c, const alice_kv4_batc
     if (rc) return rc;
     const size_t dim = (size_t)c->shape.kv_heads * c->shape.dim;
     // side by side in one buffer is fine; the same floats for both are not
-    if (k->p == v->p || (a.k_ld == dim && a.v_ld == dim && !apart(k, span(b->now.tokens, dim, dim), v, span(b->now.tokens, dim, dim))))
+    if (k->p == v->p || (a.k_ld == dim && a.v_ld == dim && !apart(k, rows_span(b->now.tokens, dim, dim), v, rows_span(b->now.tokens, dim, dim))))
         return alice_fail(ALICE_E_INVALID, "%s: k and v share memory", who);
     CU(launch_kv4_read(a, b->now.tokens, e->num_sms, e->stream, e->pdl));
     return ALICE_OK;
@@ -241,7 +239,7 @@ int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4
     if ((rc = check_rope(who, e, rope, rot_dims, neox, c->shape.dim, b->now.end, a.rope))) return rc;
     if (!std::isfinite(scale)) return alice_fail(ALICE_E_INVALID, "%s: scale is not finite", who);
     // a query is read by several CTAs, at any time before the last of its output is there
-    if (!apart(q, span(b->now.tokens, q_stride, dim), out, span(b->now.tokens, out_stride, dim)))
+    if (!apart(q, rows_span(b->now.tokens, q_stride, dim), out, rows_span(b->now.tokens, out_stride, dim)))
         return alice_fail(ALICE_E_INVALID, "%s: q and out share memory", who);
     CU(cudaSetDevice(e->device));
     a.plan = b->plan; a.shape = c->shape; a.pool = c->pool; a.q = q->p; a.out = out->p; a.q_ld = q_stride; a.out_ld = out_stride;

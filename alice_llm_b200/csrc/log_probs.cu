@@ -17,6 +17,7 @@
 #include "abi_internal.cuh"
 #include "common.cuh"
 #include "log_probs.cuh"
+#include "rows.cuh"
 
 namespace alice {
 
@@ -423,7 +424,9 @@ extern "C" int32_t alice_log_probs(alice_engine* e, const alice_buf* logits, uin
     if (top > LOGP_MAX_TOP || top > vocab) return alice_fail(ALICE_E_SHAPE, "%s: %u alternatives; up to %u, and no more than %u tokens", who, top, LOGP_MAX_TOP, vocab);
     if (!targets && (log_probs || rank)) return alice_fail(ALICE_E_INVALID, "%s: log probabilities and ranks need targets", who);
     if (top && (!top_ids || !top_log_probs)) return alice_fail(ALICE_E_INVALID, "%s: %u alternatives without room for them", who, top);
-    const size_t read = rows ? (rows - 1) * stride + vocab : 0, tops = (size_t)rows * top;
+    if (!rows_fit(logits->len, rows, stride, vocab))
+        return alice_fail(ALICE_E_SHAPE, "%s: logits holds %zu words, less than %u rows of %u that are %zu apart", who, logits->len, rows, vocab, stride);
+    const size_t read = rows_span(rows, stride, vocab), tops = (size_t)rows * top;
     struct { const char* name; const alice_buf* b; size_t n; bool out; } all[] = {
         {"logits", logits, read, false}, {"targets", targets, rows, false}, {"log_probs", log_probs, rows, true}, {"entropy", entropy, rows, true},
         {"rank", rank, rows, true}, {"top_ids", top ? top_ids : nullptr, tops, true}, {"top_log_probs", top ? top_log_probs : nullptr, tops, true}};
