@@ -6,15 +6,18 @@
 // with d, m a block's step and minimum. Codes of values enter less 8 (and m is m + 8 d), so that the two parts of a sum over many keys do
 // not cancel; unpacking two of them is a mask and an exact addition in half precision. (Masked bits alone are exact operands too, as numbers
 // below 2^-14, but the products of those lose bits in the sum: results were 4e-5 to 4e-4 off.) The other operand, q or p * d, is a pair of half-precision
-// numbers (value and remainder, 22 bits), scaled by powers of two into the middle of their range.
+// numbers (value and remainder, 22 bits), scaled by powers of two into the middle of their range: queries by one for a row, steps by one for each block of 32 dims.
 // With up to 4 rows the pair fills two columns of the product, with more they are two products.
 //
 // All tiles of all jobs and key heads are one row of work that is cut into equal parts, a CTA an SM and again among its warps, so batches of any
 // lengths are even. A warp streams its tiles through a ring of its own (cp.async); rows that several warps or CTAs had a part in are
 // joined in shared memory, then by the CTA that is the last to bring its part.
 //
-// The running maximum m only moves when a score exceeds it by 2^8, and weighted sums go to f32 sums every 8 tiles: products
-// on tensor cores add up with less than f32 rounding, which over a long chain would add up itself.
+// Weighted sums go to f32 sums every 8 tiles: products on tensor cores add up with less than f32 rounding, which over a long chain would add up itself. What is
+// added up until then is of one magnitude: its weights have a reference of their own, the largest score of its first tiles, which moves when a score exceeds it by 2^8 or
+// when the next sums begin with all of a row's 2^8 below it, and its steps lie within 2^8 (what is heavier, or larger, and comes elsewhere takes no bits from it). Where the
+// steps of two tiles side by side lie further apart (a block of zeros with a weight counts too), these tiles' products are made in f32 by the ordinary pipes. One power of two
+// for all blocks and for all that came before, as it was at first, took 64 us instead of 67 for the row below, and with values 2^20 apart was 1 to 5 % off.
 //
 // Bound by issue: a product takes 8 clocks of an SM quarter beside which little else runs, and unpacking as long again. Measured, heads of 128: one token of 64 x 8
 // heads behind 131007 positions (168 MB) 64 us, one each of 64 users with 32 x 8 heads behind up to 4095 57 us.
@@ -377,9 +380,18 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int c = 0; c < 4; c++) acc[n][b][u][c] = 0;
-            uint32_t dtop = 0;                  // exponent field of the largest step so far, in the top bits of a half
-            __half2 dscale = __float2half2_rn(0.0f);      // 2^z on steps
-            float dback = 0;                    // 2^-z
+            // Steps in acc, by block of dims (two to a register): as half-precision bits less `least_d` they have none of the bits `too_far`; 2^(14 - e) that they are
+            // multiplied by, e in bytes of last_e.
+            constexpr uint32_t NO_STEP = 0xe001e001u, FAR = 0xe000e000u;      // 0 and nothing else
+            uint32_t least_d[NB / 2], too_far[NB / 2], last_e[NB / 4 ? NB / 4 : 1];
+            __half2 dscale[NB / 2];
+            auto no_steps = [&]() {
+#pragma unroll
+                for (int b = 0; b < NB / 2; b++) { least_d[b] = NO_STEP; too_far[b] = FAR; dscale[b] = __float2half2_rn(0.0f); }
+            };
+            no_steps();
+#pragma unroll
+            for (int b = 0; b < NB; b += 4) last_e[b / 4] = 0;
             uint32_t held = 0;                  // tiles in acc
             bool begun = false;                 // sums are in shared memory
             float4* const mine = &sh.sum[warp][slot][0][lane];
@@ -388,17 +400,19 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
             auto flush = [&]() {
 #pragma unroll
                 for (int i = 0; i < RT; i++) {
-                    const float c = mref[i] == ref[i] ? 1.0f : ex2(mref[i] - ref[i]);
+                    const float top = fmaxf(mref[i], ref[i]), c = mref[i] == top ? 1.0f : ex2(mref[i] - top), f = ref[i] == top ? 1.0f : ex2(ref[i] - top);
                     float s = l[i];
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                    lsum[i] = begun ? lsum[i] * c + s : s;
-                    l[i] = 0; mref[i] = ref[i];
+                    lsum[i] = fmaf(lsum[i], c, s * f);
+                    l[i] = 0; mref[i] = top;
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
+                        const float back = pow2((int)(last_e[b / 4] >> 8 * (b % 4) & 31) - 14) * f;
                         float am = accm[i][b];
 #pragma unroll
                         for (int o = 4; o < 32; o <<= 1) am += __shfl_xor_sync(0xffffffffu, am, o);
+                        am *= f;
                         accm[i][b] = 0;
                         float v[4];
 #pragma unroll
@@ -407,7 +421,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                             if (SPLIT) { v[2 * u] = x[0] + x[1]; v[2 * u + 1] = x[2] + x[3]; x[0] = x[1] = x[2] = x[3] = 0; }
                             else { v[2 * u] = x[i & 1]; v[2 * u + 1] = x[2 + (i & 1)]; x[i & 1] = x[2 + (i & 1)] = 0; }
                         }
-                        float4 o = make_float4(fmaf(v[0], dback, am), fmaf(v[1], dback, am), fmaf(v[2], dback, am), fmaf(v[3], dback, am));
+                        float4 o = make_float4(fmaf(v[0], back, am), fmaf(v[1], back, am), fmaf(v[2], back, am), fmaf(v[3], back, am));
                         float4* to = mine + (i * NB + b) * 32;
                         if (begun) { const float4 p = *to; o.x = fmaf(p.x, c, o.x); o.y = fmaf(p.y, c, o.y); o.z = fmaf(p.z, c, o.z); o.w = fmaf(p.w, c, o.w); }
                         *to = o;
@@ -506,6 +520,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                 auto weights = [&](auto edge_t) {
                     constexpr bool edge = decltype(edge_t)::value;       // some row does not see all of the tiles
                     bool move = false;
+                    uint32_t beyond[NB / 2] = {}, too = 0;
 #pragma unroll
                     for (int i = 0; i < RT; i++) {
                         float m = -INFINITY;
@@ -517,27 +532,72 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                                 m = fmaxf(m, s[x][i][k]);
                             }
                         move |= m * factor[i] > ref[i] + ROOM;
+                        if (held == 0) move |= !(__ballot_sync(0xffffffffu, m * factor[i] > ref[i] - ROOM) & 0x11111111u << t);      // none of the row's
                     }
-                    __half2 both = __float2half2_rn(0.0f);
 #pragma unroll
                     for (int x = 0; x < TP; x++)
 #pragma unroll
-                        for (int b = 0; b < NB / 2; b++) {
-                            if (edge) {      // keys that no row sees: whatever lies there has no part
-                                if (key + 16 * x >= far) va[x].w[b] = 0;
-                                if (key + 16 * x + 8 >= far) vb[x].w[b] = 0;
+                        for (int k = 0; k < 2; k++)
+#pragma unroll
+                            for (int b = 0; b < NB / 2; b++) {
+                                uint32_t& d = (k ? vb : va)[x].w[b];
+                                const bool none = edge && key + 16 * x + 8 * k >= far;      // keys that no row sees: whatever lies there has no part
+                                if (none) d = 0;
+                                beyond[b] |= none ? 0 : d - least_d[b];                     // a borrow is of a half that is too far itself
                             }
-                            both = __hmax2(both, __hmax2(bits_half2(va[x].w[b]), bits_half2(vb[x].w[b])));
+                    uint32_t hi[NB / 2], lo[NB / 2];
+                    auto outside = [&]() {
+                        bool out = false;
+#pragma unroll
+                        for (int b = 0; b < NB / 2; b++) out |= __vcmpgtu2(hi[b], __vadd2(least_d[b], ~too_far[b])) || __vcmplts2(lo[b], least_d[b]);
+                        return out;
+                    };
+#pragma unroll
+                    for (int b = 0; b < NB / 2; b++) too |= beyond[b] & too_far[b];
+                    bool again = __any_sync(0xffffffffu, move || too);
+                    if (again) {
+                        // The largest steps and the least; a step of 0 has the size of its minimum, and a NaN's is above all.
+#pragma unroll
+                        for (int b = 0; b < NB / 2; b++) {
+                            hi[b] = 0; lo[b] = 0x7fff7fffu;
+#pragma unroll
+                            for (int x = 0; x < TP; x++)
+#pragma unroll
+                                for (int k = 0; k < 2; k++) {
+                                    if (edge && key + 16 * x + 8 * k >= far) continue;
+                                    const uint32_t d = (k ? vb : va)[x].w[b], m = (k ? vb : va)[x].w[NB / 2 + b] & 0x7fff7fffu;
+                                    hi[b] = __vmaxu2(hi[b], d); lo[b] = __vminu2(lo[b], d | m & __vcmpeq2(d, 0));
+                                }
                         }
-                    const uint32_t dmax = max(half2_bits(both) & 0x7c00u, half2_bits(both) >> 16 & 0x7c00u);
-                    move |= dmax > dtop;
-                    if (__any_sync(0xffffffffu, move)) {
+                        again = __any_sync(0xffffffffu, move || outside());
+                    }
+                    if (again) {
                         if (held) flush();
-                        dtop = __reduce_max_sync(0xffffffffu, max(dmax, dtop));
-                        // steps to below 1, so that with weights up to 2^15 their products stay in range
-                        const int z = 14 - (int)(dtop >> 10);
-                        dscale = __half2half2(__ushort_as_half(z >= -14 ? (z + 15) << 10 : 0x400 >> (-14 - z)));
-                        dback = pow2(-z);
+#pragma unroll
+                        for (int b = 0; b < NB / 2; b++) {
+                            uint32_t top = hi[b], scale = 0;
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            // To below 1, with weights up to 2^15 then in range: by 2^(14 - e), e the exponent field that is the last within. That of the largest step is the
+                            // one before, and the least is 2^-8 then. Of the steps below 2^-8 (fields 0 to 6) the least is 2^-4 to 2^-6 of the largest, and 2^-11 then.
+                            least_d[b] = too_far[b] = 0;
+                            if (b % 2 == 0) last_e[b / 2] = 0;
+#pragma unroll
+                            for (int k = 0; k < 2; k++) {
+                                const uint32_t d = top >> 16 * k & 0xffff, field = d >> 10;
+                                uint32_t e, least, far_bits = 0xe000;
+                                if (!d) { e = 0; least = NO_STEP & 0xffff; }
+                                else if (field >= 7) { e = field + 1; least = (field - 6) << 10; }
+                                else if (field >= 4) { e = 8; least = 512; }
+                                else if (field >= 2) { e = 4; least = 64; far_bits = 0xf000; }
+                                else if (field == 1) { e = 2; least = 16; far_bits = 0xf800; }
+                                else { e = 1; least = max(d >> 6, 1u); far_bits = 0xfc00; }
+                                least_d[b] |= least << 16 * k; too_far[b] |= far_bits << 16 * k;
+                                last_e[b / 2] |= e << 8 * (2 * (b % 2) + k);
+                                scale |= (e <= 28 ? (29 - e) << 10 : 0x400u >> (e - 28)) << 16 * k;
+                            }
+                            dscale[b] = bits_half2(scale);
+                        }
 #pragma unroll
                         for (int i = 0; i < RT; i++) {
                             float m = fmaxf(s[0][i][0], s[0][i][1]);
@@ -545,7 +605,44 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                             for (int x = 1; x < TP; x++) m = fmaxf(m, fmaxf(s[x][i][0], s[x][i][1]));
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                            ref[i] = fmaxf(ref[i], m * factor[i]);
+                            if (m > -INFINITY) ref[i] = m * factor[i];
+                        }
+                        if (__any_sync(0xffffffffu, outside())) {
+                            // Steps too far apart for one power of two: in f32 and without products, by the lanes that have the sums of these rows and dims.
+                            flush();                 // nothing is held: the sums' reference
+                            const uint32_t steps = kv4_v_scales(DIM), v_codes = kv4_v_codes(DIM) + g * (2 * NB);
+                            float f[RT];
+#pragma unroll
+                            for (int i = 0; i < RT; i++) f[i] = ref[i] == mref[i] ? 1.0f : ex2(ref[i] - mref[i]);
+#pragma unroll
+                            for (int x = 0; x < TP; x++)
+#pragma unroll
+                                for (uint32_t k = 0; k < 2; k++) {
+                                    float p[RT];
+#pragma unroll
+                                    for (int i = 0; i < RT; i++) p[i] = edge && key + 16 * x + 8 * k >= limit[i] ? 0.0f : f[i] * ex2(fmaf(s[x][i][k], factor[i], LIFT - ref[i]));
+#pragma unroll 1
+                                    for (uint32_t b = 0; b < NB; b++) {
+                                        float4 o[RT];
+#pragma unroll
+                                        for (int i = 0; i < RT; i++) o[i] = mine[(i * NB + b) * 32];
+#pragma unroll 1
+                                        for (uint32_t j = 0; j < 8 && key0 + 16 * x + 8 * k + j < far; j++) {
+                                            const uint32_t row = kv4_row(j), codes = lds16(base[x] + v_codes + (8 * k + j) * (DIM / 2) + b * 2);
+                                            const float d = f16_bits_to_f32(lds16(base[x] + steps + (8 * k + row) * (4 * NB) + b * 2));
+#pragma unroll
+                                            for (int i = 0; i < RT; i++) {
+                                                const float w = __shfl_sync(0xffffffffu, p[i], 4 * row + t) * d;
+                                                o[i].x = fmaf(w, (float)(codes & 15) - 8.0f, o[i].x); o[i].y = fmaf(w, (float)(codes >> 4 & 15) - 8.0f, o[i].y);
+                                                o[i].z = fmaf(w, (float)(codes >> 8 & 15) - 8.0f, o[i].z); o[i].w = fmaf(w, (float)(codes >> 12) - 8.0f, o[i].w);
+                                            }
+                                        }
+#pragma unroll
+                                        for (int i = 0; i < RT; i++) mine[(i * NB + b) * 32] = o[i];
+                                    }
+                                }
+                            no_steps();              // no part in the products
+                            held = FLUSH;            // and what comes next is by itself
                         }
                     }
 #pragma unroll
@@ -595,7 +692,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         }
 #pragma unroll
                     for (int b2 = 0; b2 < NB / 2; b2++) {
-                        const __half2 d2[2] = {__hmul2(bits_half2(va[x].w[b2]), dscale), __hmul2(bits_half2(vb[x].w[b2]), dscale)};
+                        const __half2 d2[2] = {__hmul2(bits_half2(va[x].w[b2]), dscale[b2]), __hmul2(bits_half2(vb[x].w[b2]), dscale[b2])};
                         Codes ca[2], cb[2];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
