@@ -36,8 +36,6 @@ struct alice_kv4_batch {
 
 namespace {
 
-bool apart(const alice_buf* x, size_t nx, const alice_buf* y, size_t ny) { return x->p + nx <= y->p || y->p + ny <= x->p; }
-
 int check_rows(const char* who, const char* name, const alice_engine* e, const alice_buf* x, uint32_t tokens, size_t& ld, size_t dim) {
     if (!x) return alice_fail(ALICE_E_INVALID, "%s: %s is null", who, name);
     if (x->e != e) return alice_fail(ALICE_E_INVALID, "%s: %s belongs to another engine", who, name);
@@ -220,9 +218,9 @@ int32_t alice_kv4_read(alice_engine* e, const alice_kv4* c, const alice_kv4_batc
     const int rc = rows_call(who, e, c, b, k, k_stride, v, v_stride, a);
     if (rc) return rc;
     const size_t dim = (size_t)c->shape.kv_heads * c->shape.dim;
-    // side by side in one buffer is fine; the same floats for both are not
-    if (k->p == v->p || (a.k_ld == dim && a.v_ld == dim && !apart(k, rows_span(b->now.tokens, dim, dim), v, rows_span(b->now.tokens, dim, dim))))
-        return alice_fail(ALICE_E_INVALID, "%s: k and v share memory", who);
+    // side by side in one buffer is fine; the same floats for both are not, nor at a replay with more tokens
+    a.most_tokens = (uint32_t)rows_apart(a.k, a.k_ld, dim, a.v, a.v_ld, dim, a.most_tokens);
+    if (k->p == v->p || a.most_tokens < b->now.tokens) return alice_fail(ALICE_E_INVALID, "%s: k and v share memory", who);
     CU(launch_kv4_read(a, b->now.tokens, e->num_sms, e->stream, e->pdl));
     return ALICE_OK;
 }
@@ -238,12 +236,11 @@ int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4
     if ((rc = check_rows(who, "out", e, out, b->now.tokens, out_stride, dim))) return rc;
     if ((rc = check_rope(who, e, rope, rot_dims, neox, c->shape.dim, b->now.end, a.rope))) return rc;
     if (!std::isfinite(scale)) return alice_fail(ALICE_E_INVALID, "%s: scale is not finite", who);
-    // a query is read by several CTAs, at any time before the last of its output is there
-    if (!apart(q, rows_span(b->now.tokens, q_stride, dim), out, rows_span(b->now.tokens, out_stride, dim)))
-        return alice_fail(ALICE_E_INVALID, "%s: q and out share memory", who);
+    // a query is read by several CTAs, at any time before the last of its output is there; a replay may have more tokens
+    a.most_tokens = (uint32_t)rows_apart(q->p, q_stride, dim, out->p, out_stride, dim, std::min(room(q, q_stride, dim), room(out, out_stride, dim)));
+    if (q->p == out->p || a.most_tokens < b->now.tokens) return alice_fail(ALICE_E_INVALID, "%s: q and out share memory", who);
     CU(cudaSetDevice(e->device));
     a.plan = b->plan; a.shape = c->shape; a.pool = c->pool; a.q = q->p; a.out = out->p; a.q_ld = q_stride; a.out_ld = out_stride;
-    a.most_tokens = std::min(room(q, q_stride, dim), room(out, out_stride, dim));
     a.group = b->group; a.scale = scale; a.part = b->part; a.tickets = b->tickets; a.status = e->status;
     a.rows = b->now.prompt_jobs && !b->now.jobs ? 0 : std::max(b->now.rows, 4u);      // a capture of an empty batch is one of single tokens
     a.prompt_jobs = b->now.prompt_jobs; a.end = b->now.end;

@@ -220,12 +220,12 @@ int32_t alice_kv4_batch_check(uint32_t pages, uint32_t page_tokens, uint32_t max
  * (j, j + rot_dims / 2) (apply_rope_neox, :5367). KvCache::append, src/llama3.rs:4773. */
 int32_t alice_kv4_append(alice_engine* e, alice_kv4* c, const alice_kv4_batch* b, const alice_buf* k, size_t k_stride, const alice_buf* v, size_t v_stride,
                          const alice_buf* rope, uint32_t rot_dims, uint32_t neox);
-/* The values the cache holds for the batch's new tokens. */
+/* The values the cache holds for the batch's new tokens. Rows of k and v may not meet (side by side in wider rows is fine), nor at a replay with more tokens. */
 int32_t alice_kv4_read(alice_engine* e, const alice_kv4* c, const alice_kv4_batch* b, alice_buf* k, size_t k_stride, alice_buf* v, size_t v_stride);
 /* out = softmax(scale * q K^T) V for the batch's new tokens over the cache: token i of a sequence sees its past + i + 1 first positions,
  * which have been appended. heads * head_dim floats a row; consecutive query heads share a key / value head; q is rotated on the way
  * like the keys. Rows of out behind the last token stay as they were. A NaN that a row sees makes it NaN, what it does not see has no
- * part in it. gqa_attention, src/llama3.rs:5431. */
+ * part in it. Rows of q and out may not meet either. gqa_attention, src/llama3.rs:5431. */
 int32_t alice_kv4_attention(alice_engine* e, const alice_kv4* c, const alice_kv4_batch* b, const alice_buf* q, size_t q_stride, alice_buf* out, size_t out_stride,
                             const alice_buf* rope, uint32_t rot_dims, uint32_t neox, float scale);
 
