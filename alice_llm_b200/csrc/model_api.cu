@@ -131,8 +131,9 @@ int32_t alice_model_log_probs(alice_model* m, const uint32_t* tokens, uint32_t n
     if (top > alice::LOGP_MAX_TOP || top > m->vocab) return alice_fail(ALICE_E_SHAPE, "%s: %u alternatives; up to %u, and no more than %u tokens", who, top, alice::LOGP_MAX_TOP, m->vocab);
     if (n && top && (!top_ids || !top_log_probs)) return alice_fail(ALICE_E_INVALID, "%s: %u alternatives without room for them", who, top);
     if (n == 0) return ALICE_OK;
-    for (uint32_t i = 0; i < n; i++)
-        if (targets[i] >= m->vocab) return alice_fail(ALICE_E_INVALID, "%s: target %u >= vocab %u", who, targets[i], m->vocab);
+    for (uint32_t i = 0; i < n; i++)      // of all pieces, before the first of them moves the position
+        if (tokens[i] >= m->vocab || targets[i] >= m->vocab)
+            return alice_fail(ALICE_E_INVALID, "%s: %s %u >= vocab %u", who, tokens[i] >= m->vocab ? "token" : "target", tokens[i] >= m->vocab ? tokens[i] : targets[i], m->vocab);
     MCU(cudaSetDevice(m->e->device));
     int rc = check_room(m, n, who);
     if (rc) return rc;

@@ -217,3 +217,20 @@ def test_refusals(eng):
         assert ei.value.code == code
     assert gm.position() == 0 and np.isfinite(gm.forward_and_read(1)).all()
     gm.free()
+
+
+def test_a_refused_text_moves_nothing(eng):
+    """A token that is none in the last piece of a text: no piece before it has been taken either."""
+    from alice_llm_b200.gpu import GpuModel
+    gm = GpuModel.load(eng, synth.make_llama(np.random.default_rng(8), CFG), kv_cache="q4")
+    text = np.arange(600) % CFG["vocab_size"]
+    gm.forward(5)
+    before = [x.copy() for x in gm.kv_read(1, 0, 1)]
+    for bad in (599, 300, 0):
+        wrong = text.copy()
+        wrong[bad] = CFG["vocab_size"]
+        with pytest.raises(_lib.AliceError) as ei:
+            gm.log_probs(wrong, text)
+        assert ei.value.code == _lib.E_INVALID and gm.position() == 1
+    assert all(np.array_equal(a, b) for a, b in zip(before, gm.kv_read(1, 0, 1)))
+    gm.free()
