@@ -137,6 +137,15 @@ def keys_and_values(gen, tokens, kv_heads, dim):
     return k, v
 
 
+def _engine():
+    """The one engine of a program, on the stream of its tensors."""
+    from alice_llm_b200.gpu import GpuEngine
+    if not hasattr(_engine, "one"):
+        _engine.one = GpuEngine()
+    _engine.one.set_stream(torch.cuda.current_stream().cuda_stream)
+    return _engine.one
+
+
 def prepare(case, seed):
     gen = torch.Generator(device=DEV)
     gen.manual_seed(seed)
@@ -164,9 +173,7 @@ def prepare(case, seed):
         k, v = keys_and_values(gen, pages * page, kh, dim)
         st["kc"], st["vc"] = _in_codes(k), _in_codes(v)           # what the pages hold: [pages * page, kv heads, ...]
     if own:
-        from alice_llm_b200.gpu import GpuEngine
-        e = GpuEngine()
-        e.set_stream(torch.cuda.current_stream().cuda_stream)
+        e = _engine()
         wrap = lambda t: e.buf_from_device(t.data_ptr(), t.numel())  # noqa: E731
         cache = e.kv4_cache(pages, page, kh, dim)
         batch = e.kv4_batch(cache, case.get("heads", kh), len(past), sum(tokens), wide)
@@ -198,9 +205,7 @@ def _prepare_log_probs(case, gen):
     target = torch.where(likely, x.argmax(1), torch.randint(0, v, (n,), generator=gen, device=DEV)).to(torch.int32)
     st = dict(case=case, x=x, target=target)
     if own:
-        from alice_llm_b200.gpu import GpuEngine
-        e = GpuEngine()
-        e.set_stream(torch.cuda.current_stream().cuda_stream)
+        e = _engine()
         wrap = lambda t: e.buf_from_device(t.data_ptr(), t.numel())  # noqa: E731
         st["lp"], st["entropy"] = torch.empty(n, device=DEV), torch.empty(n, device=DEV)
         st["rank"] = torch.empty(n, dtype=torch.int32, device=DEV)
