@@ -16,11 +16,12 @@
 // Weighted sums go to f32 sums every 8 tiles: products on tensor cores add up with less than f32 rounding, which over a long chain would add up itself. What is
 // added up until then is of one magnitude: its weights have a reference of their own, the largest score of its first tiles, which moves when a score exceeds it by 2^8 or
 // when the next sums begin with all of a row's 2^8 below it, and its steps lie within 2^8 (what is heavier, or larger, and comes elsewhere takes no bits from it). Where the
-// steps of two tiles side by side lie further apart (a block of zeros with a weight counts too), these tiles' products are made in f32 by the ordinary pipes. One power of two
-// for all blocks and for all that came before, as it was at first, took 64 us instead of 67 for the row below, and with values 2^20 apart was 1 to 5 % off.
+// steps of two tiles side by side lie further apart (a block of zeros with a weight counts too), these tiles' products are made in f32 by the ordinary pipes: 270 us where that is
+// so in all of 131008 positions. One power of two for all blocks and for all that came before took 64 us instead of 69 there, and with values 2^20 apart was 1 to 5 % off.
 //
-// Bound by issue: a product takes 8 clocks of an SM quarter beside which little else runs, and unpacking as long again. Measured, heads of 128: one token of 64 x 8
-// heads behind 131007 positions (168 MB) 64 us, one each of 64 users with 32 x 8 heads behind up to 4095 57 us.
+// Bound by latency with few warps: two (R = 4: three) a quarter of an SM by registers, issue slots 47 % (57), tensor pipe 24 % (16), stalls led by fixed latencies of dependent
+// instructions; start, merges and the join are 12 to 15 us of a large call. Measured, heads of 128: one token of 64 x 8 heads behind 131007 positions (168 MB) 69 us, one each
+// of 64 users with 32 x 8 heads behind up to 4095 61 us.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -40,8 +41,8 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 constexpr int STAGES = 4;
-constexpr uint32_t FLUSH = 8;        // tiles (131008 positions: 4 tiles 1.6e-6 off and 71.8 us, 8 1.9e-6 and 66.2, 16 2.7e-6 and 64.2)
-constexpr float ROOM = 8.0f;         // what a score may exceed the reference by, in powers of two
+constexpr uint32_t FLUSH = 8;        // tiles (131008 positions: 4 tiles 1.2e-6 off and 76 us, 8 1.6e-6 and 69.6, 16 2.4e-6 and 67.8)
+constexpr float ROOM = 8.0f;         // what a score may exceed the reference by, and what all scores of a row may be below it, in powers of two
 constexpr float LIFT = 7.0f;         // weights are 2^7 times as large as they are (sums of them too): up to 2^15
 
 // Parts of a row's sums brought to one reference, N at a time.
@@ -517,6 +518,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                     const uint32_t vsrow = base[x] + kv4_v_scales(DIM) + g * (4 * NB);
                     va[x] = lds_words<NB>(vsrow); vb[x] = lds_words<NB>(vsrow + 32 * NB);
                 }
+                bool begin_anew = false;         // what is held goes to shared memory first, and these tiles are looked at again
                 auto weights = [&](auto edge_t) {
                     constexpr bool edge = decltype(edge_t)::value;       // some row does not see all of the tiles
                     bool move = false;
@@ -572,31 +574,34 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         again = __any_sync(0xffffffffu, move || outside());
                     }
                     if (again) {
-                        if (held) flush();
+                        if (held) { begin_anew = true; return; }
+                        // A block by each of NB lanes. To below 1, with weights up to 2^15 then in range: by 2^(14 - e), e the exponent field that is the last within. That of the
+                        // largest step is the one before, and the least is 2^-8 then. Of the steps below 2^-8 (fields 0 to 6) the least is 2^-4 to 2^-6 of the largest, and
+                        // 2^-11 then.
+                        uint32_t d = 0;
 #pragma unroll
                         for (int b = 0; b < NB / 2; b++) {
-                            uint32_t top = hi[b], scale = 0;
+                            uint32_t top = hi[b];
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            // To below 1, with weights up to 2^15 then in range: by 2^(14 - e), e the exponent field that is the last within. That of the largest step is the
-                            // one before, and the least is 2^-8 then. Of the steps below 2^-8 (fields 0 to 6) the least is 2^-4 to 2^-6 of the largest, and 2^-11 then.
-                            least_d[b] = too_far[b] = 0;
-                            if (b % 2 == 0) last_e[b / 2] = 0;
+                            if (lane / 2 % (NB / 2) == b) d = lane & 1 ? top >> 16 : top & 0xffff;
+                        }
+                        const uint32_t field = d >> 10;
+                        uint32_t e = field + 1, least = (field - 6) << 10, far_bits = 0xe000;
+                        if (field < 7) {
+                            e = field >= 4 ? 8 : field >= 2 ? 4 : field + 1;
+                            least = field >= 4 ? 512 : field >= 2 ? 64 : field ? 16 : max(d >> 6, 1u);
+                            far_bits = field >= 4 ? 0xe000 : field >= 2 ? 0xf000 : field ? 0xf800 : 0xfc00;
+                            if (!d) { least = NO_STEP & 0xffff; far_bits = 0xe000; }
+                        }
+                        const uint32_t range = least | far_bits << 16, power = (e <= 28 ? (29 - e) << 10 : 0x400u >> (e - 28)) | e << 16;
 #pragma unroll
-                            for (int k = 0; k < 2; k++) {
-                                const uint32_t d = top >> 16 * k & 0xffff, field = d >> 10;
-                                uint32_t e, least, far_bits = 0xe000;
-                                if (!d) { e = 0; least = NO_STEP & 0xffff; }
-                                else if (field >= 7) { e = field + 1; least = (field - 6) << 10; }
-                                else if (field >= 4) { e = 8; least = 512; }
-                                else if (field >= 2) { e = 4; least = 64; far_bits = 0xf000; }
-                                else if (field == 1) { e = 2; least = 16; far_bits = 0xf800; }
-                                else { e = 1; least = max(d >> 6, 1u); far_bits = 0xfc00; }
-                                least_d[b] |= least << 16 * k; too_far[b] |= far_bits << 16 * k;
-                                last_e[b / 2] |= e << 8 * (2 * (b % 2) + k);
-                                scale |= (e <= 28 ? (29 - e) << 10 : 0x400u >> (e - 28)) << 16 * k;
-                            }
-                            dscale[b] = bits_half2(scale);
+                        for (int b = 0; b < NB / 2; b++) {
+                            const uint32_t r0 = __shfl_sync(0xffffffffu, range, 2 * b), r1 = __shfl_sync(0xffffffffu, range, 2 * b + 1), p0 = __shfl_sync(0xffffffffu, power, 2 * b),
+                                           p1 = __shfl_sync(0xffffffffu, power, 2 * b + 1);
+                            least_d[b] = __byte_perm(r0, r1, 0x5410); too_far[b] = __byte_perm(r0, r1, 0x7632); dscale[b] = bits_half2(__byte_perm(p0, p1, 0x5410));
+                            const uint32_t es = (p0 >> 16 | p1 >> 16 << 8) << 16 * (b % 2);
+                            last_e[b / 2] = b % 2 ? last_e[b / 2] | es : es;
                         }
 #pragma unroll
                         for (int i = 0; i < RT; i++) {
@@ -609,38 +614,38 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         }
                         if (__any_sync(0xffffffffu, outside())) {
                             // Steps too far apart for one power of two: in f32 and without products, by the lanes that have the sums of these rows and dims.
-                            flush();                 // nothing is held: the sums' reference
-                            const uint32_t steps = kv4_v_scales(DIM), v_codes = kv4_v_codes(DIM) + g * (2 * NB);
-                            float f[RT];
-#pragma unroll
-                            for (int i = 0; i < RT; i++) f[i] = ref[i] == mref[i] ? 1.0f : ex2(ref[i] - mref[i]);
-#pragma unroll
-                            for (int x = 0; x < TP; x++)
-#pragma unroll
-                                for (uint32_t k = 0; k < 2; k++) {
-                                    float p[RT];
-#pragma unroll
-                                    for (int i = 0; i < RT; i++) p[i] = edge && key + 16 * x + 8 * k >= limit[i] ? 0.0f : f[i] * ex2(fmaf(s[x][i][k], factor[i], LIFT - ref[i]));
 #pragma unroll 1
-                                    for (uint32_t b = 0; b < NB; b++) {
-                                        float4 o[RT];
+                            for (uint32_t xk = 0; xk < 2 * TP; xk++) {
+                                const uint32_t x = xk >> 1, k = xk & 1, tile = ring + (stage + x) % STAGES * TILE;
+                                float p[RT];
 #pragma unroll
-                                        for (int i = 0; i < RT; i++) o[i] = mine[(i * NB + b) * 32];
+                                for (int i = 0; i < RT; i++) {
+                                    float v = k ? s[0][i][1] : s[0][i][0];
+                                    if (TP == 2 && x) v = k ? s[TP - 1][i][1] : s[TP - 1][i][0];
+                                    p[i] = edge && key + 8 * xk >= limit[i] ? 0.0f : ex2(fmaf(v, factor[i], LIFT - ref[i]));
+                                }
 #pragma unroll 1
-                                        for (uint32_t j = 0; j < 8 && key0 + 16 * x + 8 * k + j < far; j++) {
-                                            const uint32_t row = kv4_row(j), codes = lds16(base[x] + v_codes + (8 * k + j) * (DIM / 2) + b * 2);
-                                            const float d = f16_bits_to_f32(lds16(base[x] + steps + (8 * k + row) * (4 * NB) + b * 2));
+                                for (uint32_t j = 0; j < 8 && key0 + 8 * xk + j < far; j++) {
+                                    const uint32_t row = kv4_row(j);
+                                    const Words<(NB + 1) / 2> codes = lds_words<(NB + 1) / 2>(tile + kv4_v_codes(DIM) + (8 * k + j) * (DIM / 2) + g * (2 * NB));
+                                    const Words<NB / 2> d = lds_words<NB / 2>(tile + kv4_v_scales(DIM) + (8 * k + row) * (4 * NB));
 #pragma unroll
-                                            for (int i = 0; i < RT; i++) {
-                                                const float w = __shfl_sync(0xffffffffu, p[i], 4 * row + t) * d;
-                                                o[i].x = fmaf(w, (float)(codes & 15) - 8.0f, o[i].x); o[i].y = fmaf(w, (float)(codes >> 4 & 15) - 8.0f, o[i].y);
-                                                o[i].z = fmaf(w, (float)(codes >> 8 & 15) - 8.0f, o[i].z); o[i].w = fmaf(w, (float)(codes >> 12) - 8.0f, o[i].w);
+                                    for (int i = 0; i < RT; i++) {
+                                        const float w = __shfl_sync(0xffffffffu, p[i], 4 * row + t);
+#pragma unroll
+                                        for (int b = 0; b < NB; b++) {
+                                            const float wd = w * half_of(d, b);
+#pragma unroll
+                                            for (int c = 0; c < 4; c++) {
+                                                float& sum = acc[SPLIT ? 0 : i >> 1][b][c >> 1][c % 2 * 2 + (SPLIT ? 0 : i & 1)];
+                                                sum = fmaf(wd, (float)(codes.w[b / 2] >> (16 * (b & 1) + 4 * c) & 15) - 8.0f, sum);
                                             }
                                         }
-#pragma unroll
-                                        for (int i = 0; i < RT; i++) mine[(i * NB + b) * 32] = o[i];
                                     }
                                 }
+                            }
+#pragma unroll
+                            for (int b = 0; b < NB; b += 4) last_e[b / 4] = 0x0e0e0e0eu;      // as they are
                             no_steps();              // no part in the products
                             held = FLUSH;            // and what comes next is by itself
                         }
@@ -673,77 +678,78 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         }
                 };
                 if (key0 + KV4_TILE * TP > least) weights(std::true_type{}); else weights(std::false_type{});
-                // ---- values: weight times step as a pair of half-precision numbers, from the weight's pair ----
+                if (!begin_anew) {
+                    // ---- values: weight times step as a pair of half-precision numbers, from the weight's pair ----
 #pragma unroll
-                for (int x = 0; x < TP; x++) {
-                    Words<(NB + 1) / 2> v[4];
-                    const uint32_t vrow = base[x] + kv4_v_codes(DIM) + t * (DIM / 2) + g * (2 * NB);
+                    for (int x = 0; x < TP; x++) {
+                        Words<(NB + 1) / 2> v[4];
+                        const uint32_t vrow = base[x] + kv4_v_codes(DIM) + t * (DIM / 2) + g * (2 * NB);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = lds_words<(NB + 1) / 2>(vrow + i * 2 * DIM);
-                    __half2 ph[NT][2], pl[NT][2];       // of two rows, or of one twice
+                        for (int i = 0; i < 4; i++) v[i] = lds_words<(NB + 1) / 2>(vrow + i * 2 * DIM);
+                        __half2 ph[NT][2], pl[NT][2];       // of two rows, or of one twice
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                        for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const float p0 = s[x][SPLIT ? 0 : 2 * n % RT][k], p1 = s[x][SPLIT ? 0 : (2 * n + 1) % RT][k];
-                            ph[n][k] = __floats2half2_rn(p0, p1);
-                            const float2 back = __half22float2(ph[n][k]);
-                            pl[n][k] = __floats2half2_rn(p0 - back.x, p1 - back.y);
-                        }
+                            for (int k = 0; k < 2; k++) {
+                                const float p0 = s[x][SPLIT ? 0 : 2 * n % RT][k], p1 = s[x][SPLIT ? 0 : (2 * n + 1) % RT][k];
+                                ph[n][k] = __floats2half2_rn(p0, p1);
+                                const float2 back = __half22float2(ph[n][k]);
+                                pl[n][k] = __floats2half2_rn(p0 - back.x, p1 - back.y);
+                            }
 #pragma unroll
-                    for (int b2 = 0; b2 < NB / 2; b2++) {
-                        const __half2 d2[2] = {__hmul2(bits_half2(va[x].w[b2]), dscale[b2]), __hmul2(bits_half2(vb[x].w[b2]), dscale[b2])};
-                        Codes ca[2], cb[2];
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const uint32_t pick = u ? 0x7632u : 0x5410u;
-                            ca[u] = unpack<8>(__byte_perm(v[0].w[b2], v[1].w[b2], pick));
-                            cb[u] = unpack<8>(__byte_perm(v[2].w[b2], v[3].w[b2], pick));
-                        }
-                        // w1 = p d to half precision, w2 = what is missing: p's value times d less w1 is exact
-                        auto product = [](__half2 hi, __half2 lo, __half2 d, __half2& w1, __half2& w2) {
-                            w1 = __hmul2(hi, d);
-                            w2 = __hfma2(lo, d, __hfma2(hi, d, __hneg2(w1)));
-                        };
-                        if (SPLIT) {
-                            __half2 w1[2], w2[2];
-#pragma unroll
-                            for (int k = 0; k < 2; k++) product(ph[0][k], pl[0][k], d2[k], w1[k], w2[k]);
+                        for (int b2 = 0; b2 < NB / 2; b2++) {
+                            const __half2 d2[2] = {__hmul2(bits_half2(va[x].w[b2]), dscale[b2]), __hmul2(bits_half2(vb[x].w[b2]), dscale[b2])};
+                            Codes ca[2], cb[2];
 #pragma unroll
                             for (int u = 0; u < 2; u++) {
                                 const uint32_t pick = u ? 0x7632u : 0x5410u;
-                                const uint32_t b0 = transposed(__byte_perm(half2_bits(w1[0]), half2_bits(w2[0]), pick)), b1 = transposed(__byte_perm(half2_bits(w1[1]), half2_bits(w2[1]), pick));
-                                mma_f16(acc[0][2 * b2 + u][0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], b0, b1);
-                                mma_f16(acc[0][2 * b2 + u][1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], b0, b1);
+                                ca[u] = unpack<8>(__byte_perm(v[0].w[b2], v[1].w[b2], pick));
+                                cb[u] = unpack<8>(__byte_perm(v[2].w[b2], v[3].w[b2], pick));
                             }
-                        } else {
+                            // w1 = p d to half precision, w2 = what is missing: p's value times d less w1 is exact
+                            auto product = [](__half2 hi, __half2 lo, __half2 d, __half2& w1, __half2& w2) {
+                                w1 = __hmul2(hi, d);
+                                w2 = __hfma2(lo, d, __hfma2(hi, d, __hneg2(w1)));
+                            };
+                            if (SPLIT) {
+                                __half2 w1[2], w2[2];
 #pragma unroll
-                            for (int u = 0; u < 2; u++)
+                                for (int k = 0; k < 2; k++) product(ph[0][k], pl[0][k], d2[k], w1[k], w2[k]);
 #pragma unroll
-                                for (int n = 0; n < NT; n++) {
-                                    __half2 w1[2], w2[2];
-#pragma unroll
-                                    for (int k = 0; k < 2; k++) product(ph[n][k], pl[n][k], u ? __high2half2(d2[k]) : __low2half2(d2[k]), w1[k], w2[k]);
-                                    float (&o)[2][4] = acc[n][2 * b2 + u];
-                                    const uint32_t b0 = transposed(half2_bits(w1[0])), b1 = transposed(half2_bits(w1[1])), e0 = transposed(half2_bits(w2[0])), e1 = transposed(half2_bits(w2[1]));
-                                    mma_f16(o[0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], b0, b1);
-                                    mma_f16(o[1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], b0, b1);
-                                    mma_f16(o[0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], e0, e1);
-                                    mma_f16(o[1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], e0, e1);
+                                for (int u = 0; u < 2; u++) {
+                                    const uint32_t pick = u ? 0x7632u : 0x5410u;
+                                    const uint32_t b0 = transposed(__byte_perm(half2_bits(w1[0]), half2_bits(w2[0]), pick)), b1 = transposed(__byte_perm(half2_bits(w1[1]), half2_bits(w2[1]), pick));
+                                    mma_f16(acc[0][2 * b2 + u][0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], b0, b1);
+                                    mma_f16(acc[0][2 * b2 + u][1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], b0, b1);
                                 }
+                            } else {
+#pragma unroll
+                                for (int u = 0; u < 2; u++)
+#pragma unroll
+                                    for (int n = 0; n < NT; n++) {
+                                        __half2 w1[2], w2[2];
+#pragma unroll
+                                        for (int k = 0; k < 2; k++) product(ph[n][k], pl[n][k], u ? __high2half2(d2[k]) : __low2half2(d2[k]), w1[k], w2[k]);
+                                        float (&o)[2][4] = acc[n][2 * b2 + u];
+                                        const uint32_t b0 = transposed(half2_bits(w1[0])), b1 = transposed(half2_bits(w1[1])), e0 = transposed(half2_bits(w2[0])), e1 = transposed(half2_bits(w2[1]));
+                                        mma_f16(o[0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], b0, b1);
+                                        mma_f16(o[1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], b0, b1);
+                                        mma_f16(o[0], ca[u].v[0], ca[u].v[1], cb[u].v[0], cb[u].v[1], e0, e1);
+                                        mma_f16(o[1], ca[u].v[2], ca[u].v[3], cb[u].v[2], cb[u].v[3], e0, e1);
+                                    }
+                            }
                         }
                     }
-                }
-                __syncwarp();
-                ask(stage);
-                stage = (stage + 1) % STAGES; at++; held++; key0 += KV4_TILE;
-                if (TP == 2 && at < end) {
+                    __syncwarp();
                     ask(stage);
                     stage = (stage + 1) % STAGES; at++; held++; key0 += KV4_TILE;
+                    if (TP == 2 && at < end) {
+                        ask(stage);
+                        stage = (stage + 1) % STAGES; at++; held++; key0 += KV4_TILE;
+                    }
                 }
-                if (held >= FLUSH) flush();
+                if (begin_anew || held >= FLUSH || at >= end) flush();
             }
-            if (held) flush();
 
             if (has_first && has_last) {        // all of the job: out it goes
 #pragma unroll
