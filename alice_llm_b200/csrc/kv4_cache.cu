@@ -133,7 +133,8 @@ __device__ __forceinline__ Held held(const Eight& x, const Eight& y, const Eight
 }  // namespace
 
 // Keys and values of a step into their pages. A warp's heads share the token's place and angles. 5470 tokens of 8 heads of 128 (52 MB read
-// and written): 26.6 us, bound by its instructions; one head a warp takes 36, three CTAs an SM (80 registers) 30, all in f64 66.
+// and written): 26.6 us, bound by latency: rows are asked for when those before are stored, for lack of registers (issue slots 54 %, 4.8 of the stalls an issue wait for
+// loads); one head a warp takes 36, three CTAs an SM (80 registers) 30, all in f64 66.
 template <int NB>
 __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const __grid_constant__ Kv4RowsArgs a) {
     using W = Walk<NB>;
@@ -206,7 +207,8 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const __grid_constan
     }
 }
 
-// And out again: m + d * code, one rounding. Bound by what it writes: 5470 tokens of 8 heads of 128 (45 MB) 13.0 us.
+// And out again: m + d * code, one rounding. 5470 tokens of 8 heads of 128 (45 MB of rows written, which stay in L2) 13.0 us, bound by latency: 7.4 stalls an issue wait for
+// codes and scales of 2 and 4 bytes a lane, issue slots 51 %.
 template <int NB>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4RowsArgs a) {
     using W = Walk<NB>;

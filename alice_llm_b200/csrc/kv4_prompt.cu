@@ -5,6 +5,8 @@
 // remainder, 22 bits; d * (code - 8) has 15) and a product three of them: value value, value remainder, remainder value. The second part is the same for
 // the 32 dims of a block, so it is a few more columns of the operand, against the sums of a block's queries in one product and with sums of its
 // own in the other. Of 256 keys both are scaled by a power of two to below 2^15: what is 2^18 and more below the largest of them has fewer than 22 bits, 2^-40 of that largest.
+// Weights are 2^7 to 2^15 at a row's largest: those 2^-10 and less of it have fewer than 22 bits, 2^-31 of it. (Values 2^20 times as large as the others with weights of 1e-10: 4e-6 off,
+// 2^30 times 4e-3; a key without a value that has all but 1e-7 of the weight: 4e-4. csrc/kv4_attn.cu has no such limits.)
 //
 // Twenty warps: one brings tiles of the pool (bulk copies, a ring of four blocks), one looks their scales over ahead of that (largest magnitude, NaN), four and four
 // turn codes of keys and of values into operands in shared memory (2 instructions a number in half precision), two issue the products of the one and the other kind,
@@ -13,7 +15,7 @@
 // blocks add up in tensor memory and go to registers then, in f32: over a long chain the tensor cores' sums would be further off than f32's. The
 // reference of the weights moves as in csrc/kv4_attn.cu; what has been summed up in tensor memory moves with it.
 //
-// Measured: 2048 tokens x 32 heads of 128 (8 of keys) behind 1021 positions 227 us (the products alone: 124 at the measured bf16 rate; jobs of 16 rows on
+// Measured: 2048 tokens x 32 heads of 128 (8 of keys) behind 1021 positions 210 us (the products alone: 124 at the measured bf16 rate; jobs of 16 rows on
 // mma.sync: 715). A block takes 2600 clocks, the products 1630 of them: what is lost are the hand-overs from warps to warps. With operand warps that load from the pool
 // themselves it was 667 us, with one warp a row, one for all products and every block's sums to registers 252, with warps that make both operands 6 us more.
 //
@@ -602,8 +604,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_prompt_kernel(const __grid_con
 }
 
 namespace {
-// Parts of the keys of a job (a cluster): those with which clusters side by side, one after the other, take the least time. A cluster's start and join are as long as
-// eight blocks of keys (2048 tokens of 32 x 8 heads: 9 of 95 us a CTA).
+// Parts of the keys of a job (a cluster): those with which clusters side by side, one after the other, take the least time. A cluster's start and join are counted as
+// eight blocks of keys of 2600 clocks (2048 tokens of 32 x 8 heads: the start is 14 to 18 thousand of a CTA's 95 thousand clocks).
 uint32_t parts_of(uint32_t clusters, uint32_t blocks, const int (&at_once)[9]) {
     uint32_t best = 1;
     uint64_t least = ~0ull;
