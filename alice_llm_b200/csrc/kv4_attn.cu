@@ -383,12 +383,13 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                         for (int c = 0; c < 4; c++) acc[n][b][u][c] = 0;
             // Steps in acc, by block of dims (two to a register): as half-precision bits less `least_d` they have none of the bits `too_far`; 2^(14 - e) that they are
             // multiplied by, e in bytes of last_e.
-            constexpr uint32_t NO_STEP = 0xe001e001u, FAR = 0xe000e000u;      // 0 and nothing else
+            // A borrow of the lower half is one that is too far itself, or from NO_STEP, and then the upper half is taken one higher than it is: no harm at its ends.
+            constexpr uint32_t NO_STEP = 0xe001e001u, NOTHING = 0x7fff7fffu, FAR = 0xe000e000u;      // 0 and nothing else; no step at all
             uint32_t least_d[NB / 2], too_far[NB / 2], last_e[NB / 4 ? NB / 4 : 1];
             __half2 dscale[NB / 2];
             auto no_steps = [&]() {
 #pragma unroll
-                for (int b = 0; b < NB / 2; b++) { least_d[b] = NO_STEP; too_far[b] = FAR; dscale[b] = __float2half2_rn(0.0f); }
+                for (int b = 0; b < NB / 2; b++) { least_d[b] = NOTHING; too_far[b] = FAR; dscale[b] = __float2half2_rn(0.0f); }
             };
             no_steps();
 #pragma unroll
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(Cfg<NB, R>::WARPS * 32, 1) kv4_attn_kernel(con
                                 uint32_t& d = (k ? vb : va)[x].w[b];
                                 const bool none = edge && key + 16 * x + 8 * k >= far;      // keys that no row sees: whatever lies there has no part
                                 if (none) d = 0;
-                                beyond[b] |= none ? 0 : d - least_d[b];                     // a borrow is of a half that is too far itself
+                                beyond[b] |= none ? 0 : d - least_d[b];
                             }
                     uint32_t hi[NB / 2], lo[NB / 2];
                     auto outside = [&]() {

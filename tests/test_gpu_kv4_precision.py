@@ -164,3 +164,117 @@ def test_steps_at_the_ends_of_half_precision(engine):
             s = Step(engine, 4, 2, 128, 16, [500], [1], k=[k], v=[v])
             s.fill()
             check(s)
+
+
+# ---- the same with many tiles a warp ---------------------------------------------------------------------------------------------------
+
+
+def check_many(e, group, k, v, q, tokens, copies=300):
+    """`copies` sequences over the same pages but for their last one (their new tokens), which all have the rows and queries of one: every warp goes through a
+    dozen tiles and more, through the ends of sequences and their beginnings."""
+    past, dim = len(k) - tokens, k.shape[-1]
+    assert past % 16 == 0 and tokens <= 16
+    shared = past // 16
+    cache = e.kv4_cache(shared + copies, 16, 2, dim)
+    batch = e.kv4_batch(cache, 2 * group, copies, max(past, copies * tokens), shared + 1)
+    order = np.random.default_rng(0).permutation(shared + copies)
+    tables = np.concatenate([np.tile(order[:shared], (copies, 1)), order[shared:, None]], 1)
+    batch.set([0], [past], tables[:1])
+    e.kv4_append(cache, batch, e.upload_f32(k[:past]), e.upload_f32(v[:past]))
+    batch.set([past] * copies, [tokens] * copies, tables)
+    e.kv4_append(cache, batch, *(e.upload_f32(np.tile(x[past:], (copies, 1, 1))) for x in (k, v)))
+    out = e.alloc_f32(copies * q.size)
+    e.kv4_attention(cache, batch, e.upload_f32(np.tile(q, (copies, 1, 1))), out, dim ** -0.5)
+    got = e.read_f32(out).reshape(copies, *q.shape)
+    kc, vc = ref.quantize(k.astype(np.float64)), ref.quantize(v.astype(np.float64))
+    want, w = ref.attention(q.astype(np.float64), ref.values(*kc), ref.values(*vc), past, dim ** -0.5)
+    tol = ref.rms_tolerance(q, q, np.zeros_like(q), kc, vc, w, past, dim ** -0.5)
+    off = np.abs(got - want)
+    assert (off <= tol).all(), f"worst {np.max(off / tol):.3g} of the tolerance, in {np.mean((off > tol).any((1, 2, 3))):.3g} of the sequences"
+    batch.free()
+    cache.free()
+
+
+def ordinary(rng, tokens, group, dim):
+    return rng.normal(size=(tokens, 2 * group, dim)).astype(np.float32)
+
+
+MANY = [(1, 1, 64), (7, 1, 64), (4, 3, 64), (1, 1, 128), (4, 1, 128), (7, 1, 128), (4, 3, 128), (1, 1, 256), (7, 1, 256)]
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+def test_many_ordinary(engine, group, tokens, dim):
+    rng = np.random.default_rng(1)
+    k, v = plain(rng, 704, tokens, dim)
+    check_many(engine, group, k * np.float32(2), v, ordinary(rng, tokens, group, dim), tokens)
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+def test_many_scores_that_rise_and_fall(engine, group, tokens, dim):
+    """References that move up and down: by waves, by steps, at single keys."""
+    n = 704 + tokens
+    for shape in (np.linspace(0, 60, n), np.linspace(60, 0, n), 30 * np.sin(np.arange(n) / 40), np.where(np.arange(n) % 100 == 7, 25, 0), np.where(np.arange(n) // 150 % 2, 20, 0)):
+        rng = np.random.default_rng(2)
+        q, k = scored(rng, 704, tokens, dim, np.arange(n), shape[:, None, None].astype(np.float32), group)
+        _, v = plain(rng, 704, tokens, dim)
+        check_many(engine, group, k, v, q, tokens)
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+@pytest.mark.parametrize("far", [8, 16, 30])
+def test_many_blocks_of_a_head_far_apart(engine, group, tokens, dim, far):
+    rng = np.random.default_rng(far)
+    k, v = plain(rng, 704, tokens, dim)
+    apart = np.array([0, far, far // 2, 2] * 2)[:dim // 32]
+    v *= np.repeat(np.stack([2.0 ** (8 - apart), 2.0 ** (8 - apart[::-1])]), 32, 1).astype(np.float32)
+    check_many(engine, group, k, v, ordinary(rng, tokens, group, dim), tokens)
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+@pytest.mark.parametrize("far", [16, 20, 30])
+@pytest.mark.parametrize("at", [[0], [350], [0, 100, 101, 500], list(range(32, 64)), list(range(64, 400, 3)), list(range(0, 704, 50))])
+def test_many_large_values_that_hardly_count(engine, group, tokens, dim, far, at):
+    rng = np.random.default_rng(far)
+    q, k = scored(rng, 704, tokens, dim, at, -23.0, group)
+    _, v = plain(rng, 704, tokens, dim)
+    v *= 2.0 ** -14
+    v[at] *= np.float32(2.0 ** far)
+    check_many(engine, group, k, v, q, tokens)
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+@pytest.mark.parametrize("value", [0.0, 2.0 ** -20, 2.0 ** -9, 2.0 ** -5])
+@pytest.mark.parametrize("at", [[0], [17], [350], [0, 40, 300, 301]])
+def test_many_keys_with_nearly_all_the_weight_and_little_value(engine, group, tokens, dim, value, at):
+    rng = np.random.default_rng(5)
+    q, k = scored(rng, 704, tokens, dim, at, 16.0, group)
+    _, v = plain(rng, 704, tokens, dim)
+    v[at, 0] *= np.float32(value)
+    v[at, 1, 32:64] *= np.float32(value)
+    check_many(engine, group, k, v, q, tokens)
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+def test_many_tiles_of_every_magnitude(engine, group, tokens, dim):
+    """Steps that grow, shrink and jump from tile to tile, over all that half precision has; zeros among them."""
+    n = 704 + tokens
+    tile = np.arange(n) // 16
+    for e in (tile / 2 - 20, 2 - tile / 2, (tile * 7) % 29 - 18, np.where(tile % 5 == 0, 3, -12), np.where(np.arange(n) % 24 == 0, -np.inf, tile % 9)):
+        rng = np.random.default_rng(6)
+        k, v = plain(rng, 704, tokens, dim)
+        v *= (2.0 ** e)[:, None, None].astype(np.float32)
+        check_many(engine, group, k, v, ordinary(rng, tokens, group, dim), tokens)
+
+
+@pytest.mark.parametrize("group,tokens,dim", MANY)
+def test_many_least_steps_behind_steps_far_apart(engine, group, tokens, dim):
+    """Odd blocks of 32 dims have steps of 2^-24 throughout; the others are zero but for the first two tiles of one, where they lie far apart."""
+    rng = np.random.default_rng(7)
+    k, v = plain(rng, 704, tokens, dim)
+    k *= 0.1
+    blocks = v.reshape(len(v), 2, dim // 32, 32)
+    blocks[:, :, 1::2] = rng.integers(0, 16, blocks[:, :, 1::2].shape) * 2.0 ** -24
+    blocks[:, :, 1::2, 0], blocks[:, :, 1::2, 1] = 0, 15 * 2.0 ** -24
+    blocks[:, :, 0::2] = 0
+    blocks[:32, :, 0 if dim == 64 else 2] = rng.normal(size=(32, 2, 32)) * np.where(np.arange(32) % 3 == 0, 2.0 ** -20, 1.0)[:, None, None]
+    check_many(engine, group, k, v, ordinary(rng, tokens, group, dim), tokens)
