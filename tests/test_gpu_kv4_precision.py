@@ -278,3 +278,38 @@ def test_many_least_steps_behind_steps_far_apart(engine, group, tokens, dim):
     blocks[:, :, 0::2] = 0
     blocks[:32, :, 0 if dim == 64 else 2] = rng.normal(size=(32, 2, 32)) * np.where(np.arange(32) % 3 == 0, 2.0 ** -20, 1.0)[:, None, None]
     check_many(engine, group, k, v, ordinary(rng, tokens, group, dim), tokens)
+
+
+# ---- jobs of 128 rows -------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", ["flat", "up", "down", "waves", "peaks", "steps"])
+def test_prompts_behind_long_contexts(engine, dim, shape):
+    """Numbers of one magnitude, references that move up and stay: dozens of blocks of keys, several to a part of the keys."""
+    group, tokens, past = 2, 24, 3000
+    n = np.arange(past + tokens)
+    rng = np.random.default_rng(8)
+    if shape == "flat":
+        k, v = plain(rng, past, tokens, dim)
+        q = ordinary(rng, tokens, group, dim)
+    else:
+        lead = {"up": n / 60, "down": 50 - n / 60, "waves": 12 * np.sin(n / 90), "peaks": np.where(n % 400 == 7, 12, 0), "steps": np.where(n // 500 % 2, 8, 0)}[shape]
+        q, k = scored(rng, past, tokens, dim, n, lead[:, None, None].astype(np.float32), group)
+        _, v = plain(rng, past, tokens, dim)
+    s = Step(engine, 2 * group, 2, dim, 64, [past], [tokens], seed=8, k=[k], v=[v])
+    s.q = q
+    s.fill()
+    check(s)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompts_with_blocks_of_a_head_far_apart(engine, dim):
+    """Within what one power of two for 256 positions holds: steps 2^16 apart keep 22 bits less two."""
+    group, tokens = 2, 24
+    rng = np.random.default_rng(16)
+    k, v = plain(rng, 700, tokens, dim)
+    v *= np.repeat(2.0 ** -np.array([0, 16, 8, 2])[:dim // 32], 32)[None, None].astype(np.float32)
+    s = Step(engine, 2 * group, 2, dim, 16, [700], [tokens], seed=16, k=[k], v=[v])
+    s.fill()
+    check(s)
